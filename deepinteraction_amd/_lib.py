@@ -9,10 +9,10 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libdeepinteraction_hip.so')
 
-DI_F32, DI_F16, DI_F16_HL = 0, 1, 2
+DI_F32, DI_F16, DI_F16_HL, DI_BF16 = 0, 1, 2, 3
 ABI_VERSION = 2
 
-_c_p, _c_i, _c_f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_c_p, _c_i, _c_f, _c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
 # name -> argtypes, mirrors include/deepinteraction_hip.h one to one
 SIGNATURES = {
@@ -51,6 +51,9 @@ SIGNATURES = {
     'di_polar_bev_sample_fwd': [_c_p] * 7 + [_c_i] * 8 + [_c_p],
     'di_mha_small_fwd': [_c_p, _c_i, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_f, _c_i, _c_p],
     'di_add_layernorm_fwd': [_c_p] * 5 + [ctypes.c_longlong, _c_i, _c_f, _c_i, _c_p],
+    'di_layernorm_fwd': [_c_p, _c_ll, _c_i] * 2 + [_c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_p, _c_p, _c_ll, _c_i, _c_f, _c_p],
+    'di_layernorm_bwd': [_c_p, _c_ll, _c_i, _c_p, _c_ll] + [_c_p, _c_ll, _c_i] * 2 + [_c_p, _c_i, _c_p, _c_p, _c_p, _c_i] + [_c_p] * 4 +
+                        [_c_ll, _c_i, _c_p],
     'di_ms_deform_attn_bwd': [_c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_i, _c_p],
     'di_grid_gather_bwd': [_c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p],
     'di_polar_bev_sample_bwd': [_c_p] * 6 + [_c_i] * 8 + [_c_p],
@@ -96,8 +99,9 @@ SIGNATURES = {
 VALUE_FUNCS = {'di_mha_decode_scratch_floats': [_c_i] * 4, 'di_i2p_key_table_bytes': [_c_i] * 4, 'di_i2p_dense_bytes': [_c_i] * 5, 'di_topk_workspace_bytes': [_c_i] * 3,
                'di_token_splitk_workspace_bytes': [_c_i] * 2, 'di_mha_decode_x_ranges': [_c_i] * 3,
                'di_graph_node_count': [_c_p], 'di_local_attn_ring_timeouts': [_c_p], 'di_bn_workspace_floats': [_c_i],
+               'di_layernorm_bwd_workspace_floats': [_c_ll, _c_i],
                'di_timed_consumed': [], 'di_wgrad_workspace_floats': [ctypes.c_longlong, _c_i, _c_i]}
-_LONGLONG = {'di_i2p_dense_bytes', 'di_wgrad_workspace_floats', 'di_topk_workspace_bytes', 'di_i2p_key_table_bytes', 'di_graph_node_count', 'di_token_splitk_workspace_bytes'}
+_LONGLONG = {'di_layernorm_bwd_workspace_floats', 'di_i2p_dense_bytes', 'di_wgrad_workspace_floats', 'di_topk_workspace_bytes', 'di_i2p_key_table_bytes', 'di_graph_node_count', 'di_token_splitk_workspace_bytes'}
 
 # ---- the step program of di_token_program (structs of include/deepinteraction_hip.h)
 TOK_LOAD, TOK_LOAD_PARTS, TOK_ATTN, TOK_COMBINE, TOK_LINEAR, TOK_ROWOP, TOK_STORE, TOK_HEADS = range(1, 9)

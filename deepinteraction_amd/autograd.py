@@ -6,6 +6,7 @@ predictions, exactly as in the reference (F.grid_sample's grid at encoder_utils.
 data; the RoI boxes come from deep-copied, decoded predictions, decoder_utils.py:672-679)."""
 import torch
 from torch.amp import custom_bwd, custom_fwd
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -166,6 +167,38 @@ class I2PAttention(torch.autograd.Function):
         g_img, g_q = ops.i2p_attention_bwd(img, qfold, grad_ctx, pillars, coors, num_points, proj, aug_rev,
                                            ctx.ori_hw, ctx.dropout_p, ctx.seed, grad_mass=grad_mass)
         return g_img.to(img.dtype), g_q.to(qfold.dtype), None, None, None, None, None, None, None, None, None
+
+
+class AddLayerNorm(torch.autograd.Function):
+    """y = LayerNorm(x + res) (csrc/layernorm.hip, layernorm_bwd.hip; res may be None), or (y, x + res) with `with_sum`: the post-norm
+    and pre-norm steps of a training forward.  x and res are kept, not their sum; with_sum keeps the sum instead."""
+
+    @staticmethod
+    @_fwd
+    def forward(ctx, x, res, weight, bias, eps, out_dtype, with_sum):
+        y, total, mean, rstd = ops.layernorm_train_fwd(x, weight, bias, res, eps, with_sum, out_dtype)
+        ctx.save_for_backward(x if total is None else total, res if total is None else None, weight, mean, rstd)
+        ctx.types = (x.dtype, None if res is None else res.dtype)
+        ctx.set_materialize_grads(False)
+        return (y, total) if with_sum else y
+
+    @staticmethod
+    @once_differentiable
+    @_bwd
+    def backward(ctx, gy, gsum=None):
+        x, res, weight, mean, rstd = ctx.saved_tensors
+        xt, rt = ctx.types
+        need = ctx.needs_input_grad
+        if gy is None:                                   # only the sum went on
+            gx, gw, gb = gsum, None, None
+        else:
+            gx, gres, gw, gb = ops.layernorm_train_bwd(gy, x, weight, mean, rstd, res=res, grad_sum=gsum)
+        if gx is None:
+            return (None,) * 7
+        if gy is None or res is None:
+            gres = None if rt is None else gx.to(rt)
+        return (gx.to(xt) if need[0] else None, gres if need[1] else None, gw if need[2] else None, gb if need[3] else None,
+                None, None, None)
 
 
 # ---------------------------------------------------------------------------------- DeepInteraction++ samplers

@@ -1083,6 +1083,146 @@ def add_layernorm(x, res, weight, bias, eps=1e-5):
     return out
 
 
+# ------------------------------------------------------------------ LayerNorm with its residual add, forward and backward
+_DT3 = {torch.float32: _lib.DI_F32, torch.float16: _lib.DI_F16, torch.bfloat16: _lib.DI_BF16}
+
+
+def _code3(t):
+    try:
+        return _DT3[t if isinstance(t, torch.dtype) else t.dtype]
+    except KeyError:
+        raise TypeError(f'float32, float16 or bfloat16 tensors are supported, got {t if isinstance(t, torch.dtype) else t.dtype}')
+
+
+def _same_device(first, *ts):
+    """Every tensor on the device of the first: a launch goes to THAT device's current stream."""
+    if not first.is_cuda:
+        _dev(first)
+    at = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != at:
+            _dev(t)
+            raise ValueError(f'tensors on {first.device} and {t.device} in one call')
+
+
+def _launch(name, n, t, *args):
+    """`_lib.call` on the device of `t`, on that device's current stream (appended to the arguments)."""
+    at = t.get_device()
+    if at != torch.cuda.current_device():
+        with torch.cuda.device(at):
+            return _launch(name, n, t, *args)
+    if PROFILE is None:
+        return _lib.call('di_' + name, *args, torch._C._cuda_getCurrentRawStream(at))
+    return _profiled(name, n, lambda: _lib.call('di_' + name, *args, torch._C._cuda_getCurrentRawStream(at)))
+
+
+def _row_view(t, C):
+    """(…, C) -> (tensor, row stride): as it is when its rows are uniformly strided with unit column stride (a view of packed
+    columns), else a dense copy."""
+    if t.is_contiguous():
+        return t, C
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    ok = t.stride(-1) == 1 or C == 1
+    rs, dims = None, 1                                              # the rows' stride: from the innermost dim of more than one
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if rs is None:
+            rs, dims = t.stride(d), t.shape[d]
+        else:
+            ok = ok and t.stride(d) == rs * dims
+            dims *= t.shape[d]
+    if not ok or (rs is not None and rs < 0):
+        t, rs = t.contiguous(), C
+    return t, C if rs is None else rs
+
+
+LAYERNORM_MAX_C = 16384
+
+
+def _layernorm_fwd(x, weight, bias, res, eps, with_sum, out_dtype, stats):
+    _same_device(x, weight, bias, res)
+    C = x.shape[-1] if x.dim() else 0
+    if not 1 <= C <= LAYERNORM_MAX_C:
+        raise ValueError(f'layernorm: {C} columns (1 .. {LAYERNORM_MAX_C} are supported)')
+    if weight.shape != (C,) or bias.shape != (C,) or weight.dtype != bias.dtype:
+        raise ValueError(f'layernorm: weight {tuple(weight.shape)} / bias {tuple(bias.shape)} of one dtype and shape ({C},) expected')
+    if res is not None and res.shape != x.shape:
+        raise ValueError(f'layernorm: x {tuple(x.shape)} and res {tuple(res.shape)} differ')
+    if with_sum and res is None:
+        raise ValueError('layernorm: with_sum without a residual (the sum is x)')
+    if out_dtype is None:
+        out_dtype = x.dtype if res is None else torch.promote_types(x.dtype, res.dtype)
+    codes = [_code3(x), _code3(x if res is None else res), _code3(weight), _code3(out_dtype)]
+    rows = x.numel() // C
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_sum else None
+    mean, rstd = (torch.empty(rows, dtype=torch.float32, device=x.device) for _ in range(2)) if stats else (None, None)
+    xv, xs = _row_view(x, C)
+    rv, rs = (None, 0) if res is None else _row_view(res, C)
+    w, b = weight.contiguous(), bias.contiguous()
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    _launch('layernorm_fwd', rows, x, xv.data_ptr(), xs, codes[0], ptr(rv), rs, codes[1], w.data_ptr(), b.data_ptr(), codes[2],
+            y.data_ptr(), codes[3], ptr(total), ptr(mean), ptr(rstd), rows, C, float(eps))
+    return y, total, mean, rstd
+
+
+def layernorm(x, weight, bias, res=None, eps=1e-5, with_sum=False, out_dtype=None):
+    """LayerNorm(x + res) over the last dim, any width up to 16 384 (res may be None); inference form.  x, res (..., C): views
+    with uniformly strided rows are read in place; float32 or one 16-bit type (float16 / bfloat16), each its own; weight / bias
+    (C,) float32 or that 16-bit type.  The result has `out_dtype` (default: the promoted type of x and res; 16-bit only when both
+    are).  with_sum: (y, x + res) - the sum is rounded to x's type first and the rounded value normalised, as a network that
+    carries it on sees it."""
+    y, total, _, _ = _layernorm_fwd(x, weight, bias, res, eps, with_sum, out_dtype, False)
+    return (y, total) if with_sum else y
+
+
+def layernorm_train_fwd(x, weight, bias, res=None, eps=1e-5, with_sum=False, out_dtype=None):
+    """`layernorm` with the row statistics kept for the backward: (y, sum or None, mean (rows,), rstd (rows,))."""
+    return _layernorm_fwd(x, weight, bias, res, eps, with_sum, out_dtype, True)
+
+
+def layernorm_train_bwd(grad_y, x, weight, mean, rstd, res=None, grad_sum=None, grad_dtype=None):
+    """Gradients of `layernorm_train_fwd`: (grad_x, grad_res, grad_weight, grad_bias).  x and res are what the forward read; where
+    it returned the sum, x = that sum and res = None (grad_x is then the gradient of both).  grad_sum: gradient of the returned
+    sum (added).  grad_res is None without res, and grad_x itself when both have one type.  grad_dtype: grad_x's type (x's).
+    Deterministic: the weight's and bias's reductions run in a fixed order, in float32."""
+    _same_device(grad_y, x, weight, mean, rstd, res, grad_sum)
+    C = x.shape[-1]
+    rows = x.numel() // C if C else 0
+    if not 1 <= C <= LAYERNORM_MAX_C or weight.shape != (C,):
+        raise ValueError(f'layernorm: x {tuple(x.shape)}, weight {tuple(weight.shape)}')
+    for name, t in (('grad_y', grad_y), ('res', res), ('grad_sum', grad_sum)):
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f'layernorm: {name} {tuple(t.shape)} and x {tuple(x.shape)} differ')
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
+            raise ValueError('layernorm: mean and rstd are the float32 rows that the forward returned')
+    grad_dtype = x.dtype if grad_dtype is None else grad_dtype
+    codes = [_code3(grad_y), _code3(x), _code3(x if res is None else res), _code3(weight), _code3(grad_dtype)]
+    if grad_sum is not None:
+        grad_sum = grad_sum.to(x.dtype)
+    if grad_y.dtype != torch.float32 and not x.dtype == (x if res is None else res).dtype == grad_y.dtype:
+        grad_y, codes[0] = grad_y.float(), _lib.DI_F32           # a 16-bit gradient of a float32 result: exact in float32
+    gx = torch.empty(x.shape, dtype=grad_dtype, device=x.device)
+    gres = None
+    if res is not None:
+        gres = gx if res.dtype == grad_dtype else torch.empty(res.shape, dtype=res.dtype, device=x.device)
+    gw, gb = (torch.empty(C, dtype=weight.dtype, device=x.device) for _ in range(2))
+    gv, gs = _row_view(grad_y, C)
+    sv, ss = (None, 0) if grad_sum is None else _row_view(grad_sum, C)
+    xv, xs = _row_view(x, C)
+    rv, rs = (None, 0) if res is None else _row_view(res, C)
+    w = weight.contiguous()
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    ws = torch.empty(max(4, _lib.lib().di_layernorm_bwd_workspace_floats(rows, C)), dtype=torch.float32, device=x.device)
+    _launch('layernorm_bwd', rows, x, gv.data_ptr(), gs, codes[0], ptr(sv), ss, xv.data_ptr(), xs, codes[1], ptr(rv), rs, codes[2],
+            w.data_ptr(), codes[3], mean.data_ptr(), rstd.data_ptr(), gx.data_ptr(), codes[4], 0 if gres is gx else ptr(gres),
+            gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), rows, C)
+    return gx, gres, gw, gb
+
+
 def _level_array(level_hw):
     L = len(level_hw)
     return (ctypes.c_int32 * (2 * L))(*[int(x) for pair in level_hw for x in pair])

@@ -37,7 +37,12 @@
 extern "C" {
 #endif
 
-enum { DI_F32 = 0, DI_F16 = 1, DI_F16_HL = 2 /* outputs only: split pair [hi | lo] fp16, x = hi + lo / 2048 */ };
+enum {
+  DI_F32 = 0,
+  DI_F16 = 1,
+  DI_F16_HL = 2, /* outputs only: split pair [hi | lo] fp16, x = hi + lo / 2048 */
+  DI_BF16 = 3    /* the LayerNorm and cross-attention entry points only */
+};
 enum {
   DI_OK = 0,
   DI_ERR_ARG = -1,      /* unsupported shape / window / dtype */
@@ -648,6 +653,26 @@ int di_bias_act_inplace(void *y, const float *bias, const void *residual, long l
 /* FPN top-down step in place (mmdet FPN.forward: `laterals[i - 1] += F.interpolate(laterals[i], size=..., mode='nearest')`, the
  * img_neck of Fusion_0075_refactor.py:137-145): lo (n, Hl, Wl, C) += nearest(hi (n, Hh, Wh, C)), channels-last fp16, C % 8 == 0. */
 int di_upsample_add_inplace(void *lo, const void *hi, int n, int Hl, int Wl, int Hh, int Wh, int C, void *stream);
+
+/* ---------------------------------------------------------------- LayerNorm with its residual add, any width
+ * The post-norm steps `norm(x + branch)` (decoder_utils.py:96-113, :743-756, :824-837) and their backward:
+ *   s = x (+ res), y = (s - mean) * rstd * weight + bias over the last dim C (1 .. 16384), statistics in float32.
+ * Strides in ELEMENTS between rows, columns contiguous; outputs are dense.  dtypes: DI_F32 or ONE 16-bit type (DI_F16 / DI_BF16)
+ * per call, each tensor its own; y is float32, or 16-bit when x and res are.  res may be NULL.
+ * di_layernorm_fwd: `sum` (x's dtype) may be NULL; otherwise it receives s, rounded, and the rounded value is normalised.
+ *   mean / rstd (rows floats each) may both be NULL (inference).
+ * di_layernorm_bwd: gy (y's dtype), gsum (x's dtype, may be NULL: the gradient of `sum`) -> gx (its own dtype), gres (res's
+ *   dtype, may be NULL; equal to gx), gweight / gbias (weight's dtype).  x, res: what the forward read - or x = `sum`, res = NULL.
+ *   workspace: di_layernorm_bwd_workspace_floats(rows, C) floats (< 0: unsupported), private to the call until it has run.
+ * rows == 0 is allowed (gweight = gbias = 0). */
+int di_layernorm_fwd(const void *x, long long x_row_stride, int x_dtype, const void *res, long long res_row_stride, int res_dtype,
+                     const void *weight, const void *bias, int w_dtype, void *y, int y_dtype, void *sum, float *mean, float *rstd,
+                     long long rows, int C, float eps, void *stream);
+long long di_layernorm_bwd_workspace_floats(long long rows, int C);
+int di_layernorm_bwd(const void *gy, long long gy_row_stride, int y_dtype, const void *gsum, long long gsum_row_stride, const void *x,
+                     long long x_row_stride, int x_dtype, const void *res, long long res_row_stride, int res_dtype, const void *weight,
+                     int w_dtype, const float *mean, const float *rstd, void *gx, int gx_dtype, void *gres, void *gweight, void *gbias,
+                     float *workspace, long long rows, int C, void *stream);
 
 #ifdef __cplusplus
 }
