@@ -51,6 +51,8 @@ SIGNATURES = {
     'di_polar_bev_sample_fwd': [_c_p] * 7 + [_c_i] * 8 + [_c_p],
     'di_mha_small_fwd': [_c_p, _c_i, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_f, _c_i, _c_p],
     'di_add_layernorm_fwd': [_c_p] * 5 + [ctypes.c_longlong, _c_i, _c_f, _c_i, _c_p],
+    'di_attention_fwd': [_c_p] * 5,
+    'di_attention_bwd': [_c_p] * 4 + [_c_ll, _c_ll, _c_p] + [_c_p, _c_ll, _c_ll] * 2 + [_c_p, _c_p],
     'di_layernorm_fwd': [_c_p, _c_ll, _c_i] * 2 + [_c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_p, _c_p, _c_ll, _c_i, _c_f, _c_p],
     'di_layernorm_bwd': [_c_p, _c_ll, _c_i, _c_p, _c_ll] + [_c_p, _c_ll, _c_i] * 2 + [_c_p, _c_i, _c_p, _c_p, _c_p, _c_i] + [_c_p] * 4 +
                         [_c_ll, _c_i, _c_p],
@@ -100,8 +102,9 @@ VALUE_FUNCS = {'di_mha_decode_scratch_floats': [_c_i] * 4, 'di_i2p_key_table_byt
                'di_token_splitk_workspace_bytes': [_c_i] * 2, 'di_mha_decode_x_ranges': [_c_i] * 3,
                'di_graph_node_count': [_c_p], 'di_local_attn_ring_timeouts': [_c_p], 'di_bn_workspace_floats': [_c_i],
                'di_layernorm_bwd_workspace_floats': [_c_ll, _c_i],
+               'di_attention_fwd_workspace_floats': [_c_p], 'di_attention_bwd_workspace_floats': [_c_p],
                'di_timed_consumed': [], 'di_wgrad_workspace_floats': [ctypes.c_longlong, _c_i, _c_i]}
-_LONGLONG = {'di_layernorm_bwd_workspace_floats', 'di_i2p_dense_bytes', 'di_wgrad_workspace_floats', 'di_topk_workspace_bytes', 'di_i2p_key_table_bytes', 'di_graph_node_count', 'di_token_splitk_workspace_bytes'}
+_LONGLONG = {'di_attention_fwd_workspace_floats', 'di_attention_bwd_workspace_floats', 'di_layernorm_bwd_workspace_floats', 'di_i2p_dense_bytes', 'di_wgrad_workspace_floats', 'di_topk_workspace_bytes', 'di_i2p_key_table_bytes', 'di_graph_node_count', 'di_token_splitk_workspace_bytes'}
 
 # ---- the step program of di_token_program (structs of include/deepinteraction_hip.h)
 TOK_LOAD, TOK_LOAD_PARTS, TOK_ATTN, TOK_COMBINE, TOK_LINEAR, TOK_ROWOP, TOK_STORE, TOK_HEADS = range(1, 9)
@@ -119,6 +122,14 @@ class TokHeads(ctypes.Structure):
     _fields_ = [('w2', _c_p), ('b2', _c_p), ('qpos', _c_p), ('keep', _c_p), ('pos_out', _c_p),
                 ('out', _c_p * TOK_MAX_HEADS), ('first', _c_p * TOK_MAX_HEADS), ('cls', _c_i * TOK_MAX_HEADS),
                 ('nheads', _c_i), ('center_head', _c_i), ('ldo', _c_i), ('col0', _c_i), ('qpos2', _c_p), ('pos2_out', _c_p)]
+
+
+
+class Attention(ctypes.Structure):
+    _fields_ = ([(n, _c_p) for n in ('q', 'k', 'v')] + [(n, _c_ll) for n in ('q_bs', 'q_rs', 'k_bs', 'k_rs', 'v_bs', 'v_rs')] +
+                [('key_lengths', _c_p), ('key_mask', _c_p), ('key_mask_bs', _c_ll), ('allowed', _c_p), ('allowed_bs', _c_ll),
+                 ('allowed_rs', _c_ll)] + [(n, _c_i) for n in ('B', 'L', 'S', 'heads', 'kv_heads', 'head_dim', 'dtype')] +
+                [('scale', _c_f), ('dropout_p', _c_f), ('seed', ctypes.c_ulonglong)])
 
 
 _lib = None

@@ -1,0 +1,231 @@
+// Attention of a set of queries to the states of another sequence: operand fragments, tiles and argument blocks shared by the
+// forward (attention_fwd.h) and backward (attention_bwd.h) kernels.
+//
+// Rows.  The G query heads that share a key head are rows of one problem: row r < G L of (sample b, key head) is query r % L of
+// head G hk + r / L.  lse / delta of (b, head, query) are then simply row r of a (B Hk, G L) matrix.
+//
+// Matrix instructions.  Every product is built from 16 x 16 tiles whose result has lane (i = lane % 16, g = lane / 16) hold
+// column i, rows 4 g .. 4 g + 3.  Two forms of operand fragments:
+//   row fragment: lane (i, g) holds row i's elements of the contraction over the head dim - 8 (32-wide products), 4 (16-wide,
+//     head dim 16) 16-bit elements, or a float4 that feeds four 4-wide float32 products; the order inside a contraction is free,
+//     so both operands simply use the same one and every fragment is one wide load;
+//   transposed fragment: column 16 dt + i of the rows 4 g + r - the contraction runs over the tile's ROWS (keys or queries).
+//     16-bit: two ds_read_b64_tr_b16 (two tiles of 16 rows, one 32-wide product); float32: four ds_read_b32.
+// A result tile's registers are, as they are, the other operand of a product that contracts over its rows: the probabilities and
+// score gradients never leave registers.
+#pragma once
+#include "di_common.h"
+
+namespace di {
+namespace at {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.4028234663852886e38f;
+
+__device__ __forceinline__ short to_half_bits(float x) { return __builtin_bit_cast(short, (_Float16)x); }
+__device__ __forceinline__ short to_bf_bits(float x) { return __builtin_bit_cast(short, (__bf16)x); }
+
+// TY: DI_F32 / DI_F16 / DI_BF16; DP: the head dim padded to 16, 32, 64 or 128
+template <int TY, int DP>
+struct Mm {
+  static constexpr bool WIDE = TY == DI_F32;
+  static constexpr int SZ = WIDE ? 4 : 2;
+  static constexpr int KD = WIDE || DP == 16 ? 16 : 32;         // head dims per row fragment
+  static constexpr int NK = DP / KD, ND = DP / 16;
+  static constexpr int CH = WIDE ? 16 : 32, NT = CH / 16;       // rows (keys / queries) per contraction over rows
+  static constexpr int PPR = DP * SZ / 16;                      // 16-byte pieces of a tile row
+  // tile row strides in bytes: + 16 keeps the 16-byte row fragments of 16 rows in different banks, + 32 (16-bit) the transposing reads
+  static constexpr int ROWS = DP * SZ + 16;
+  static constexpr int TRS = WIDE ? DP * 4 + 16 : (DP == 16 ? 32 : DP * 2 + 32);
+  struct RF {
+    u4 v;
+  };
+  struct TF {
+    u4 v;
+  };
+  struct PF {
+    u4 v;
+  };
+
+  static __device__ __forceinline__ int d0(int kk, int g) { return KD * kk + (WIDE || DP == 16 ? 4 : 8) * g; }
+  static __device__ __forceinline__ RF row_frag(const char *row, int kk, int g) {
+    RF f;
+    if constexpr (!WIDE && DP == 16) {
+      const u2 t = *reinterpret_cast<const u2 *>(row + 2 * d0(kk, g));
+      f.v = u4{t[0], t[1], 0, 0};
+    } else {
+      f.v = *reinterpret_cast<const u4 *>(row + SZ * d0(kk, g));
+    }
+    return f;
+  }
+  // from global memory: dims past D and rows that are not there are zeros
+  static __device__ __forceinline__ RF row_frag_of(const char *row, int kk, int g, int D, bool ok) {
+    RF f;
+    f.v = u4{0, 0, 0, 0};
+    if (ok && d0(kk, g) < D) f = row_frag(row, kk, g);
+    return f;
+  }
+  static __device__ __forceinline__ f4 dot(const RF &a, const RF &b, f4 c) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[j]), __uint_as_float(b.v[j]), c, 0, 0, 0);
+      return c;
+    } else if constexpr (DP == 16) {
+      const u2 x = {a.v[0], a.v[1]}, y = {b.v[0], b.v[1]};
+      if constexpr (TY == DI_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4, x), __builtin_bit_cast(h4, y), c, 0, 0, 0);
+      else
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, x), __builtin_bit_cast(s4, y), c, 0, 0, 0);
+    } else if constexpr (TY == DI_F16) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a.v), __builtin_bit_cast(h8, b.v), c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a.v), __builtin_bit_cast(b8, b.v), c, 0, 0, 0);
+    }
+  }
+  // columns 16 dt .. + 15 of the CH rows from row0 of a tile
+  static __device__ __forceinline__ TF tr_frag(const char *tile, int stride, int row0, int dt, int i, int g) {
+    TF f;
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) f.v[r] = *reinterpret_cast<const unsigned *>(tile + (row0 + 4 * g + r) * stride + 4 * (16 * dt + i));
+    } else {
+      const char *at = tile + (row0 + 4 * g + (i >> 2)) * stride + 32 * dt + 8 * (i & 3);
+      const tr4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4 __attribute__((address_space(3))) *)at);
+      const tr4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4 __attribute__((address_space(3))) *)(at + 16 * stride));
+      const u2 a = __builtin_bit_cast(u2, lo), b = __builtin_bit_cast(u2, hi);
+      f.v = u4{a[0], a[1], b[0], b[1]};
+    }
+    return f;
+  }
+  // result tiles (float32) -> operand of the contraction over their rows; 16-bit: rounded to nearest, half a step of the type -
+  // the same relative error for every size of probability, and independent from one to the next in the sums that follow
+  static __device__ __forceinline__ PF pack(const f4 (&p)[NT]) {
+    PF f;
+    if constexpr (WIDE) {
+      f.v = __builtin_bit_cast(u4, p[0]);
+    } else {
+      s8 s;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * t + r] = TY == DI_F16 ? to_half_bits(p[t][r]) : to_bf_bits(p[t][r]);
+      f.v = __builtin_bit_cast(u4, s);
+    }
+    return f;
+  }
+  static __device__ __forceinline__ f4 acc(const TF &a, const PF &p, f4 c) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[j]), __uint_as_float(p.v[j]), c, 0, 0, 0);
+      return c;
+    } else if constexpr (TY == DI_F16) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a.v), __builtin_bit_cast(h8, p.v), c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a.v), __builtin_bit_cast(b8, p.v), c, 0, 0, 0);
+    }
+  }
+  // four consecutive head dims of an output row
+  static __device__ __forceinline__ void store4(char *p, const f4 &x) {
+    if constexpr (WIDE) {
+      *reinterpret_cast<f4 *>(p) = x;
+    } else {
+      s4 s;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] = TY == DI_F16 ? to_half_bits(x[r]) : to_bf_bits(x[r]);
+      *reinterpret_cast<s4 *>(p) = s;
+    }
+  }
+  static __device__ __forceinline__ float widen_dot(const RF &a, const RF &b) {      // products of the elements of two row fragments
+    float t = 0.f;
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t = fmaf(__uint_as_float(a.v[j]), __uint_as_float(b.v[j]), t);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned short x = (unsigned short)(a.v[j] >> (16 * e)), y = (unsigned short)(b.v[j] >> (16 * e));
+          if constexpr (TY == DI_F16) t = fmaf((float)__builtin_bit_cast(_Float16, x), (float)__builtin_bit_cast(_Float16, y), t);
+          else t = fmaf(__uint_as_float((unsigned)x << 16), __uint_as_float((unsigned)y << 16), t);
+        }
+      }
+    }
+    return t;
+  }
+};
+
+// ---- attention dropout: keep or drop (row, key) from a counter-based hash, so that the backward regenerates the mask.  `mix` is
+// the 32-bit integer mixer "lowbias32" (C. Wellons, "Prospecting for hash functions", 2018).  One 16-bit number per pair: the drop
+// probability is a multiple of 2^-16, and the kept pairs are scaled by the reciprocal of exactly that.
+__device__ __forceinline__ unsigned mix(unsigned x) {
+  x ^= x >> 16; x *= 0x7feb352du;
+  x ^= x >> 15; x *= 0x846ca68bu;
+  return x ^ (x >> 16);
+}
+__device__ __forceinline__ unsigned drop_row(unsigned long long seed, unsigned long long row) {
+  return mix(mix((unsigned)seed + (unsigned)row * 0x9e3779b9u) ^ (unsigned)(seed >> 32) ^ ((unsigned)(row >> 32) * 0x85ebca6bu));
+}
+// numbers of the keys 4 k4 .. 4 k4 + 3 of a row: low and high halves of two words
+__device__ __forceinline__ unsigned drop_pair(unsigned row, unsigned k4, bool second) {
+  const unsigned x = mix(row ^ (k4 * 0xc2b2ae35u));
+  return second ? mix(x + 0x68bc21ebu) : x;
+}
+
+struct Args {
+  const char *q, *k, *v;
+  char *o;                               // forward: (B, L, H D); backward: the forward's output
+  const char *go;
+  char *gq, *gk, *gv;
+  float *lse, *delta;                    // (B Hk, G L); lse in the exp2 domain, -inf for an empty row
+  float *part, *part_ml;                 // split over keys: sums (splits, B Hk, G L, D) and (max, sum) pairs
+  float *part_k, *part_v;                // split over rows: (splits, B Hk, S, D)
+  const int *klen;
+  const unsigned char *kmask, *allowed;
+  long long q_bs, q_rs, k_bs, k_rs, v_bs, v_rs, go_bs, go_rs, gk_bs, gk_rs, gv_bs, gv_rs, kmask_bs, allowed_bs, allowed_rs;   // strides (q .. gv: bytes)
+  int B, L, S, Hk, G, D;
+  int splits, range;                     // key (or row) ranges of a split grid
+  int blocks;                            // row blocks (or key blocks)
+  float scale2;                          // softmax scale * log2(e)
+  float scale;
+  unsigned drop;                         // threshold of 65536; 0 = no dropout
+  float keep_scale;
+  unsigned long long seed;
+  const unsigned long long *seed_ptr;
+};
+
+__device__ __forceinline__ unsigned long long seed_of(const Args &a) { return a.seed + (a.seed_ptr != nullptr ? *a.seed_ptr : 0ull); }
+
+// block -> (row block, key head, split, sample); neighbours in this order - which read the same keys, or other heads of the same
+// rows of memory - are on one XCD and share its L2
+struct Where {
+  int blk, hk, sp, b;
+};
+__device__ __forceinline__ Where where(const Args &a) {
+  int id = xcd_remap(blockIdx.x, gridDim.x);
+  Where w;
+  w.blk = id % a.blocks; id /= a.blocks;
+  w.hk = id % a.Hk; id /= a.Hk;
+  w.sp = id % a.splits;
+  w.b = id / a.splits;
+  return w;
+}
+
+__device__ __forceinline__ int keys_of(const Args &a, int b) {
+  if (a.klen == nullptr) return a.S;
+  const int n = a.klen[b];
+  return n < 0 ? 0 : (n < a.S ? n : a.S);
+}
+
+}  // namespace at
+}  // namespace di

@@ -1,0 +1,165 @@
+// Entry points of the attention to another sequence (attention.h, attention_fwd.h, attention_bwd.h): checks, plans, dispatch.
+// Reference: the decoder layer's attention to the BEV map (decoder_utils.py:96-103, :421-485), the RoI blocks' attention among the
+// queries of a view (:743-746) and the ray decoder's attention to an image column (fusion_transformerv4.py:715-769).
+#include <math.h>
+
+#include "attention_plan.h"
+
+namespace di {
+namespace at {
+
+// Row blocks, and - where they are fewer than `want` - ranges of the walked side (multiples of `tile`) so that about `want`
+// workgroups run.
+static void cut(Plan &p, long long problems, int rows, int per_block, int walked, int tile, long long want) {
+  p.blocks = (rows + per_block - 1) / per_block;
+  const long long n = problems * (p.blocks > 0 ? p.blocks : 1);
+  const int tiles = walked > 0 ? (int)(((long long)walked + tile - 1) / tile) : 1;
+  long long splits = n > 0 ? want / n : 1;
+  splits = splits < 1 ? 1 : (splits > tiles ? tiles : splits);
+  const int per = (int)((tiles + splits - 1) / splits);
+  p.range = per > 0x7fffffff / tile ? 0x7fffffff : per * tile;
+  p.splits = (tiles + per - 1) / per;
+}
+
+static int plan_rows(const di_attention &t, Plan &p) {
+  const int cus = device_cus();
+  if (cus <= 0) return DI_ERR_LAUNCH;
+  const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
+  p.big = rows <= 16 ? 0 : (rows <= 64 ? 1 : 2);
+  const int per = p.big == 0 ? 16 : (p.big == 1 ? 64 : 64 * row_tiles(DP));
+  const int tile = p.big == 0 && t.dtype != DI_F32 ? 128 : 64;
+  cut(p, (long long)t.B * t.kv_heads, rows, per, t.S, tile, 4ll * cus);
+  return DI_OK;
+}
+
+static int plan_keys(const di_attention &t, Plan &p) {
+  const int cus = device_cus();
+  if (cus <= 0) return DI_ERR_LAUNCH;
+  const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
+  p.big = t.S > 64;
+  const int per = 64 * (p.big ? key_tiles(t.dtype, DP) : 1), tile = DP * (t.dtype == DI_F32 ? 4 : 2) >= 256 ? 32 : 64;
+  cut(p, (long long)t.B * t.kv_heads, t.S, per, rows, tile, 2ll * cus);
+  return DI_OK;
+}
+
+static bool aligned(const void *p, long long bs, long long rs, int size) {
+  return ((uintptr_t)p & 15) == 0 && (bs * size) % 16 == 0 && (rs * size) % 16 == 0;
+}
+
+static int check(const di_attention *t) {
+  DI_REQUIRE(t != nullptr, "attention: null pointer");
+  DI_REQUIRE(t->dtype == DI_F32 || t->dtype == DI_F16 || t->dtype == DI_BF16, "attention: unsupported dtype %d", t->dtype);
+  DI_REQUIRE(t->B >= 0 && t->L >= 0 && t->S >= 0, "attention: negative size");
+  DI_REQUIRE(t->heads > 0 && t->kv_heads > 0 && t->heads % t->kv_heads == 0, "attention: %d query heads, %d key heads", t->heads, t->kv_heads);
+  DI_REQUIRE(t->head_dim > 0 && t->head_dim % 8 == 0 && t->head_dim <= 128, "attention: head_dim %d (a multiple of 8, at most 128)", t->head_dim);
+  DI_REQUIRE(t->scale > 0.f && isfinite(t->scale), "attention: the scale must be positive and finite");
+  DI_REQUIRE(t->dropout_p >= 0.f && t->dropout_p < 1.f, "attention: dropout probability %f", (double)t->dropout_p);
+  const long long rows = (long long)(t->heads / t->kv_heads) * t->L;
+  DI_REQUIRE(rows <= 0x3fffffff && t->S <= 0x3fffffff, "attention: more than 2^30 rows or keys");
+  // every grid: problems x blocks x splits, and the joins' rows x head_dim / 4 / 256
+  const long long most = (long long)t->B * t->kv_heads * ((rows > t->S ? rows : t->S) / 16 + 2);
+  DI_REQUIRE(most <= 0x7fffffff / 2, "attention: too many rows for one launch");
+  const int sz = t->dtype == DI_F32 ? 4 : 2;
+  if (t->B == 0) return DI_OK;
+  DI_REQUIRE(t->L == 0 || (t->q != nullptr && aligned(t->q, t->q_bs, t->q_rs, sz)), "attention: q must start and step on 16 bytes");
+  DI_REQUIRE(t->S == 0 || (t->k != nullptr && t->v != nullptr && aligned(t->k, t->k_bs, t->k_rs, sz) && aligned(t->v, t->v_bs, t->v_rs, sz)),
+             "attention: k and v must start and step on 16 bytes");
+  return DI_OK;
+}
+
+static Args args_of(const di_attention *t) {
+  Args a = {};
+  const int sz = t->dtype == DI_F32 ? 4 : 2;
+  a.q = (const char *)t->q; a.k = (const char *)t->k; a.v = (const char *)t->v;
+  a.q_bs = t->q_bs * sz; a.q_rs = t->q_rs * sz;
+  a.k_bs = t->k_bs * sz; a.k_rs = t->k_rs * sz;
+  a.v_bs = t->v_bs * sz; a.v_rs = t->v_rs * sz;
+  a.klen = t->key_lengths;
+  a.kmask = t->key_mask; a.kmask_bs = t->key_mask_bs;
+  a.allowed = t->allowed; a.allowed_bs = t->allowed_bs; a.allowed_rs = t->allowed_rs;
+  a.B = t->B; a.L = t->L; a.S = t->S; a.Hk = t->kv_heads; a.G = t->heads / t->kv_heads; a.D = t->head_dim;
+  a.scale = t->scale;
+  a.scale2 = t->scale * kLog2e;
+  a.drop = (unsigned)(t->dropout_p * 65536.f + 0.5f);
+  if (a.drop > 65535u) a.drop = 65535u;
+  a.keep_scale = 65536.f / (float)(65536u - a.drop);
+  a.seed = t->seed;
+  a.seed_ptr = i2p_seed_ptr();
+  return a;
+}
+
+}  // namespace at
+}  // namespace di
+
+extern "C" {
+
+long long di_attention_fwd_workspace_floats(const di_attention *t) {
+  using namespace di::at;
+  if (check(t) != DI_OK) return -1;
+  Plan p;
+  if (plan_rows(*t, p) != DI_OK) return -1;
+  return p.splits == 1 ? 0 : (long long)p.splits * t->B * t->heads * t->L * (t->head_dim + 2);
+}
+
+long long di_attention_bwd_workspace_floats(const di_attention *t) {
+  using namespace di::at;
+  if (check(t) != DI_OK) return -1;
+  Plan p, k;
+  if (plan_rows(*t, p) != DI_OK || plan_keys(*t, k) != DI_OK) return -1;
+  const long long rows = (long long)t->B * t->heads * t->L, keys = (long long)t->B * t->kv_heads * t->S;
+  const long long gq = p.splits == 1 ? 0 : p.splits * rows * t->head_dim, gkv = k.splits == 1 ? 0 : 2ll * k.splits * keys * t->head_dim;
+  return (rows + 3) / 4 * 4 + (gq > gkv ? gq : gkv);            // delta | one launch's sums, then the other's
+}
+
+int di_attention_fwd(const di_attention *t, void *out, float *lse, float *workspace, void *stream) {
+  using namespace di::at;
+  if (int rc = check(t)) return rc;
+  if (t->B == 0 || t->L == 0) return DI_OK;
+  DI_REQUIRE(out != nullptr && ((uintptr_t)out & 15) == 0, "attention: the output must start on 16 bytes");
+  Plan p;
+  if (int rc = plan_rows(*t, p)) return rc;
+  Args a = args_of(t);
+  a.o = (char *)out;
+  a.lse = lse;
+  if (p.splits > 1) {
+    DI_REQUIRE(workspace != nullptr && ((uintptr_t)workspace & 15) == 0, "attention: workspace");
+    a.part = workspace;
+    a.part_ml = workspace + (long long)p.splits * t->B * t->heads * t->L * t->head_dim;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  return t->dtype == DI_F32 ? launch_fwd<DI_F32>(a, p, s) : t->dtype == DI_F16 ? launch_fwd<DI_F16>(a, p, s) : launch_fwd<DI_BF16>(a, p, s);
+}
+
+int di_attention_bwd(const di_attention *t, const void *out, const float *lse, const void *grad_out, long long go_bs, long long go_rs,
+                     void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs, long long gv_rs, float *workspace,
+                     void *stream) {
+  using namespace di::at;
+  if (int rc = check(t)) return rc;
+  if (t->B == 0 || (t->L == 0 && t->S == 0)) return DI_OK;
+  const int sz = t->dtype == DI_F32 ? 4 : 2;
+  DI_REQUIRE(t->L == 0 || (out && lse && grad_out && gq && ((uintptr_t)out & 15) == 0 && ((uintptr_t)gq & 15) == 0 && aligned(grad_out, go_bs, go_rs, sz)),
+             "attention: out, grad_out and grad_q must start (and grad_out step) on 16 bytes");
+  DI_REQUIRE(t->S == 0 || (gk && gv && aligned(gk, gk_bs, gk_rs, sz) && aligned(gv, gv_bs, gv_rs, sz)),
+             "attention: grad_k and grad_v must start and step on 16 bytes");
+  DI_REQUIRE((workspace != nullptr || t->L == 0) && ((uintptr_t)workspace & 15) == 0, "attention: workspace");   // no rows: one range, no sums
+  Plan p, k;
+  if (int rc = plan_rows(*t, p)) return rc;
+  if (int rc = plan_keys(*t, k)) return rc;
+  Args a = args_of(t);
+  a.o = (char *)const_cast<void *>(out);
+  a.lse = const_cast<float *>(lse);
+  a.go = (const char *)grad_out;
+  a.go_bs = go_bs * sz; a.go_rs = go_rs * sz;
+  a.gq = (char *)gq; a.gk = (char *)gk; a.gv = (char *)gv;
+  a.gk_bs = gk_bs * sz; a.gk_rs = gk_rs * sz; a.gv_bs = gv_bs * sz; a.gv_rs = gv_rs * sz;
+  const long long rows = (long long)t->B * t->heads * t->L, keys = (long long)t->B * t->kv_heads * t->S;
+  a.delta = workspace;
+  a.part = a.part_k = workspace + (rows + 3) / 4 * 4;
+  a.part_v = a.part_k + k.splits * keys * t->head_dim;
+  hipStream_t s = (hipStream_t)stream;
+  return t->dtype == DI_F32   ? launch_bwd<DI_F32>(a, p, k, s)
+         : t->dtype == DI_F16 ? launch_bwd<DI_F16>(a, p, k, s)
+                              : launch_bwd<DI_BF16>(a, p, k, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,389 @@
+// Backward of the attention to another sequence (attention_fwd.h).  With p_j = exp2(scale2 q . k_j - lse), dp_j = go . v_j,
+// delta = go . o and ds_j = p_j (dp_j - delta):
+//
+//     gq = scale sum_j ds_j k_j        gk_j = scale sum_rows ds_j q        gv_j = sum_rows p_j go
+//
+// Two launches, neither with atomics, both deterministic: `gq` keeps a block of rows in registers and walks over the keys (the
+// forward's structure; it also writes delta), `gk, gv` keeps a block of keys and walks over the rows.  Both form the scores again:
+// 14 D instead of 10 D operations a pair, but no partial result of the long side ever leaves the chip.
+//   gq:      S^T = K Q^T, dP^T = V go^T (16 keys x 16 rows), gq^T += K^T dS^T
+//   gk, gv:  S = Q K^T, dP = go V^T (16 rows x 16 keys), gv^T += go^T P, gk^T += Q^T dS
+// Where there are few blocks, the walked side is split over workgroups and their float32 sums are added in a fixed order.
+#pragma once
+#include "attention_fwd.h"
+
+namespace di {
+namespace at {
+
+template <int TY, int DP, int MT, int WQ>
+struct GqCfg {
+  using M = Mm<TY, DP>;
+  static constexpr int WK = 4 / WQ;
+  static constexpr int CPT = WQ == 1 ? 1 : 64 / M::CH;
+  static constexpr int TILE = WK * CPT * M::CH;
+  static constexpr int V_AT = TILE * M::TRS, BIAS_AT = V_AT + TILE * M::ROWS;
+  static constexpr int JOIN = WQ == 1 ? 4 * 16 * DP * 4 : 0;
+  static constexpr int LDS = BIAS_AT + TILE * 4 > JOIN ? BIAS_AT + TILE * 4 : JOIN;
+  static constexpr int ROWS_PER_BLOCK = 16 * MT * WQ;
+  static constexpr int NP = (TILE * M::PPR + 255) / 256;
+};
+
+template <int TY, int DP, int MT, int WQ>
+__global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
+  using C = GqCfg<TY, DP, MT, WQ>;
+  using M = Mm<TY, DP>;
+  extern __shared__ __align__(16) char lds[];
+  float *bias = reinterpret_cast<float *>(lds + C::BIAS_AT);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int wq = wave % WQ, wk = wave / WQ;
+  const Where at = where(a);
+  const int rows = a.G * a.L, ntile = (rows + 15) / 16;
+  const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
+  const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
+  const unsigned char *km = a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
+  const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
+
+  typename M::RF qf[MT][M::NK], gf[MT][M::NK];
+  f4 acc[MT][M::ND];
+  float lse[MT], delta[MT];
+  int row[MT], query[MT];
+  unsigned drow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int tile = (at.blk * MT + t) * WQ + wq;
+    row[t] = tile < ntile ? 16 * tile + i : rows;
+    const bool ok = row[t] < rows;
+    const int r = min(row[t], rows - 1), head = a.G == 1 ? 0 : r / a.L;
+    query[t] = r - head * a.L;
+    const long long col = (long long)(at.hk * a.G + head) * a.D * M::SZ;
+    const char *qp = a.q + at.b * a.q_bs + query[t] * a.q_rs + col, *gp = a.go + at.b * a.go_bs + query[t] * a.go_rs + col;
+    const char *op = a.o + ((long long)at.b * a.L + query[t]) * a.Hk * a.G * a.D * M::SZ + col;
+    float d = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < M::NK; ++kk) {
+      qf[t][kk] = M::row_frag_of(qp, kk, g, a.D, ok);
+      gf[t][kk] = M::row_frag_of(gp, kk, g, a.D, ok);
+      d += M::widen_dot(gf[t][kk], M::row_frag_of(op, kk, g, a.D, ok));
+    }
+    d += __shfl_xor(d, 16);
+    d += __shfl_xor(d, 32);
+    delta[t] = d;
+    const float e = ok ? a.lse[row_id + r] : INFINITY;
+    lse[t] = e == -INFINITY ? INFINITY : e;                     // an empty row: every probability 0
+    if (ok && at.sp == 0 && wk == 0 && g == 0) a.delta[row_id + row[t]] = d;
+#pragma unroll
+    for (int j = 0; j < M::ND; ++j) acc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
+    drow[t] = a.drop ? drop_row(seed_of(a), row_id + r) : 0;
+  }
+  if (a.splits > 1 && k0 >= k1) return;
+
+  KeyStage<C> st;
+  if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
+  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
+    __syncthreads();
+    st.commit(lds, M::TRS, M::ROWS, C::V_AT);
+    const bool ragged = km != nullptr || t0 + C::TILE > k1;
+    if (ragged && threadIdx.x < C::TILE) {
+      const int s = t0 + threadIdx.x;
+      bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
+    }
+    __syncthreads();
+    if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
+#pragma unroll
+    for (int c = 0; c < C::CPT; ++c) {
+      const int kc = (wk * C::CPT + c) * M::CH;
+      if (t0 + kc >= k1) break;
+      f4 s[MT][M::NT], dp[MT][M::NT];
+#pragma unroll
+      for (int u = 0; u < M::NT; ++u) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) s[t][u] = dp[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < M::NK; ++kk) {
+          const typename M::RF kf = M::row_frag(lds + (kc + 16 * u + i) * M::TRS, kk, g);
+          const typename M::RF vf = M::row_frag(lds + C::V_AT + (kc + 16 * u + i) * M::ROWS, kk, g);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
+            dp[t][u] = M::dot(vf, gf[t][kk], dp[t][u]);
+          }
+        }
+        if (ragged) {
+          const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][u][r] = bb[r] == 0.f ? s[t][u][r] : -INFINITY;
+        }
+        if (a.allowed != nullptr) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, s[t][u]);
+        }
+      }
+      typename M::PF df[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        f4 ds[M::NT];
+#pragma unroll
+        for (int u = 0; u < M::NT; ++u) {
+          if (a.drop) {
+            const unsigned k4 = (unsigned)(t0 + kc + 16 * u + 4 * g) >> 2;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const unsigned x = drop_pair(drow[t], k4, h);
+              dp[t][u][2 * h] = (x & 0xffffu) >= a.drop ? dp[t][u][2 * h] * a.keep_scale : 0.f;
+              dp[t][u][2 * h + 1] = (x >> 16) >= a.drop ? dp[t][u][2 * h + 1] * a.keep_scale : 0.f;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            ds[u][r] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], a.scale2, -lse[t])) * (dp[t][u][r] - delta[t]);
+        }
+        df[t] = M::pack(ds);
+      }
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d) {
+        const typename M::TF kf = M::tr_frag(lds, M::TRS, kc, d, i, g);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t][d] = M::acc(kf, df[t], acc[t][d]);
+      }
+    }
+  }
+
+  if constexpr (WQ == 1) {                                      // add the four wavefronts (MT = 1)
+    float *j = reinterpret_cast<float *>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) j[(wave * 16 + i) * DP + 16 * d + 4 * g + r] = acc[0][d][r];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d)
+#pragma unroll
+      for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[0][d][r] += j[(w * 16 + i) * DP + 16 * d + 4 * g + r];
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    if (row[t] >= rows) continue;
+    if (a.splits > 1) {
+      float *p = a.part + ((long long)at.sp * a.B * a.Hk * rows + row_id + row[t]) * a.D;
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+        if (16 * d + 4 * g < a.D) *reinterpret_cast<f4 *>(p + 16 * d + 4 * g) = acc[t][d];
+    } else {
+      const int head = a.G == 1 ? 0 : row[t] / a.L;
+      char *p = a.gq + (((long long)at.b * a.L + query[t]) * a.Hk * a.G + at.hk * a.G + head) * a.D * M::SZ;
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+        if (16 * d + 4 * g < a.D) M::store4(p + (16 * d + 4 * g) * M::SZ, acc[t][d] * a.scale);
+    }
+  }
+}
+
+// gq = scale * the ranges' sums; a thread per 4 head dims
+template <int TY>
+__global__ __launch_bounds__(256) void attention_gq_join_kernel(Args a) {
+  using M = Mm<TY, 16>;
+  const int rows = a.G * a.L, q4 = a.D / 4;
+  const long long all = (long long)a.B * a.Hk * rows, id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= all * q4) return;
+  const long long rid = id / q4;
+  const int d = 4 * (int)(id % q4), r = (int)(rid % rows), hk = (int)(rid / rows % a.Hk), b = (int)(rid / rows / a.Hk);
+  const int n = min(a.splits, (keys_of(a, b) + a.range - 1) / a.range);
+  f4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < n; ++s) o += *reinterpret_cast<const f4 *>(a.part + (s * all + rid) * a.D + d);
+  const int head = r / a.L;
+  M::store4(a.gq + ((((long long)b * a.L + (r - head * a.L)) * a.Hk * a.G + hk * a.G + head) * a.D + d) * M::SZ, o * a.scale);
+}
+
+template <int TY, int DP, int NT>
+struct GkvCfg {
+  using M = Mm<TY, DP>;
+  static constexpr int BR = DP * M::SZ >= 256 ? 32 : 64;        // rows per tile
+  static constexpr int KEYS = 64 * NT;
+  static constexpr int G_AT = BR * M::TRS, ST_AT = 2 * G_AT;    // both tiles are read in rows and transposed
+  static constexpr int LDS = ST_AT + 2 * BR * 4;
+  static constexpr int NP = (BR * M::PPR + 255) / 256;
+  // P of a normalised row is about 1 / S: in float16 it is scaled by 2^14 (the largest power of two whose product with 1 is finite
+  // with room to spare) so that probabilities down to 2^-28 keep their 11 bits; exact to undo
+  static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f;
+};
+
+template <int TY, int DP, int NT>
+__global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
+  using C = GkvCfg<TY, DP, NT>;
+  using M = Mm<TY, DP>;
+  extern __shared__ __align__(16) char lds[];
+  float *slse = reinterpret_cast<float *>(lds + C::ST_AT), *sdelta = slse + C::BR;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
+  const Where at = where(a);
+  const int rows = a.G * a.L, nkeys = keys_of(a, at.b);
+  const int key0 = at.blk * C::KEYS;
+  const int r0 = at.sp * a.range, r1 = key0 < nkeys ? min(r0 + a.range, rows) : r0;     // a block without keys: zeros
+  const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
+  const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
+
+  typename M::RF kf[NT][M::NK], vf[NT][M::NK];
+  f4 gk[NT][M::ND], gv[NT][M::ND];
+  bool valid[NT];
+  int key[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    key[n] = key0 + (wave * NT + n) * 16 + i;
+    valid[n] = key[n] < nkeys && (a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
+#pragma unroll
+    for (int kk = 0; kk < M::NK; ++kk) {
+      kf[n][kk] = M::row_frag_of(kb + key[n] * a.k_rs, kk, g, a.D, valid[n]);
+      vf[n][kk] = M::row_frag_of(vb + key[n] * a.v_rs, kk, g, a.D, valid[n]);
+    }
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d) gk[n][d] = gv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const unsigned long long seed = a.drop ? seed_of(a) : 0;
+
+  u4 qs[C::NP], gs[C::NP];
+  float ls = INFINITY, de = 0.f;
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int j = 0; j < C::NP; ++j) {
+      const int e = tid + 256 * j, rr = e / M::PPR, p = e % M::PPR, r = t0 + rr;
+      qs[j] = gs[j] = u4{0, 0, 0, 0};
+      if (r < r1 && rr < C::BR && p * 16 < a.D * M::SZ) {
+        const int head = a.G == 1 ? 0 : r / a.L, l = r - head * a.L;
+        const long long col = (long long)(at.hk * a.G + head) * a.D * M::SZ + p * 16;
+        qs[j] = *reinterpret_cast<const u4 *>(a.q + at.b * a.q_bs + l * a.q_rs + col);
+        gs[j] = *reinterpret_cast<const u4 *>(a.go + at.b * a.go_bs + l * a.go_rs + col);
+      }
+    }
+    if (tid < C::BR) {
+      const bool ok = t0 + tid < r1;
+      ls = ok ? a.lse[row_id + t0 + tid] : INFINITY;
+      de = ok ? a.delta[row_id + t0 + tid] : 0.f;
+    }
+  };
+  if (r0 < r1) fetch(r0);
+  for (int t0 = r0; t0 < r1; t0 += C::BR) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < C::NP; ++j) {
+      const int e = tid + 256 * j, rr = e / M::PPR, p = e % M::PPR;
+      if (C::BR * M::PPR % 256 == 0 || rr < C::BR) {
+        *reinterpret_cast<u4 *>(lds + rr * M::TRS + p * 16) = qs[j];
+        *reinterpret_cast<u4 *>(lds + C::G_AT + rr * M::TRS + p * 16) = gs[j];
+      }
+    }
+    if (tid < C::BR) {
+      slse[tid] = ls == -INFINITY ? INFINITY : ls;
+      sdelta[tid] = de;
+    }
+    __syncthreads();
+    if (t0 + C::BR < r1) fetch(t0 + C::BR);
+#pragma unroll 1
+    for (int rc = 0; rc < C::BR; rc += M::CH) {
+      if (t0 + rc >= r1) break;
+      typename M::PF pf[NT], df[NT];
+      f4 p[NT][M::NT], ds[NT][M::NT];
+#pragma unroll
+      for (int u = 0; u < M::NT; ++u) {
+        f4 s[NT], dp[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = dp[n] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < M::NK; ++kk) {
+          const typename M::RF qf = M::row_frag(lds + (rc + 16 * u + i) * M::TRS, kk, g);
+          const typename M::RF gf = M::row_frag(lds + C::G_AT + (rc + 16 * u + i) * M::TRS, kk, g);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            s[n] = M::dot(qf, kf[n][kk], s[n]);
+            dp[n] = M::dot(gf, vf[n][kk], dp[n]);
+          }
+        }
+        const f4 l4 = *reinterpret_cast<const f4 *>(slse + rc + 16 * u + 4 * g), d4 = *reinterpret_cast<const f4 *>(sdelta + rc + 16 * u + 4 * g);
+        const int rfirst = t0 + rc + 16 * u + 4 * g;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (a.allowed != nullptr) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int rr = min(rfirst + r, rows - 1);
+              if (valid[n] && a.allowed[at.b * a.allowed_bs + (rr % a.L) * a.allowed_rs + key[n]] == 0) s[n][r] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float pr = valid[n] ? __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale2, -l4[r])) : 0.f;
+            float keep = 1.f;
+            if (a.drop) {
+              const unsigned x = drop_pair(drop_row(seed, row_id + rfirst + r), (unsigned)key[n] >> 2, (key[n] & 2) != 0);
+              keep = ((key[n] & 1) ? x >> 16 : x & 0xffffu) >= a.drop ? a.keep_scale : 0.f;
+            }
+            p[n][u][r] = keep == 0.f ? 0.f : pr * C::P_SCALE;             // the kept ones' scale: at the end
+            ds[n][u][r] = pr * (dp[n][r] * keep - d4[r]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        pf[n] = M::pack(p[n]);
+        df[n] = M::pack(ds[n]);
+      }
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d) {
+        const typename M::TF gt = M::tr_frag(lds + C::G_AT, M::TRS, rc, d, i, g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) gv[n][d] = M::acc(gt, pf[n], gv[n][d]);
+        const typename M::TF qt = M::tr_frag(lds, M::TRS, rc, d, i, g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) gk[n][d] = M::acc(qt, df[n], gk[n][d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (key[n] >= a.S) continue;
+    if (a.splits > 1) {
+      const long long rec = (((long long)at.sp * a.B + at.b) * a.Hk + at.hk) * a.S + key[n];
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+        if (16 * d + 4 * g < a.D) {
+          *reinterpret_cast<f4 *>(a.part_k + rec * a.D + 16 * d + 4 * g) = gk[n][d];
+          *reinterpret_cast<f4 *>(a.part_v + rec * a.D + 16 * d + 4 * g) = gv[n][d];
+        }
+    } else {
+      const long long col = (long long)at.hk * a.D * M::SZ;
+      char *pk = a.gk + at.b * a.gk_bs + key[n] * a.gk_rs + col, *pv = a.gv + at.b * a.gv_bs + key[n] * a.gv_rs + col;
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+        if (16 * d + 4 * g < a.D) {
+          M::store4(pk + (16 * d + 4 * g) * M::SZ, gk[n][d] * a.scale);
+          M::store4(pv + (16 * d + 4 * g) * M::SZ, gv[n][d] * (a.keep_scale / C::P_SCALE));
+        }
+    }
+  }
+}
+
+template <int TY>
+__global__ __launch_bounds__(256) void attention_gkv_join_kernel(Args a) {
+  using M = Mm<TY, 16>;
+  const int q4 = a.D / 4;
+  const long long all = (long long)a.B * a.Hk * a.S, id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= all * q4) return;
+  const long long rid = id / q4;
+  const int d = 4 * (int)(id % q4), s = (int)(rid % a.S), hk = (int)(rid / a.S % a.Hk), b = (int)(rid / a.S / a.Hk);
+  f4 k = {0.f, 0.f, 0.f, 0.f}, v = k;
+  for (int r = 0; r < a.splits; ++r) {
+    k += *reinterpret_cast<const f4 *>(a.part_k + (r * all + rid) * a.D + d);
+    v += *reinterpret_cast<const f4 *>(a.part_v + (r * all + rid) * a.D + d);
+  }
+  const long long col = ((long long)hk * a.D + d) * M::SZ;
+  M::store4(a.gk + b * a.gk_bs + s * a.gk_rs + col, k * a.scale);
+  M::store4(a.gv + b * a.gv_bs + s * a.gv_rs + col, v * (a.keep_scale / GkvCfg<TY, 16, 1>::P_SCALE));
+}
+
+}  // namespace at
+}  // namespace di

@@ -1,0 +1,299 @@
+// Forward of the attention to another sequence.  Per row:  s_j = scale q . k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),
+// one pass over the keys with the running maximum m and sum.
+//
+// S^T = K Q^T (16 keys x 16 rows a tile: a row is a lane's column, its running maximum and sum are two registers), O^T += V^T P^T
+// with the exponentials' registers as the operand.  The keys' tile goes through LDS (loads of the next one in flight in registers
+// behind the products), where four wavefronts read it: WQ = 4 wavefronts with MT row tiles each on the same keys, or - up to 16
+// rows, single queries - WQ = 1, four wavefronts on four parts of the tile, joined at the end.  Few row blocks: the keys are split
+// over workgroups, which leave (m, sum, O) in float32 for a second launch to join.
+//
+// The maximum is corrected only when a score exceeds it by more than 8 (a factor of 256 in exp2's argument, harmless in float32 and
+// in the 16-bit probabilities): the test is one comparison per tile against the lane's own scores, the exchange between lanes and
+// the correction of the sums run when any lane asks for them - a few times per row, not once per tile.
+#pragma once
+#include "attention.h"
+
+namespace di {
+namespace at {
+
+template <int TY, int DP, int MT, int WQ>
+struct FwdCfg {
+  using M = Mm<TY, DP>;
+  static constexpr int WK = 4 / WQ;
+  static constexpr int CPT = WQ == 1 ? 1 : 64 / M::CH;          // chunks of CH keys per wavefront and tile
+  static constexpr int TILE = WK * CPT * M::CH;
+  static constexpr int V_AT = TILE * M::ROWS, BIAS_AT = V_AT + TILE * M::TRS;
+  static constexpr int JOIN = WQ == 1 ? 4 * 16 * (DP + 2) * 4 : 0;
+  static constexpr int LDS = BIAS_AT + TILE * 4 > JOIN ? BIAS_AT + TILE * 4 : JOIN;
+  static constexpr int ROWS_PER_BLOCK = 16 * MT * WQ;
+  static constexpr int NP = (TILE * M::PPR + 255) / 256;        // pieces per thread, K and V each
+};
+
+// the staged loads of a tile of keys: key rows t0 .. of K and V, zeros where there is no key (so that no NaN of an excluded key
+// or of memory behind the last one reaches a product)
+template <class C>
+struct KeyStage {
+  u4 k[C::NP], v[C::NP];
+  __device__ __forceinline__ void fetch(const Args &a, const char *kb, const char *vb, const unsigned char *km, int t0, int k1) {
+    using M = typename C::M;
+#pragma unroll
+    for (int j = 0; j < C::NP; ++j) {
+      const int e = threadIdx.x + 256 * j, key = e / M::PPR, p = e % M::PPR, s = t0 + key;
+      k[j] = v[j] = u4{0, 0, 0, 0};
+      bool ok = s < k1 && key < C::TILE && p * 16 < a.D * M::SZ;
+      if (km != nullptr && ok) ok = km[s] != 0;
+      if (ok) {
+        k[j] = *reinterpret_cast<const u4 *>(kb + s * a.k_rs + p * 16);
+        v[j] = *reinterpret_cast<const u4 *>(vb + s * a.v_rs + p * 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void commit(char *lds, int kstride, int vstride, int v_at) {
+    using M = typename C::M;
+#pragma unroll
+    for (int j = 0; j < C::NP; ++j) {
+      const int e = threadIdx.x + 256 * j, key = e / M::PPR, p = e % M::PPR;
+      if (C::TILE * M::PPR % 256 == 0 || key < C::TILE) {
+        *reinterpret_cast<u4 *>(lds + key * kstride + p * 16) = k[j];
+        *reinterpret_cast<u4 *>(lds + v_at + key * vstride + p * 16) = v[j];
+      }
+    }
+  }
+};
+
+// 4 keys x 1 row of the (row, key) mask; keys past the end count as allowed (their scores are excluded by the bias)
+__device__ __forceinline__ void exclude(const unsigned char *row, int key, int S, f4 &s) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (key + r < S && row[key + r] == 0) s[r] = -INFINITY;
+}
+
+template <int TY, int DP, int MT, int WQ>
+__global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
+  using C = FwdCfg<TY, DP, MT, WQ>;
+  using M = Mm<TY, DP>;
+  extern __shared__ __align__(16) char lds[];
+  float *bias = reinterpret_cast<float *>(lds + C::BIAS_AT);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int wq = wave % WQ, wk = wave / WQ;
+  const Where at = where(a);
+  const int rows = a.G * a.L, ntile = (rows + 15) / 16;
+  const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
+  if (a.splits > 1 && k0 >= k1) return;                         // the join knows the sample's keys, too
+  const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
+  const unsigned char *km = a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
+  const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
+
+  typename M::RF qf[MT][M::NK];
+  f4 o[MT][M::ND];
+  float m[MT], l[MT];
+  int row[MT], query[MT];
+  unsigned drow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int tile = (at.blk * MT + t) * WQ + wq;               // row tiles dealt out to the wavefronts in turn
+    row[t] = tile < ntile ? 16 * tile + i : rows;
+    const int r = min(row[t], rows - 1), head = a.G == 1 ? 0 : r / a.L;
+    query[t] = r - head * a.L;
+    const char *qp = a.q + at.b * a.q_bs + query[t] * a.q_rs + (long long)(at.hk * a.G + head) * a.D * M::SZ;
+#pragma unroll
+    for (int kk = 0; kk < M::NK; ++kk) qf[t][kk] = M::row_frag_of(qp, kk, g, a.D, row[t] < rows);
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
+    m[t] = kLowest;
+    l[t] = 0.f;
+    drow[t] = a.drop ? drop_row(seed_of(a), row_id + r) : 0;
+  }
+
+  KeyStage<C> st;
+  if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
+  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
+    __syncthreads();                                            // the last tile's reads are done
+    st.commit(lds, M::ROWS, M::TRS, C::V_AT);
+    const bool ragged = km != nullptr || t0 + C::TILE > k1;
+    if (ragged && threadIdx.x < C::TILE) {
+      const int s = t0 + threadIdx.x;
+      bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
+    }
+    __syncthreads();
+    if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
+#pragma unroll
+    for (int c = 0; c < C::CPT; ++c) {
+      const int kc = (wk * C::CPT + c) * M::CH;                 // first key of the chunk in the tile
+      if (t0 + kc >= k1) break;
+      f4 s[MT][M::NT];
+#pragma unroll
+      for (int u = 0; u < M::NT; ++u) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) s[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < M::NK; ++kk) {
+          const typename M::RF kf = M::row_frag(lds + (kc + 16 * u + i) * M::ROWS, kk, g);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
+        }
+        if (ragged) {
+          const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][u][r] = bb[r] == 0.f ? s[t][u][r] : -INFINITY;
+        }
+        if (a.allowed != nullptr) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, s[t][u]);
+        }
+      }
+      float mx[MT];
+      bool over = false;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        mx[t] = kLowest;
+#pragma unroll
+        for (int u = 0; u < M::NT; ++u) mx[t] = fmaxf(fmaxf(fmaxf(s[t][u][0], s[t][u][1]), fmaxf(s[t][u][2], s[t][u][3])), mx[t]);
+        mx[t] *= a.scale2;
+        over |= mx[t] > m[t] + 8.f;
+      }
+      if (__any(over)) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          float x = fmaxf(mx[t], __shfl_xor(mx[t], 16));
+          x = fmaxf(x, __shfl_xor(x, 32));
+          x = fmaxf(x, m[t]);
+          const float f = __builtin_amdgcn_exp2f(m[t] - x);
+          m[t] = x;
+          l[t] *= f;
+#pragma unroll
+          for (int d = 0; d < M::ND; ++d) o[t][d] *= f;
+        }
+      }
+      typename M::PF pf[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        f4 p[M::NT];
+#pragma unroll
+        for (int u = 0; u < M::NT; ++u) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[u][r] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], a.scale2, -m[t]));
+          l[t] += (p[u][0] + p[u][1]) + (p[u][2] + p[u][3]);
+          if (a.drop) {
+            const unsigned k4 = (unsigned)(t0 + kc + 16 * u + 4 * g) >> 2;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const unsigned x = drop_pair(drow[t], k4, h);
+              p[u][2 * h] = (x & 0xffffu) >= a.drop ? p[u][2 * h] : 0.f;      // the kept ones' scale: at the end
+              p[u][2 * h + 1] = (x >> 16) >= a.drop ? p[u][2 * h + 1] : 0.f;
+            }
+          }
+        }
+        pf[t] = M::pack(p);
+      }
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d) {
+        const typename M::TF vf = M::tr_frag(lds + C::V_AT, M::TRS, kc, d, i, g);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) o[t][d] = M::acc(vf, pf[t], o[t][d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    l[t] += __shfl_xor(l[t], 16);
+    l[t] += __shfl_xor(l[t], 32);
+  }
+
+  if constexpr (WQ == 1) {                                      // join the four wavefronts (MT = 1)
+    float *j = reinterpret_cast<float *>(lds);                  // (4, 16, DP + 2)
+    __syncthreads();
+    float *mine = j + (wave * 16 + i) * (DP + 2);
+    if (g == 0) {
+      mine[0] = m[0];
+      mine[1] = l[0];
+    }
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mine[2 + 16 * d + 4 * g + r] = o[0][d][r];
+    __syncthreads();
+    if (wave != 0) return;
+    float top = m[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, j[(w * 16 + i) * (DP + 2)]);
+    l[0] = 0.f;
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d) o[0][d] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float *p = j + (w * 16 + i) * (DP + 2);
+      const float f = __builtin_amdgcn_exp2f(p[0] - top);
+      l[0] = fmaf(p[1], f, l[0]);
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[0][d][r] = fmaf(p[2 + 16 * d + 4 * g + r], f, o[0][d][r]);
+    }
+    m[0] = top;
+  }
+
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    if (row[t] >= rows) continue;
+    if (a.splits > 1) {
+      const long long rec = (long long)at.sp * a.B * a.Hk * rows + row_id + row[t];
+      if (g == 0) {
+        a.part_ml[2 * rec] = m[t];
+        a.part_ml[2 * rec + 1] = l[t];
+      }
+      float *p = a.part + rec * a.D;
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+        if (16 * d + 4 * g < a.D) *reinterpret_cast<f4 *>(p + 16 * d + 4 * g) = o[t][d];
+    } else {
+      const float inv = l[t] == 0.f ? 0.f : a.keep_scale / l[t];         // an empty row: zeros
+      if (a.lse != nullptr && g == 0) a.lse[row_id + row[t]] = l[t] == 0.f ? -INFINITY : m[t] + __builtin_amdgcn_logf(l[t]);
+      const int head = a.G == 1 ? 0 : row[t] / a.L;
+      char *p = a.o + (((long long)at.b * a.L + query[t]) * a.Hk * a.G + at.hk * a.G + head) * a.D * M::SZ;
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+        if (16 * d + 4 * g < a.D) M::store4(p + (16 * d + 4 * g) * M::SZ, o[t][d] * inv);
+    }
+  }
+}
+
+// The ranges' states of a row joined; one 16-lane group per row, 4 head dims a lane and step.
+template <int TY>
+__global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
+  using M = Mm<TY, 16>;
+  const int i = threadIdx.x & 15;
+  const int rows = a.G * a.L;
+  const long long all = (long long)a.B * a.Hk * rows, id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (id >= all) return;
+  const int r = (int)(id % rows), hk = (int)(id / rows % a.Hk), b = (int)(id / rows / a.Hk);
+  const int n = min(a.splits, (keys_of(a, b) + a.range - 1) / a.range);
+  float top = kLowest;
+  for (int s = i; s < n; s += 16) top = fmaxf(top, a.part_ml[2 * (s * all + id)]);
+  top = row16_max(top);
+  float l = 0.f;
+  for (int s = i; s < n; s += 16) {
+    const float *p = a.part_ml + 2 * (s * all + id);
+    l = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - top), l);
+  }
+  l = row16_sum(l);
+  const float inv = l == 0.f ? 0.f : a.keep_scale / l;
+  if (a.lse != nullptr && i == 0) a.lse[id] = l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l);
+  const int head = r / a.L;
+  char *out = a.o + (((long long)b * a.L + (r - head * a.L)) * a.Hk * a.G + hk * a.G + head) * a.D * M::SZ;
+  for (int d = 4 * i; d < a.D; d += 64) {
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < n; ++s) {
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * all + id)] - top);
+      const f4 p = *reinterpret_cast<const f4 *>(a.part + (s * all + id) * a.D + d);
+      o += p * f;
+    }
+    M::store4(out + d * M::SZ, o * inv);
+  }
+}
+
+}  // namespace at
+}  // namespace di

@@ -1,0 +1,99 @@
+// Dispatch of the attention kernels of one element type by head dim and variant.
+#pragma once
+#include "attention_bwd.h"
+#include "attention_plan.h"
+
+namespace di {
+namespace at {
+
+template <class K>
+static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &a, hipStream_t s, const char *name) {
+  if (grid <= 0) return DI_OK;
+  if (int rc = ensure_lds(raised, (const void *)kernel, lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), lds, s, a);
+  return check_launch(name);
+}
+
+template <int TY, int DP, int MT, int WQ>
+static int fwd(const Args &a, hipStream_t s) {
+  static LdsRaised raised;
+  return go(attention_fwd_kernel<TY, DP, MT, WQ>, raised, FwdCfg<TY, DP, MT, WQ>::LDS, (long long)a.B * a.splits * a.Hk * a.blocks, a, s,
+            "attention_fwd");
+}
+template <int TY, int DP, int MT, int WQ>
+static int gq(const Args &a, hipStream_t s) {
+  static LdsRaised raised;
+  return go(attention_gq_kernel<TY, DP, MT, WQ>, raised, GqCfg<TY, DP, MT, WQ>::LDS, (long long)a.B * a.splits * a.Hk * a.blocks, a, s,
+            "attention_gq");
+}
+template <int TY, int DP, int NT>
+static int gkv(const Args &a, hipStream_t s) {
+  static LdsRaised raised;
+  return go(attention_gkv_kernel<TY, DP, NT>, raised, GkvCfg<TY, DP, NT>::LDS, (long long)a.B * a.splits * a.Hk * a.blocks, a, s,
+            "attention_gkv");
+}
+
+static void take(Args &a, const Plan &p) {
+  a.blocks = p.blocks;
+  a.splits = p.splits;
+  a.range = p.range;
+}
+
+template <int TY>
+int launch_fwd(const Args &args, const Plan &p, hipStream_t s) {
+  Args a = args;
+  take(a, p);
+  int rc;
+#define DI_AT_FWD(DP) \
+  rc = p.big == 0 ? fwd<TY, DP, 1, 1>(a, s) : p.big == 1 ? fwd<TY, DP, 1, 4>(a, s) : fwd<TY, DP, row_tiles(DP), 4>(a, s)
+  switch (padded(a.D)) {
+    case 16: DI_AT_FWD(16); break;
+    case 32: DI_AT_FWD(32); break;
+    case 64: DI_AT_FWD(64); break;
+    default: DI_AT_FWD(128); break;
+  }
+#undef DI_AT_FWD
+  if (rc != DI_OK || p.splits == 1) return rc;
+  const long long all = (long long)a.B * a.Hk * a.G * a.L;
+  hipLaunchKernelGGL((attention_join_kernel<TY>), dim3((unsigned)((all + 15) / 16)), dim3(256), 0, s, a);
+  return check_launch("attention_join");
+}
+
+template <int TY>
+int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) {
+  Args a = args;
+  int rc = DI_OK;
+  take(a, pq);
+#define DI_AT_GQ(DP) \
+  rc = pq.big == 0 ? gq<TY, DP, 1, 1>(a, s) : pq.big == 1 ? gq<TY, DP, 1, 4>(a, s) : gq<TY, DP, row_tiles(DP), 4>(a, s)
+  if (a.L > 0) switch (padded(a.D)) {
+    case 16: DI_AT_GQ(16); break;
+    case 32: DI_AT_GQ(32); break;
+    case 64: DI_AT_GQ(64); break;
+    default: DI_AT_GQ(128); break;
+  }
+#undef DI_AT_GQ
+  if (rc != DI_OK) return rc;
+  if (pq.splits > 1) {
+    const long long n = (long long)a.B * a.Hk * a.G * a.L * (a.D / 4);
+    hipLaunchKernelGGL((attention_gq_join_kernel<TY>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    if ((rc = check_launch("attention_gq_join")) != DI_OK) return rc;
+  }
+  if (a.S == 0) return DI_OK;
+  take(a, pk);
+#define DI_AT_GKV(DP) rc = pk.big ? gkv<TY, DP, key_tiles(TY, DP)>(a, s) : gkv<TY, DP, 1>(a, s)
+  switch (padded(a.D)) {
+    case 16: DI_AT_GKV(16); break;
+    case 32: DI_AT_GKV(32); break;
+    case 64: DI_AT_GKV(64); break;
+    default: DI_AT_GKV(128); break;
+  }
+#undef DI_AT_GKV
+  if (rc != DI_OK || pk.splits == 1) return rc;
+  const long long n = (long long)a.B * a.Hk * a.S * (a.D / 4);
+  hipLaunchKernelGGL((attention_gkv_join_kernel<TY>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+  return check_launch("attention_gkv_join");
+}
+
+}  // namespace at
+}  // namespace di

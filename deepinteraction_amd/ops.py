@@ -1223,6 +1223,149 @@ def layernorm_train_bwd(grad_y, x, weight, mean, rstd, res=None, grad_sum=None, 
     return gx, gres, gw, gb
 
 
+# ------------------------------------------------------------------ attention to the states of another sequence
+def _bool_bytes(t, name):
+    if t.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f'cross_attention: {name} is a bool (or uint8) tensor, got {t.dtype}')
+    return t
+
+
+def _seq_view(t):
+    """(B, N, E) as it is when its columns are contiguous and its rows start on 16 bytes, else a dense copy; an expanded batch
+    (stride 0) is read in place."""
+    n = t.element_size()
+    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * n % 16 == 0 and t.stride(1) * n % 16 == 0 \
+            and t.stride(0) >= 0 and t.stride(1) >= 0:
+        return t
+    return t.contiguous()
+
+
+def _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed):
+    """The checked argument block (and the tensors that it points to)."""
+    _same_device(q, k, v, key_lengths, key_mask, allowed)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0]:
+        raise ValueError(f'cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f'cross_attention: q {q.dtype}, k {k.dtype}, v {v.dtype}')
+    B, L, E = q.shape
+    S, Ek = k.shape[1], k.shape[2]
+    if num_heads <= 0 or E % num_heads or E == 0:
+        raise ValueError(f'cross_attention: {E} columns in {num_heads} heads')
+    D = E // num_heads
+    if D % 8 or D > 128:
+        raise ValueError(f'cross_attention: head_dim {D} (a multiple of 8, at most 128)')
+    if Ek == 0 or Ek % D or num_heads % (Ek // D):
+        raise ValueError(f'cross_attention: {Ek} key columns for {num_heads} heads of {D}')
+    t = _lib.Attention()
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f'cross_attention: scale {scale} (positive and finite)')
+    if not 0.0 <= dropout_p < 1.0:
+        raise ValueError(f'cross_attention: dropout_p {dropout_p} (0 <= p < 1)')
+    q, k, v = _seq_view(q), _seq_view(k), _seq_view(v)
+    keep = [q, k, v]
+    t.q, t.k, t.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    t.q_bs, t.q_rs, _ = q.stride()
+    t.k_bs, t.k_rs, _ = k.stride()
+    t.v_bs, t.v_rs, _ = v.stride()
+    if key_lengths is not None:
+        if key_lengths.shape != (B,) or key_lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f'cross_attention: key_lengths {key_lengths.dtype} {tuple(key_lengths.shape)}, int32 ({B},) expected')
+        if key_lengths.dtype == torch.int64:
+            key_lengths = key_lengths.clamp(0, S).int()
+        key_lengths = key_lengths.contiguous()
+        keep.append(key_lengths)
+        t.key_lengths = key_lengths.data_ptr()
+    if key_mask is not None:
+        if key_mask.shape != (B, S):
+            raise ValueError(f'cross_attention: key_mask {tuple(key_mask.shape)}, ({B}, {S}) expected')
+        key_mask = _bool_bytes(key_mask, 'key_mask')
+        if S > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        keep.append(key_mask)
+        t.key_mask, t.key_mask_bs = key_mask.data_ptr(), key_mask.stride(0)
+    if allowed is not None:
+        if allowed.shape != (B, L, S):
+            raise ValueError(f'cross_attention: allowed {tuple(allowed.shape)}, ({B}, {L}, {S}) expected')
+        allowed = _bool_bytes(allowed, 'allowed')
+        if S > 1 and allowed.stride(2) != 1:
+            allowed = allowed.contiguous()
+        keep.append(allowed)
+        t.allowed, t.allowed_bs, t.allowed_rs = allowed.data_ptr(), allowed.stride(0), allowed.stride(1)
+    t.B, t.L, t.S, t.heads, t.kv_heads, t.head_dim, t.dtype = B, L, S, num_heads, Ek // D, D, _code3(q)
+    t.scale, t.dropout_p, t.seed = scale, float(dropout_p), int(seed) & 0xFFFFFFFFFFFFFFFF
+    return t, keep
+
+
+def _on_device(q, f):
+    """f() with q's device current: plans ask for its number of compute units."""
+    if q.get_device() == torch.cuda.current_device():
+        return f()
+    with torch.cuda.device(q.device):
+        return f()
+
+
+def _attention_workspace(name, ref, q):
+    n = _on_device(q, lambda: getattr(_lib.lib(), name)(ref))
+    if n < 0:
+        raise _lib.HipLibraryError(f'{name}: {_lib.lib().di_last_error().decode()}')
+    return torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+
+
+def _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, stats):
+    t, keep = _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((t.B, t.heads, t.L), dtype=torch.float32, device=q.device) if stats else None
+    ref = ctypes.addressof(t)
+    ws = _attention_workspace('di_attention_fwd_workspace_floats', ref, q)
+    _launch('attention_fwd', t.B, q, ref, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr())
+    return out, lse
+
+
+def cross_attention(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None):
+    """softmax(scale q k^T) v per head, q (B, L, heads * D) to the states k, v (B, S, key heads * D) of another sequence - one query
+    per sample or thousands; D a multiple of 8, at most 128, `scale` D^-1/2 by default; float32, float16 or bfloat16, softmax and sums
+    in float32.  Fewer key heads than heads: heads // key heads query heads share one.  k and v (and q) may be columns of one packed
+    projection: strided rows are read in place.
+    Keys that take part (optional, combined): the first key_lengths[b] (int32; int64 is converted); key_mask (B, S) and allowed
+    (B, L, S), bool, True = takes part, expanded views are fine.  What lies behind key_lengths or under key_mask may hold anything;
+    keys that only `allowed` excludes have to be finite.  A query without keys gives zeros."""
+    return _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, 0.0, 0, False)[0]
+
+
+def cross_attention_train_fwd(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None, dropout_p=0.0, seed=0):
+    """`cross_attention` with the per-query log2-sum-exp2 kept for the backward: (out, lse (B, heads, L)).  dropout_p: dropout of the
+    attention weights, decided per (query, head, key) by a counter-based hash of `seed` (plus the word of `set_i2p_seed_tensor`)
+    that the backward regenerates; p is rounded to a multiple of 2^-16."""
+    return _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, True)
+
+
+def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None,
+                              dropout_p=0.0, seed=0, grads_kv=None):
+    """(grad_q, grad_k, grad_v) of `cross_attention_train_fwd`; the softmax is recomputed from `lse`, deterministic.  grads_kv: write
+    grad_k and grad_v into these (B, S, key heads * D) tensors (halves of one packed gradient) instead of allocating them."""
+    t, keep = _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+    _same_device(q, out, grad_out, lse, *(grads_kv or ()))
+    if out.shape != q.shape or out.dtype != q.dtype or grad_out.shape != q.shape:
+        raise ValueError(f'cross_attention: out {tuple(out.shape)}, grad_out {tuple(grad_out.shape)}, q {tuple(q.shape)}')
+    if lse.shape != (t.B, t.heads, t.L) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError('cross_attention: lse is the tensor that the forward returned')
+    out, go = out.contiguous(), _seq_view(grad_out.to(q.dtype))
+    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if grads_kv is None:
+        gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+    else:
+        gk, gv = grads_kv
+        for x in (gk, gv):
+            if x.shape != k.shape or x.dtype != k.dtype or _seq_view(x) is not x or (t.B > 1 and x.stride(0) == 0):
+                raise ValueError('cross_attention: grads_kv have the shape and type of k, contiguous columns and rows on 16 bytes')
+    ref = ctypes.addressof(t)
+    ws = _attention_workspace('di_attention_bwd_workspace_floats', ref, q)
+    _launch('attention_bwd', t.B, q, ref, out.data_ptr(), lse.data_ptr(), go.data_ptr(), go.stride(0), go.stride(1), gq.data_ptr(),
+            gk.data_ptr(), gk.stride(0), gk.stride(1), gv.data_ptr(), gv.stride(0), gv.stride(1), 0 if ws is None else ws.data_ptr())
+    return gq, gk, gv
+
+
 def _level_array(level_hw):
     L = len(level_hw)
     return (ctypes.c_int32 * (2 * L))(*[int(x) for pair in level_hw for x in pair])

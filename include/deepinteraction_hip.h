@@ -674,6 +674,40 @@ int di_layernorm_bwd(const void *gy, long long gy_row_stride, int y_dtype, const
                      int w_dtype, const float *mean, const float *rstd, void *gx, int gx_dtype, void *gres, void *gweight, void *gbias,
                      float *workspace, long long rows, int C, void *stream);
 
+/* ---------------------------------------------------------------- attention to the states of another sequence, forward and backward
+ * out = softmax(scale q k^T) v per head over the keys that take part: decoder_utils.py:96-103 and :421-485 (queries -> BEV map),
+ * :743-746 (queries of a view), fusion_transformerv4.py:715-769 (rays -> image column), in the forms that training needs.
+ *   q (B, L, heads * head_dim), k / v (B, S, kv_heads * head_dim); batch and row strides in ELEMENTS, head columns contiguous, rows
+ *   on 16-byte boundaries (packed projections are read in place).  heads % kv_heads == 0: query head h reads key head
+ *   h / (heads / kv_heads).  head_dim: a multiple of 8, <= 128.  dtype DI_F32 / DI_F16 / DI_BF16, softmax and sums in float32.
+ *   Keys that take part (all optional, combined): the first key_lengths[b] (int32, clamped to 0 .. S); key_mask (B, S) bytes != 0;
+ *   allowed (B, L, S) bytes != 0, any batch / row strides (0: shared).  K and V of keys excluded by the first two are never read
+ *   into a product; those excluded by `allowed` enter as 0 * v and have to be finite.  A row without keys gives zeros, lse -inf and
+ *   no gradient.
+ *   dropout_p: attention dropout from a counter-based hash of (seed + the device word of di_i2p_set_seed_ptr, row, key), the same
+ *   in forward and backward; p is rounded to a multiple of 2^-16.
+ * di_attention_fwd: out (B, L, heads * head_dim) dense; lse (B, heads, L) float32, log2-sum-exp2 of scale log2(e) q k (may be NULL).
+ * di_attention_bwd: grad_q dense, grad_k / grad_v (B, S, kv_heads * head_dim) with strides, every row written.
+ * workspace: the floats that the matching function returns (< 0: unsupported), private to the call until it has run. */
+typedef struct {
+  const void *q, *k, *v;
+  long long q_bs, q_rs, k_bs, k_rs, v_bs, v_rs;
+  const int32_t *key_lengths;
+  const uint8_t *key_mask;
+  long long key_mask_bs;
+  const uint8_t *allowed;
+  long long allowed_bs, allowed_rs;
+  int B, L, S, heads, kv_heads, head_dim, dtype;
+  float scale, dropout_p;
+  unsigned long long seed;
+} di_attention;
+long long di_attention_fwd_workspace_floats(const di_attention *t);
+long long di_attention_bwd_workspace_floats(const di_attention *t);
+int di_attention_fwd(const di_attention *t, void *out, float *lse, float *workspace, void *stream);
+int di_attention_bwd(const di_attention *t, const void *out, const float *lse, const void *grad_out, long long go_bs, long long go_rs,
+                     void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs, long long gv_rs,
+                     float *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
