@@ -24,7 +24,10 @@ FLAGS = ['-O3', '-std=c++17', '-fPIC', '-shared', '-Wno-cuda-compat', '-Wno-unus
 # per-file flags; DI_PACKED_FP32=1 (experiments only) compiles WITH the packed instructions
 # i2p_dense.hip: MFMA results in arch VGPRs (the accumulators are touched by a rare VALU rescale; with AGPR accumulators
 # the compiler moves all 32 of them to VGPRs and back around every block - 64 moves per 12 MFMAs)
-EXTRA = {'i2p_dense.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form']}
+# attention_*.hip: the same - scores and sums are touched by the vector unit between the products (AGPR accumulators cost a third of the
+# inner loop's instructions as moves)
+_VGPR_FORM = ['-mllvm', '-amdgpu-mfma-vgpr-form']
+EXTRA = {name: _VGPR_FORM for name in ('i2p_dense.hip', 'attention_f32.hip', 'attention_f16.hip', 'attention_bf16.hip')}
 if os.environ.get('DI_PACKED_FP32') == '1':
     FLAGS = [f for f in FLAGS if f not in ('-Xclang', '-target-feature', '-packed-fp32-ops')]
 

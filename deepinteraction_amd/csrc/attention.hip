@@ -36,8 +36,10 @@ static int plan_keys(const di_attention &t, Plan &p) {
   const int cus = device_cus();
   if (cus <= 0) return DI_ERR_LAUNCH;
   const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
-  p.big = t.S > 64;
-  const int per = 64 * (p.big ? key_tiles(t.dtype, DP) : 1), tile = DP * (t.dtype == DI_F32 ? 4 : 2) >= 256 ? 32 : 64;
+  const int most = key_tiles(t.dtype, DP);
+  p.big = 1;
+  while (p.big < most && 64 * p.big < t.S) p.big *= 2;
+  const int per = 64 * p.big, tile = DP * (t.dtype == DI_F32 ? 4 : 2) >= 256 ? 32 : 64;
   cut(p, (long long)t.B * t.kv_heads, t.S, per, rows, tile, 2ll * cus);
   return DI_OK;
 }

@@ -28,7 +28,7 @@ struct GqCfg {
   static constexpr int NP = (TILE * M::PPR + 255) / 256;
 };
 
-template <int TY, int DP, int MT, int WQ>
+template <int TY, int DP, int MT, int WQ, bool FULL>
 __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   using C = GqCfg<TY, DP, MT, WQ>;
   using M = Mm<TY, DP>;
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   const int rows = a.G * a.L, ntile = (rows + 15) / 16;
   const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
-  const unsigned char *km = a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
+  const unsigned char *km = !FULL || a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
   const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
 
   typename M::RF qf[MT][M::NK], gf[MT][M::NK];
@@ -73,26 +73,16 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
     if (ok && at.sp == 0 && wk == 0 && g == 0) a.delta[row_id + row[t]] = d;
 #pragma unroll
     for (int j = 0; j < M::ND; ++j) acc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
-    drow[t] = a.drop ? drop_row(seed_of(a), row_id + r) : 0;
+    drow[t] = FULL && a.drop ? drop_row(seed_of(a), row_id + r) : 0;
   }
   if (a.splits > 1 && k0 >= k1) return;
 
-  KeyStage<C> st;
-  if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
-  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
-    __syncthreads();
-    st.commit(lds, M::TRS, M::ROWS, C::V_AT);
-    const bool ragged = km != nullptr || t0 + C::TILE > k1;
-    if (ragged && threadIdx.x < C::TILE) {
-      const int s = t0 + threadIdx.x;
-      bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
-    }
-    __syncthreads();
-    if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
+  auto tile = [&](auto edge, int t0) {                          // one tile of keys; EDGE: keys are tested
+    constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;
-      if (t0 + kc >= k1) break;
+      if (EDGE && t0 + kc >= k1) break;
       f4 s[MT][M::NT], dp[MT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
@@ -108,14 +98,14 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
             dp[t][u] = M::dot(vf, gf[t][kk], dp[t][u]);
           }
         }
-        if (ragged) {
+        if (EDGE) {
           const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][u][r] = bb[r] == 0.f ? s[t][u][r] : -INFINITY;
         }
-        if (a.allowed != nullptr) {
+        if (FULL && a.allowed != nullptr) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
             if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, s[t][u]);
@@ -127,7 +117,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         f4 ds[M::NT];
 #pragma unroll
         for (int u = 0; u < M::NT; ++u) {
-          if (a.drop) {
+          if (FULL && a.drop) {
             const unsigned k4 = (unsigned)(t0 + kc + 16 * u + 4 * g) >> 2;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -149,6 +139,22 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         for (int t = 0; t < MT; ++t) acc[t][d] = M::acc(kf, df[t], acc[t][d]);
       }
     }
+  };
+
+  KeyStage<C> st;
+  if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
+  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
+    __syncthreads();
+    st.commit(lds, M::TRS, M::ROWS, C::V_AT);
+    const bool edge = FULL || t0 + C::TILE > k1;
+    if (edge && threadIdx.x < C::TILE) {
+      const int s = t0 + threadIdx.x;
+      bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
+    }
+    __syncthreads();
+    if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
+    if (edge) tile(std::true_type(), t0);
+    else tile(std::false_type(), t0);
   }
 
   if constexpr (WQ == 1) {                                      // add the four wavefronts (MT = 1)
@@ -185,22 +191,6 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   }
 }
 
-// gq = scale * the ranges' sums; a thread per 4 head dims
-template <int TY>
-__global__ __launch_bounds__(256) void attention_gq_join_kernel(Args a) {
-  using M = Mm<TY, 16>;
-  const int rows = a.G * a.L, q4 = a.D / 4;
-  const long long all = (long long)a.B * a.Hk * rows, id = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= all * q4) return;
-  const long long rid = id / q4;
-  const int d = 4 * (int)(id % q4), r = (int)(rid % rows), hk = (int)(rid / rows % a.Hk), b = (int)(rid / rows / a.Hk);
-  const int n = min(a.splits, (keys_of(a, b) + a.range - 1) / a.range);
-  f4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n; ++s) o += *reinterpret_cast<const f4 *>(a.part + (s * all + rid) * a.D + d);
-  const int head = r / a.L;
-  M::store4(a.gq + ((((long long)b * a.L + (r - head * a.L)) * a.Hk * a.G + hk * a.G + head) * a.D + d) * M::SZ, o * a.scale);
-}
-
 template <int TY, int DP, int NT>
 struct GkvCfg {
   using M = Mm<TY, DP>;
@@ -214,7 +204,7 @@ struct GkvCfg {
   static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f;
 };
 
-template <int TY, int DP, int NT>
+template <int TY, int DP, int NT, bool FULL>
 __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
   using C = GkvCfg<TY, DP, NT>;
   using M = Mm<TY, DP>;
@@ -235,7 +225,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     key[n] = key0 + (wave * NT + n) * 16 + i;
-    valid[n] = key[n] < nkeys && (a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
+    valid[n] = key[n] < nkeys && (!FULL || a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
 #pragma unroll
     for (int kk = 0; kk < M::NK; ++kk) {
       kf[n][kk] = M::row_frag_of(kb + key[n] * a.k_rs, kk, g, a.D, valid[n]);
@@ -244,7 +234,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
 #pragma unroll
     for (int d = 0; d < M::ND; ++d) gk[n][d] = gv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  const unsigned long long seed = a.drop ? seed_of(a) : 0;
+  const unsigned long long seed = FULL && a.drop ? seed_of(a) : 0;
 
   u4 qs[C::NP], gs[C::NP];
   float ls = INFINITY, de = 0.f;
@@ -307,7 +297,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         const int rfirst = t0 + rc + 16 * u + 4 * g;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if (a.allowed != nullptr) {
+          if (FULL && a.allowed != nullptr) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int rr = min(rfirst + r, rows - 1);
@@ -316,14 +306,17 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float pr = valid[n] ? __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale2, -l4[r])) : 0.f;
-            float keep = 1.f;
-            if (a.drop) {
+            // (a column is one key: whatever the column of an excluded key holds stays there, and is dropped at the end)
+            const float pr = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale2, -l4[r]));
+            if (FULL && a.drop) {
               const unsigned x = drop_pair(drop_row(seed, row_id + rfirst + r), (unsigned)key[n] >> 2, (key[n] & 2) != 0);
-              keep = ((key[n] & 1) ? x >> 16 : x & 0xffffu) >= a.drop ? a.keep_scale : 0.f;
+              const bool kept = ((key[n] & 1) ? x >> 16 : x & 0xffffu) >= a.drop;
+              p[n][u][r] = kept ? pr * C::P_SCALE : 0.f;          // the kept ones' scale: at the end
+              dp[n][r] = kept ? dp[n][r] * a.keep_scale : 0.f;
+            } else {
+              p[n][u][r] = pr * C::P_SCALE;
             }
-            p[n][u][r] = keep == 0.f ? 0.f : pr * C::P_SCALE;             // the kept ones' scale: at the end
-            ds[n][u][r] = pr * (dp[n][r] * keep - d4[r]);
+            ds[n][u][r] = pr * (dp[n][r] - d4[r]);
           }
         }
       }
@@ -346,6 +339,10 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (key[n] >= a.S) continue;
+    if (!valid[n]) {
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d) gk[n][d] = gv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
     if (a.splits > 1) {
       const long long rec = (((long long)at.sp * a.B + at.b) * a.Hk + at.hk) * a.S + key[n];
 #pragma unroll

@@ -11,6 +11,8 @@
 // in the 16-bit probabilities): the test is one comparison per tile against the lane's own scores, the exchange between lanes and
 // the correction of the sums run when any lane asks for them - a few times per row, not once per tile.
 #pragma once
+#include <type_traits>
+
 #include "attention.h"
 
 namespace di {
@@ -61,6 +63,10 @@ struct KeyStage {
   }
 };
 
+// max without the quieting of its operands (v_max_f32 x, x) that fmaxf needs for values that may be signalling NaN: two instructions less
+// a score.  A NaN score loses the comparison but stays a NaN in the exponential.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
 // 4 keys x 1 row of the (row, key) mask; keys past the end count as allowed (their scores are excluded by the bias)
 __device__ __forceinline__ void exclude(const unsigned char *row, int key, int S, f4 &s) {
 #pragma unroll
@@ -68,7 +74,8 @@ __device__ __forceinline__ void exclude(const unsigned char *row, int key, int S
     if (key + r < S && row[key + r] == 0) s[r] = -INFINITY;
 }
 
-template <int TY, int DP, int MT, int WQ>
+// FULL: with a key mask, a (query, key) mask or dropout; without them only the last tile of a range is tested key by key
+template <int TY, int DP, int MT, int WQ, bool FULL>
 __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
   using C = FwdCfg<TY, DP, MT, WQ>;
   using M = Mm<TY, DP>;
@@ -81,7 +88,7 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
   const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
   if (a.splits > 1 && k0 >= k1) return;                         // the join knows the sample's keys, too
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
-  const unsigned char *km = a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
+  const unsigned char *km = !FULL || a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
   const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
 
   typename M::RF qf[MT][M::NK];
@@ -102,25 +109,16 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
     for (int d = 0; d < M::ND; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
     m[t] = kLowest;
     l[t] = 0.f;
-    drow[t] = a.drop ? drop_row(seed_of(a), row_id + r) : 0;
+    drow[t] = FULL && a.drop ? drop_row(seed_of(a), row_id + r) : 0;
   }
 
-  KeyStage<C> st;
-  if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
-  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
-    __syncthreads();                                            // the last tile's reads are done
-    st.commit(lds, M::ROWS, M::TRS, C::V_AT);
-    const bool ragged = km != nullptr || t0 + C::TILE > k1;
-    if (ragged && threadIdx.x < C::TILE) {
-      const int s = t0 + threadIdx.x;
-      bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
-    }
-    __syncthreads();
-    if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
+  // one tile of keys; EDGE: keys are tested
+  auto tile = [&](auto edge, int t0) {
+    constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;                 // first key of the chunk in the tile
-      if (t0 + kc >= k1) break;
+      if (EDGE && t0 + kc >= k1) break;
       f4 s[MT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
@@ -132,14 +130,14 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
 #pragma unroll
           for (int t = 0; t < MT; ++t) s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
         }
-        if (ragged) {
+        if (EDGE) {
           const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][u][r] = bb[r] == 0.f ? s[t][u][r] : -INFINITY;
         }
-        if (a.allowed != nullptr) {
+        if (FULL && a.allowed != nullptr) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
             if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, s[t][u]);
@@ -151,7 +149,9 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
       for (int t = 0; t < MT; ++t) {
         mx[t] = kLowest;
 #pragma unroll
-        for (int u = 0; u < M::NT; ++u) mx[t] = fmaxf(fmaxf(fmaxf(s[t][u][0], s[t][u][1]), fmaxf(s[t][u][2], s[t][u][3])), mx[t]);
+        for (int u = 0; u < M::NT; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx[t] = larger(s[t][u][r], mx[t]);
         mx[t] *= a.scale2;
         over |= mx[t] > m[t] + 8.f;
       }
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) p[u][r] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], a.scale2, -m[t]));
           l[t] += (p[u][0] + p[u][1]) + (p[u][2] + p[u][3]);
-          if (a.drop) {
+          if (FULL && a.drop) {
             const unsigned k4 = (unsigned)(t0 + kc + 16 * u + 4 * g) >> 2;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -196,6 +196,22 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
         for (int t = 0; t < MT; ++t) o[t][d] = M::acc(vf, pf[t], o[t][d]);
       }
     }
+  };
+
+  KeyStage<C> st;
+  if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
+  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
+    __syncthreads();                                            // the last tile's reads are done
+    st.commit(lds, M::ROWS, M::TRS, C::V_AT);
+    const bool edge = FULL || t0 + C::TILE > k1;
+    if (edge && threadIdx.x < C::TILE) {
+      const int s = t0 + threadIdx.x;
+      bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
+    }
+    __syncthreads();
+    if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
+    if (edge) tile(std::true_type(), t0);
+    else tile(std::false_type(), t0);
   }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
@@ -261,38 +277,45 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
   }
 }
 
-// The ranges' states of a row joined; one 16-lane group per row, 4 head dims a lane and step.
-template <int TY>
+// The ranges' sums of a row joined: a wavefront per row, 4 head dims a lane, the other lanes on further ranges.  STATS: forward,
+// every range has its own maximum and sum; otherwise gq, plain sums.
+template <int TY, bool STATS>
 __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
   using M = Mm<TY, 16>;
-  const int i = threadIdx.x & 15;
-  const int rows = a.G * a.L;
-  const long long all = (long long)a.B * a.Hk * rows, id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int lane = threadIdx.x & 63;
+  const int rows = a.G * a.L, nd = a.D <= 16 ? 4 : a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32;      // lanes across the head dim
+  const long long all = (long long)a.B * a.Hk * rows, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (id >= all) return;
   const int r = (int)(id % rows), hk = (int)(id / rows % a.Hk), b = (int)(id / rows / a.Hk);
   const int n = min(a.splits, (keys_of(a, b) + a.range - 1) / a.range);
-  float top = kLowest;
-  for (int s = i; s < n; s += 16) top = fmaxf(top, a.part_ml[2 * (s * all + id)]);
-  top = row16_max(top);
-  float l = 0.f;
-  for (int s = i; s < n; s += 16) {
-    const float *p = a.part_ml + 2 * (s * all + id);
-    l = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - top), l);
-  }
-  l = row16_sum(l);
-  const float inv = l == 0.f ? 0.f : a.keep_scale / l;
-  if (a.lse != nullptr && i == 0) a.lse[id] = l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l);
-  const int head = r / a.L;
-  char *out = a.o + (((long long)b * a.L + (r - head * a.L)) * a.Hk * a.G + hk * a.G + head) * a.D * M::SZ;
-  for (int d = 4 * i; d < a.D; d += 64) {
-    f4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; ++s) {
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * all + id)] - top);
-      const f4 p = *reinterpret_cast<const f4 *>(a.part + (s * all + id) * a.D + d);
-      o += p * f;
+  float top = kLowest, l = 0.f;
+  if (STATS) {
+    for (int s = lane; s < n; s += 64) top = fmaxf(top, a.part_ml[2 * (s * all + id)]);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    for (int s = lane; s < n; s += 64) {
+      const float *p = a.part_ml + 2 * (s * all + id);
+      l = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - top), l);
     }
-    M::store4(out + d * M::SZ, o * inv);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+    if (a.lse != nullptr && lane == 0) a.lse[id] = l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l);
   }
+  const int d = 4 * (lane % nd);
+  f4 o = {0.f, 0.f, 0.f, 0.f};
+  if (d < a.D)
+    for (int s = lane / nd; s < n; s += 64 / nd) {
+      const f4 p = *reinterpret_cast<const f4 *>(a.part + (s * all + id) * a.D + d);
+      if (STATS) o += p * __builtin_amdgcn_exp2f(a.part_ml[2 * (s * all + id)] - top);
+      else o += p;
+    }
+  for (int x = nd; x < 64; x *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+  if (lane >= nd || d >= a.D) return;
+  const int head = r / a.L;
+  char *out = (STATS ? a.o : a.gq) + ((((long long)b * a.L + (r - head * a.L)) * a.Hk * a.G + hk * a.G + head) * a.D + d) * M::SZ;
+  M::store4(out, o * (STATS ? (l == 0.f ? 0.f : a.keep_scale / l) : a.scale));
 }
 
 }  // namespace at

@@ -6,6 +6,8 @@
 namespace di {
 namespace at {
 
+static bool needs_full(const Args &a) { return a.kmask != nullptr || a.allowed != nullptr || a.drop != 0; }
+
 template <class K>
 static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &a, hipStream_t s, const char *name) {
   if (grid <= 0) return DI_OK;
@@ -16,21 +18,27 @@ static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &
 
 template <int TY, int DP, int MT, int WQ>
 static int fwd(const Args &a, hipStream_t s) {
-  static LdsRaised raised;
-  return go(attention_fwd_kernel<TY, DP, MT, WQ>, raised, FwdCfg<TY, DP, MT, WQ>::LDS, (long long)a.B * a.splits * a.Hk * a.blocks, a, s,
-            "attention_fwd");
+  static LdsRaised plain, full;
+  const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
+  constexpr int lds = FwdCfg<TY, DP, MT, WQ>::LDS;
+  return needs_full(a) ? go(attention_fwd_kernel<TY, DP, MT, WQ, true>, full, lds, grid, a, s, "attention_fwd")
+                       : go(attention_fwd_kernel<TY, DP, MT, WQ, false>, plain, lds, grid, a, s, "attention_fwd");
 }
 template <int TY, int DP, int MT, int WQ>
 static int gq(const Args &a, hipStream_t s) {
-  static LdsRaised raised;
-  return go(attention_gq_kernel<TY, DP, MT, WQ>, raised, GqCfg<TY, DP, MT, WQ>::LDS, (long long)a.B * a.splits * a.Hk * a.blocks, a, s,
-            "attention_gq");
+  static LdsRaised plain, full;
+  const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
+  constexpr int lds = GqCfg<TY, DP, MT, WQ>::LDS;
+  return needs_full(a) ? go(attention_gq_kernel<TY, DP, MT, WQ, true>, full, lds, grid, a, s, "attention_gq")
+                       : go(attention_gq_kernel<TY, DP, MT, WQ, false>, plain, lds, grid, a, s, "attention_gq");
 }
 template <int TY, int DP, int NT>
 static int gkv(const Args &a, hipStream_t s) {
-  static LdsRaised raised;
-  return go(attention_gkv_kernel<TY, DP, NT>, raised, GkvCfg<TY, DP, NT>::LDS, (long long)a.B * a.splits * a.Hk * a.blocks, a, s,
-            "attention_gkv");
+  static LdsRaised plain, full;
+  const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
+  constexpr int lds = GkvCfg<TY, DP, NT>::LDS;
+  return needs_full(a) ? go(attention_gkv_kernel<TY, DP, NT, true>, full, lds, grid, a, s, "attention_gkv")
+                       : go(attention_gkv_kernel<TY, DP, NT, false>, plain, lds, grid, a, s, "attention_gkv");
 }
 
 static void take(Args &a, const Plan &p) {
@@ -55,7 +63,7 @@ int launch_fwd(const Args &args, const Plan &p, hipStream_t s) {
 #undef DI_AT_FWD
   if (rc != DI_OK || p.splits == 1) return rc;
   const long long all = (long long)a.B * a.Hk * a.G * a.L;
-  hipLaunchKernelGGL((attention_join_kernel<TY>), dim3((unsigned)((all + 15) / 16)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((attention_join_kernel<TY, true>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, a);
   return check_launch("attention_join");
 }
 
@@ -75,13 +83,16 @@ int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) 
 #undef DI_AT_GQ
   if (rc != DI_OK) return rc;
   if (pq.splits > 1) {
-    const long long n = (long long)a.B * a.Hk * a.G * a.L * (a.D / 4);
-    hipLaunchKernelGGL((attention_gq_join_kernel<TY>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    const long long all = (long long)a.B * a.Hk * a.G * a.L;
+    hipLaunchKernelGGL((attention_join_kernel<TY, false>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, a);
     if ((rc = check_launch("attention_gq_join")) != DI_OK) return rc;
   }
   if (a.S == 0) return DI_OK;
   take(a, pk);
-#define DI_AT_GKV(DP) rc = pk.big ? gkv<TY, DP, key_tiles(TY, DP)>(a, s) : gkv<TY, DP, 1>(a, s)
+#define DI_AT_GKV(DP)                                                                                                 \
+  rc = pk.big == 4 && key_tiles(TY, DP) >= 4   ? gkv<TY, DP, key_tiles(TY, DP) >= 4 ? 4 : 1>(a, s)                     \
+       : pk.big == 2 && key_tiles(TY, DP) >= 2 ? gkv<TY, DP, key_tiles(TY, DP) >= 2 ? 2 : 1>(a, s)                     \
+                                               : gkv<TY, DP, 1>(a, s)
   switch (padded(a.D)) {
     case 16: DI_AT_GKV(16); break;
     case 32: DI_AT_GKV(32); break;

@@ -6,7 +6,7 @@ namespace di {
 namespace at {
 
 struct Plan {
-  int big;                               // 0: up to 16 rows, 1: up to 64 rows (or keys), 2: more
+  int big;                               // rows: 0 = up to 16, 1 = up to 64, 2 = more; keys: tiles per wavefront
   int blocks, splits, range;
 };
 
