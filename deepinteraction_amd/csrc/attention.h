@@ -196,6 +196,7 @@ struct Args {
   int B, L, S, Hk, G, D;
   int splits, range;                     // key (or row) ranges of a split grid
   int blocks;                            // row blocks (or key blocks)
+  bool allowed_words;                    // every row of `allowed` starts on 4 bytes
   float scale2;                          // softmax scale * log2(e)
   float scale;
   unsigned drop;                         // threshold of 65536; 0 = no dropout
@@ -206,13 +207,21 @@ struct Args {
 
 __device__ __forceinline__ unsigned long long seed_of(const Args &a) { return a.seed + (a.seed_ptr != nullptr ? *a.seed_ptr : 0ull); }
 
-// block -> (row block, key head, split, sample); neighbours in this order - which read the same keys, or other heads of the same
-// rows of memory - are on one XCD and share its L2
+// block -> (row block, key head, split, sample).  The blocks of one (sample, split) read the same memory rows - the same keys, or other
+// heads of them - and go to one XCD, whose L2 they share; the (sample, split) units are dealt out to the XCDs in turn, so that samples
+// of different lengths load them evenly.  Fewer than 8 units (or the last few): consecutive chunks of the block list per XCD.
 struct Where {
   int blk, hk, sp, b;
 };
 __device__ __forceinline__ Where where(const Args &a) {
-  int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int unit = a.blocks * a.Hk, units = a.B * a.splits, even = units / 8 * 8 * unit;
+  int id = blockIdx.x;
+  if (id < even) {
+    const int xcd = id % 8, j = id / 8;
+    id = (j / unit * 8 + xcd) * unit + j % unit;
+  } else {
+    id = even + xcd_remap(id - even, units * unit - even);
+  }
   Where w;
   w.blk = id % a.blocks; id /= a.blocks;
   w.hk = id % a.Hk; id /= a.Hk;

@@ -2,20 +2,22 @@
 // Reference: the decoder layer's attention to the BEV map (decoder_utils.py:96-103, :421-485), the RoI blocks' attention among the
 // queries of a view (:743-746) and the ray decoder's attention to an image column (fusion_transformerv4.py:715-769).
 #include <math.h>
+#include <stdlib.h>
 
 #include "attention_plan.h"
 
 namespace di {
 namespace at {
 
-// Row blocks, and - where they are fewer than `want` - ranges of the walked side (multiples of `tile`) so that about `want`
-// workgroups run.
-static void cut(Plan &p, long long problems, int rows, int per_block, int walked, int tile, long long want) {
+// Blocks, and - where they are fewer than `want` - ranges of the walked side (whole tiles, at least `least` of them) so that about
+// `want` workgroups run.
+static void cut(Plan &p, long long problems, int rows, int per_block, int walked, int tile, int least, long long want) {
   p.blocks = (rows + per_block - 1) / per_block;
   const long long n = problems * (p.blocks > 0 ? p.blocks : 1);
   const int tiles = walked > 0 ? (int)(((long long)walked + tile - 1) / tile) : 1;
   long long splits = n > 0 ? want / n : 1;
-  splits = splits < 1 ? 1 : (splits > tiles ? tiles : splits);
+  if (splits > tiles / least) splits = tiles / least;
+  if (splits < 1) splits = 1;
   const int per = (int)((tiles + splits - 1) / splits);
   p.range = per > 0x7fffffff / tile ? 0x7fffffff : per * tile;
   p.splits = (tiles + per - 1) / per;
@@ -24,28 +26,57 @@ static void cut(Plan &p, long long problems, int rows, int per_block, int walked
 static int plan_rows(const di_attention &t, Plan &p) {
   const int cus = device_cus();
   if (cus <= 0) return DI_ERR_LAUNCH;
+  static const int W = getenv("AT_W") ? atoi(getenv("AT_W")) : 2, W1 = getenv("AT_W1") ? atoi(getenv("AT_W1")) : 4;
   const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
-  p.big = rows <= 16 ? 0 : (rows <= 64 ? 1 : 2);
-  const int per = p.big == 0 ? 16 : (p.big == 1 ? 64 : 64 * row_tiles(DP));
-  const int tile = p.big == 0 && t.dtype != DI_F32 ? 128 : 64;
-  cut(p, (long long)t.B * t.kv_heads, rows, per, t.S, tile, 4ll * cus);
+  const long long problems = (long long)t.B * t.kv_heads;
+  if (rows <= 16) {
+    p.big = 0;
+    cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, (long long)W1 * cus);
+    return DI_OK;
+  }
+  p.big = 2;
+  cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, (long long)W * cus * (t.key_lengths ? 2 : 1));
+  if (rows <= 64 || problems * p.blocks * p.splits < cus) {
+    p.big = 1;
+    cut(p, problems, rows, 64, t.S, 64, 4, (long long)W * cus * (t.key_lengths ? 2 : 1));
+  }
   return DI_OK;
 }
 
 static int plan_keys(const di_attention &t, Plan &p) {
   const int cus = device_cus();
   if (cus <= 0) return DI_ERR_LAUNCH;
-  const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
-  const int most = key_tiles(t.dtype, DP);
-  p.big = 1;
-  while (p.big < most && 64 * p.big < t.S) p.big *= 2;
-  const int per = 64 * p.big, tile = DP * (t.dtype == DI_F32 ? 4 : 2) >= 256 ? 32 : 64;
-  cut(p, (long long)t.B * t.kv_heads, t.S, per, rows, tile, 2ll * cus);
+  const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L, least = least_key_tiles(DP);
+  const int tile = tile_rows(t.dtype, DP);
+  const long long problems = (long long)t.B * t.kv_heads;
+  static const int W = getenv("AT_WK") ? atoi(getenv("AT_WK")) : 2;
+  const int S = t.S > 0 ? t.S : 1;                              // without keys, one block still writes gq's zeros
+  for (p.big = key_tiles(t.dtype, DP); p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
+    if (32 * p.big >= t.S) continue;
+    cut(p, problems, S, 64 * p.big, rows, tile, 4, (long long)W * cus);
+    if (problems * p.blocks * p.splits >= cus) return DI_OK;
+  }
+  cut(p, problems, S, 64 * p.big, rows, tile, 4, (long long)W * cus);
   return DI_OK;
 }
 
+// floats of the backward's workspace: delta | the sums of gq | the sums of gk and gv.  Two launches: gq's are joined before the others
+// are written.
+struct Room {
+  long long gq, gkv;
+};
+static Room room_of(const di_attention &t, const Plan &p, const Plan &k) {
+  const long long rows = (long long)t.B * t.heads * t.L, keys = (long long)t.B * t.kv_heads * t.S;
+  const int n = one_launch(padded(t.head_dim)) ? k.blocks : p.splits;
+  Room r;
+  r.gq = n > 1 ? n * rows * t.head_dim : 0;
+  r.gkv = k.splits > 1 ? 2ll * k.splits * keys * t.head_dim : 0;
+  return r;
+}
+
 static bool aligned(const void *p, long long bs, long long rs, int size) {
-  return ((uintptr_t)p & 15) == 0 && (bs * size) % 16 == 0 && (rs * size) % 16 == 0;
+  // a tile's rows (128 at the most) are addressed with 32 bits from its first
+  return ((uintptr_t)p & 15) == 0 && (bs * size) % 16 == 0 && (rs * size) % 16 == 0 && rs >= 0 && rs * size < (1ll << 24);
 }
 
 static int check(const di_attention *t) {
@@ -63,9 +94,9 @@ static int check(const di_attention *t) {
   DI_REQUIRE(most <= 0x7fffffff / 2, "attention: too many rows for one launch");
   const int sz = t->dtype == DI_F32 ? 4 : 2;
   if (t->B == 0) return DI_OK;
-  DI_REQUIRE(t->L == 0 || (t->q != nullptr && aligned(t->q, t->q_bs, t->q_rs, sz)), "attention: q must start and step on 16 bytes");
+  DI_REQUIRE(t->L == 0 || (t->q != nullptr && aligned(t->q, t->q_bs, t->q_rs, sz)), "attention: q must start and step on 16 bytes, its rows less than 16 MB apart");
   DI_REQUIRE(t->S == 0 || (t->k != nullptr && t->v != nullptr && aligned(t->k, t->k_bs, t->k_rs, sz) && aligned(t->v, t->v_bs, t->v_rs, sz)),
-             "attention: k and v must start and step on 16 bytes");
+             "attention: k and v must start and step on 16 bytes, their rows less than 16 MB apart");
   return DI_OK;
 }
 
@@ -77,8 +108,11 @@ static Args args_of(const di_attention *t) {
   a.k_bs = t->k_bs * sz; a.k_rs = t->k_rs * sz;
   a.v_bs = t->v_bs * sz; a.v_rs = t->v_rs * sz;
   a.klen = t->key_lengths;
-  a.kmask = t->key_mask; a.kmask_bs = t->key_mask_bs;
-  a.allowed = t->allowed; a.allowed_bs = t->allowed_bs; a.allowed_rs = t->allowed_rs;
+  if (t->S > 0) {                                              // no keys: nothing that a mask could exclude
+    a.kmask = t->key_mask; a.kmask_bs = t->key_mask_bs;
+    a.allowed_words = ((uintptr_t)t->allowed & 3) == 0 && t->allowed_bs % 4 == 0 && t->allowed_rs % 4 == 0;
+    a.allowed = t->allowed; a.allowed_bs = t->allowed_bs; a.allowed_rs = t->allowed_rs;
+  }
   a.B = t->B; a.L = t->L; a.S = t->S; a.Hk = t->kv_heads; a.G = t->heads / t->kv_heads; a.D = t->head_dim;
   a.scale = t->scale;
   a.scale2 = t->scale * kLog2e;
@@ -108,9 +142,8 @@ long long di_attention_bwd_workspace_floats(const di_attention *t) {
   if (check(t) != DI_OK) return -1;
   Plan p, k;
   if (plan_rows(*t, p) != DI_OK || plan_keys(*t, k) != DI_OK) return -1;
-  const long long rows = (long long)t->B * t->heads * t->L, keys = (long long)t->B * t->kv_heads * t->S;
-  const long long gq = p.splits == 1 ? 0 : p.splits * rows * t->head_dim, gkv = k.splits == 1 ? 0 : 2ll * k.splits * keys * t->head_dim;
-  return (rows + 3) / 4 * 4 + (gq > gkv ? gq : gkv);            // delta | one launch's sums, then the other's
+  const Room r = room_of(*t, p, k);
+  return ((long long)t->B * t->heads * t->L + 3) / 4 * 4 + r.gq + r.gkv;
 }
 
 int di_attention_fwd(const di_attention *t, void *out, float *lse, float *workspace, void *stream) {
@@ -154,10 +187,10 @@ int di_attention_bwd(const di_attention *t, const void *out, const float *lse, c
   a.go_bs = go_bs * sz; a.go_rs = go_rs * sz;
   a.gq = (char *)gq; a.gk = (char *)gk; a.gv = (char *)gv;
   a.gk_bs = gk_bs * sz; a.gk_rs = gk_rs * sz; a.gv_bs = gv_bs * sz; a.gv_rs = gv_rs * sz;
-  const long long rows = (long long)t->B * t->heads * t->L, keys = (long long)t->B * t->kv_heads * t->S;
   a.delta = workspace;
-  a.part = a.part_k = workspace + (rows + 3) / 4 * 4;
-  a.part_v = a.part_k + k.splits * keys * t->head_dim;
+  a.part = workspace + ((long long)t->B * t->heads * t->L + 3) / 4 * 4;
+  a.part_k = a.part + room_of(*t, p, k).gq;
+  a.part_v = a.part_k + (long long)k.splits * t->B * t->kv_heads * t->S * t->head_dim;
   hipStream_t s = (hipStream_t)stream;
   return t->dtype == DI_F32   ? launch_bwd<DI_F32>(a, p, k, s)
          : t->dtype == DI_F16 ? launch_bwd<DI_F16>(a, p, k, s)

@@ -9,6 +9,10 @@
 //   gq:      S^T = K Q^T, dP^T = V go^T (16 keys x 16 rows), gq^T += K^T dS^T
 //   gk, gv:  S = Q K^T, dP = go V^T (16 rows x 16 keys), gv^T += go^T P, gk^T += Q^T dS
 // Where there are few blocks, the walked side is split over workgroups and their float32 sums are added in a fixed order.
+// Heads of up to 32 dims: ONE launch.  The key-block kernel forms gq as well - every wavefront from its own keys, its score gradients
+// transposed through LDS, the four shares added per tile of rows, the key blocks' sums joined by the forward's second launch.  The
+// scores are formed once, and rows of few dims make the key blocks' sums small (rows x D floats per 128 - 256 keys); wide heads would
+// write more sums than the second pass over the keys costs.
 #pragma once
 #include "attention_fwd.h"
 
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
-            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, s[t][u]);
+            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words, s[t][u]);
         }
       }
       typename M::PF df[MT];
@@ -142,6 +146,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   };
 
   KeyStage<C> st;
+  st.init(a);
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
   for (int t0 = k0; t0 < k1; t0 += C::TILE) {
     __syncthreads();
@@ -191,22 +196,28 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   }
 }
 
-template <int TY, int DP, int NT>
+// GQ: the launch forms gq as well (narrow heads)
+template <int TY, int DP, int NT, bool GQ>
 struct GkvCfg {
   using M = Mm<TY, DP>;
-  static constexpr int BR = DP * M::SZ >= 256 ? 32 : 64;        // rows per tile
+  static constexpr int BR = DP * M::SZ >= 256 || (GQ && DP > 16) ? 32 : 64;        // rows per tile
   static constexpr int KEYS = 64 * NT;
   static constexpr int G_AT = BR * M::TRS, ST_AT = 2 * G_AT;    // both tiles are read in rows and transposed
-  static constexpr int LDS = ST_AT + 2 * BR * 4;
+  static constexpr int K_AT = ST_AT + 2 * BR * 4;               // GQ: the block's keys,
+  static constexpr int DS_AT = K_AT + KEYS * M::TRS;            // each wavefront's score gradients as (key, row),
+  static constexpr int DS_ROW = M::CH * M::SZ + (M::WIDE ? 16 : 32), DS_WAVE = 16 * NT * DS_ROW;
+  static constexpr int RED_AT = DS_AT + 4 * DS_WAVE;            // and its share of gq of the tile's rows, float32
+  static constexpr int RED_ROW = DP + 4;
+  static constexpr int LDS = GQ ? RED_AT + 4 * BR * RED_ROW * 4 : K_AT;
   static constexpr int NP = (BR * M::PPR + 255) / 256;
   // P of a normalised row is about 1 / S: in float16 it is scaled by 2^14 (the largest power of two whose product with 1 is finite
   // with room to spare) so that probabilities down to 2^-28 keep their 11 bits; exact to undo
   static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f;
 };
 
-template <int TY, int DP, int NT, bool FULL>
+template <int TY, int DP, int NT, bool GQ, bool FULL>
 __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
-  using C = GkvCfg<TY, DP, NT>;
+  using C = GkvCfg<TY, DP, NT, GQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
   float *slse = reinterpret_cast<float *>(lds + C::ST_AT), *sdelta = slse + C::BR;
@@ -214,7 +225,10 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
   const Where at = where(a);
   const int rows = a.G * a.L, nkeys = keys_of(a, at.b);
   const int key0 = at.blk * C::KEYS;
-  const int r0 = at.sp * a.range, r1 = key0 < nkeys ? min(r0 + a.range, rows) : r0;     // a block without keys: zeros
+  // a block without keys: zeros (the only block: gq's zeros, too)
+  const int r0 = at.sp * a.range, r1 = key0 < nkeys || (GQ && a.blocks == 1) ? min(r0 + a.range, rows) : r0;
+  const bool whole = key0 + C::KEYS <= nkeys && (!FULL || a.kmask == nullptr);
+  const int waves = min(4, max(1, (nkeys - key0 + 16 * NT - 1) / (16 * NT)));             // wavefronts with keys
   const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
 
@@ -235,51 +249,101 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
     for (int d = 0; d < M::ND; ++d) gk[n][d] = gv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
   }
   const unsigned long long seed = FULL && a.drop ? seed_of(a) : 0;
+  if constexpr (GQ) {                                           // the keys once more, for the products that contract over them
+    for (int e = tid; e < C::KEYS * M::PPR; e += 256) {
+      const int k = e / M::PPR, p = e % M::PPR, s = key0 + k;
+      u4 x = {0, 0, 0, 0};
+      if (s < nkeys && p * 16 < a.D * M::SZ && (!FULL || a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + s] != 0))
+        x = *reinterpret_cast<const u4 *>(kb + s * a.k_rs + p * 16);
+      *reinterpret_cast<u4 *>(lds + C::K_AT + k * M::TRS + p * 16) = x;
+    }
+  }
 
-  u4 qs[C::NP], gs[C::NP];
+  // rows of Q and go as KeyStage holds keys; a tile that lies in one head has a uniform base
+  constexpr int STEP = 256 / M::PPR;
+  u4 qs[C::NP], gs[C::NP], os[C::NP];                           // os: GQ forms delta from the forward's output
   float ls = INFINITY, de = 0.f;
+  const int piece = tid % M::PPR, first = tid / M::PPR;
+  const bool in = piece * 16 < a.D * M::SZ && (C::BR >= STEP || first < C::BR);
+  const unsigned qo = (unsigned)(first * a.q_rs) + piece * 16, go = (unsigned)(first * a.go_rs) + piece * 16;
+  const char *qb = a.q + at.b * a.q_bs, *gb = a.go + at.b * a.go_bs;
+  const long long o_rs = (long long)a.Hk * a.G * a.D * M::SZ;
+  const unsigned oo = (unsigned)(first * o_rs) + piece * 16;
+  const char *ob = a.o + at.b * a.L * o_rs;
   auto fetch = [&](int t0) {
+    const int head0 = a.G == 1 ? 0 : t0 / a.L, l0 = t0 - head0 * a.L;
+    if (t0 + C::BR <= r1 && l0 + C::BR <= a.L) {
+      const long long col = (long long)(at.hk * a.G + head0) * a.D * M::SZ;
+      const char *qt = qb + l0 * a.q_rs + col, *gt = gb + l0 * a.go_rs + col, *ot = ob + l0 * o_rs + col;
 #pragma unroll
-    for (int j = 0; j < C::NP; ++j) {
-      const int e = tid + 256 * j, rr = e / M::PPR, p = e % M::PPR, r = t0 + rr;
-      qs[j] = gs[j] = u4{0, 0, 0, 0};
-      if (r < r1 && rr < C::BR && p * 16 < a.D * M::SZ) {
-        const int head = a.G == 1 ? 0 : r / a.L, l = r - head * a.L;
-        const long long col = (long long)(at.hk * a.G + head) * a.D * M::SZ + p * 16;
-        qs[j] = *reinterpret_cast<const u4 *>(a.q + at.b * a.q_bs + l * a.q_rs + col);
-        gs[j] = *reinterpret_cast<const u4 *>(a.go + at.b * a.go_bs + l * a.go_rs + col);
+      for (int j = 0; j < C::NP; ++j) {
+        qs[j] = gs[j] = os[j] = u4{0, 0, 0, 0};
+        if (in) {
+          qs[j] = *reinterpret_cast<const u4 *>(qt + j * STEP * a.q_rs + qo);
+          gs[j] = *reinterpret_cast<const u4 *>(gt + j * STEP * a.go_rs + go);
+          if (GQ) os[j] = *reinterpret_cast<const u4 *>(ot + j * STEP * o_rs + oo);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::NP; ++j) {
+        const int r = t0 + first + j * STEP;
+        qs[j] = gs[j] = os[j] = u4{0, 0, 0, 0};
+        if (in && r < r1) {
+          const int head = a.G == 1 ? 0 : r / a.L, l = r - head * a.L;
+          const long long col = (long long)(at.hk * a.G + head) * a.D * M::SZ + piece * 16;
+          qs[j] = *reinterpret_cast<const u4 *>(qb + l * a.q_rs + col);
+          gs[j] = *reinterpret_cast<const u4 *>(gb + l * a.go_rs + col);
+          if (GQ) os[j] = *reinterpret_cast<const u4 *>(ob + l * o_rs + col);
+        }
       }
     }
     if (tid < C::BR) {
       const bool ok = t0 + tid < r1;
       ls = ok ? a.lse[row_id + t0 + tid] : INFINITY;
-      de = ok ? a.delta[row_id + t0 + tid] : 0.f;
+      if (!GQ) de = ok ? a.delta[row_id + t0 + tid] : 0.f;
     }
   };
   if (r0 < r1) fetch(r0);
   for (int t0 = r0; t0 < r1; t0 += C::BR) {
     __syncthreads();
+    if (C::BR >= STEP || first < C::BR) {
 #pragma unroll
-    for (int j = 0; j < C::NP; ++j) {
-      const int e = tid + 256 * j, rr = e / M::PPR, p = e % M::PPR;
-      if (C::BR * M::PPR % 256 == 0 || rr < C::BR) {
-        *reinterpret_cast<u4 *>(lds + rr * M::TRS + p * 16) = qs[j];
-        *reinterpret_cast<u4 *>(lds + C::G_AT + rr * M::TRS + p * 16) = gs[j];
+      for (int j = 0; j < C::NP; ++j) {
+        *reinterpret_cast<u4 *>(lds + (first + j * STEP) * M::TRS + piece * 16) = qs[j];
+        *reinterpret_cast<u4 *>(lds + C::G_AT + (first + j * STEP) * M::TRS + piece * 16) = gs[j];
+        if (GQ) {
+          float d = M::widen_dot({gs[j]}, {os[j]});
+#pragma unroll
+          for (int x = 1; x < M::PPR; x *= 2) d += __shfl_xor(d, x);
+          if (piece == 0) sdelta[first + j * STEP] = d;
+        }
       }
     }
     if (tid < C::BR) {
       slse[tid] = ls == -INFINITY ? INFINITY : ls;
-      sdelta[tid] = de;
+      if (!GQ) sdelta[tid] = de;
     }
     __syncthreads();
     if (t0 + C::BR < r1) fetch(t0 + C::BR);
 #pragma unroll 1
     for (int rc = 0; rc < C::BR; rc += M::CH) {
-      if (t0 + rc >= r1) break;
+      if (t0 + rc >= r1 || (GQ && wave >= waves)) break;
       typename M::PF pf[NT], df[NT];
       f4 p[NT][M::NT], ds[NT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
+        const int rfirst = t0 + rc + 16 * u + 4 * g;
+        unsigned char may[NT][4];                               // in flight behind the products
+        if (FULL && a.allowed != nullptr) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int rr = min(rfirst + r, rows - 1), head = a.G == 1 ? 0 : rr / a.L;
+            const unsigned char *line = a.allowed + at.b * a.allowed_bs + (rr - head * a.L) * a.allowed_rs;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) may[n][r] = line[min(key[n], a.S - 1)];
+          }
+        }
         f4 s[NT], dp[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n] = dp[n] = f4{0.f, 0.f, 0.f, 0.f};
@@ -294,15 +358,11 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
           }
         }
         const f4 l4 = *reinterpret_cast<const f4 *>(slse + rc + 16 * u + 4 * g), d4 = *reinterpret_cast<const f4 *>(sdelta + rc + 16 * u + 4 * g);
-        const int rfirst = t0 + rc + 16 * u + 4 * g;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (FULL && a.allowed != nullptr) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int rr = min(rfirst + r, rows - 1);
-              if (valid[n] && a.allowed[at.b * a.allowed_bs + (rr % a.L) * a.allowed_rs + key[n]] == 0) s[n][r] = -INFINITY;
-            }
+            for (int r = 0; r < 4; ++r) s[n][r] = may[n][r] != 0 ? s[n][r] : -INFINITY;
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -320,10 +380,50 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
           }
         }
       }
+      if (GQ && !whole) {                                       // gq sums over the columns: those of excluded keys have to be zero
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int u = 0; u < M::NT; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ds[n][u][r] = valid[n] ? ds[n][u][r] : 0.f;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         pf[n] = M::pack(p[n]);
         df[n] = M::pack(ds[n]);
+      }
+      if constexpr (GQ) {
+        // dS leaves as (key, row) rows of the wavefront's own buffer - a lane holds four rows of one key - and comes back transposed as
+        // the operand of gq^T = K^T dS^T; LDS serves a wavefront in order, no barrier
+        char *mine = lds + C::DS_AT + wave * C::DS_WAVE;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          char *at_key = mine + (16 * n + i) * C::DS_ROW + 4 * g * M::SZ;
+          if constexpr (M::WIDE) {
+            *reinterpret_cast<u4 *>(at_key) = df[n].v;
+          } else {
+            *reinterpret_cast<u2 *>(at_key) = u2{df[n].v[0], df[n].v[1]};
+            *reinterpret_cast<u2 *>(at_key + 32) = u2{df[n].v[2], df[n].v[3]};
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+        float *red = reinterpret_cast<float *>(lds + C::RED_AT) + (wave * C::BR + rc) * C::RED_ROW;
+#pragma unroll
+        for (int d = 0; d < M::ND; ++d) {
+          f4 gq[M::NT];
+#pragma unroll
+          for (int u = 0; u < M::NT; ++u) gq[u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 16 * NT; c += M::CH) {
+            const typename M::TF kt = M::tr_frag(lds + C::K_AT, M::TRS, wave * 16 * NT + c, d, i, g);
+#pragma unroll
+            for (int u = 0; u < M::NT; ++u) gq[u] = M::acc(kt, {M::tr_frag(mine, C::DS_ROW, c, u, i, g).v}, gq[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < M::NT; ++u) *reinterpret_cast<f4 *>(red + (16 * u + i) * C::RED_ROW + 16 * d + 4 * g) = gq[u];
+        }
+        __builtin_amdgcn_wave_barrier();
       }
 #pragma unroll
       for (int d = 0; d < M::ND; ++d) {
@@ -333,6 +433,22 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         const typename M::TF qt = M::tr_frag(lds, M::TRS, rc, d, i, g);
 #pragma unroll
         for (int n = 0; n < NT; ++n) gk[n][d] = M::acc(qt, df[n], gk[n][d]);
+      }
+    }
+    if constexpr (GQ) {                                         // the wavefronts' shares of the tile's gq
+      __syncthreads();
+      const float *red = reinterpret_cast<const float *>(lds + C::RED_AT);
+      for (int e = tid; e < C::BR * (DP / 4); e += 256) {
+        const int rr = e / (DP / 4), d = 4 * (e % (DP / 4)), r = t0 + rr;
+        if (r >= r1 || d >= a.D) continue;
+        f4 x = *reinterpret_cast<const f4 *>(red + rr * C::RED_ROW + d);
+        for (int w = 1; w < waves; ++w) x += *reinterpret_cast<const f4 *>(red + (w * C::BR + rr) * C::RED_ROW + d);
+        if (a.blocks > 1) {
+          *reinterpret_cast<f4 *>(a.part + ((long long)at.blk * a.B * a.Hk * rows + row_id + r) * a.D + d) = x;
+        } else {
+          const int head = a.G == 1 ? 0 : r / a.L;
+          M::store4(a.gq + (((long long)at.b * a.L + (r - head * a.L)) * o_rs) + ((at.hk * a.G + head) * a.D + d) * M::SZ, x * a.scale);
+        }
       }
     }
   }
@@ -379,7 +495,7 @@ __global__ __launch_bounds__(256) void attention_gkv_join_kernel(Args a) {
   }
   const long long col = ((long long)hk * a.D + d) * M::SZ;
   M::store4(a.gk + b * a.gk_bs + s * a.gk_rs + col, k * a.scale);
-  M::store4(a.gv + b * a.gv_bs + s * a.gv_rs + col, v * (a.keep_scale / GkvCfg<TY, 16, 1>::P_SCALE));
+  M::store4(a.gv + b * a.gv_bs + s * a.gv_rs + col, v * (a.keep_scale / GkvCfg<TY, 16, 2, true>::P_SCALE));
 }
 
 }  // namespace at

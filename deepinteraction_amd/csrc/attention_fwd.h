@@ -31,33 +31,54 @@ struct FwdCfg {
   static constexpr int NP = (TILE * M::PPR + 255) / 256;        // pieces per thread, K and V each
 };
 
-// the staged loads of a tile of keys: key rows t0 .. of K and V, zeros where there is no key (so that no NaN of an excluded key
-// or of memory behind the last one reaches a product)
+// The staged loads of a tile of keys: rows t0 .. of K and V, zeros where there is no key (so that no NaN of an excluded key or of
+// memory behind the last one reaches a product).  Thread e holds piece e % PPR of the rows e / PPR + j 256 / PPR: a uniform base per
+// tile and j, and one 32-bit lane offset each for K and V that never changes.
 template <class C>
 struct KeyStage {
+  using M = typename C::M;
+  static constexpr int STEP = 256 / M::PPR;                     // rows per piece index j
   u4 k[C::NP], v[C::NP];
+  unsigned ko, vo;
+  int key;
+  bool in;                                                      // the piece lies within the head dim (and the tile)
+  __device__ __forceinline__ void init(const Args &a) {
+    const int p = threadIdx.x % M::PPR;
+    key = threadIdx.x / M::PPR;
+    ko = (unsigned)(key * a.k_rs) + p * 16;
+    vo = (unsigned)(key * a.v_rs) + p * 16;
+    in = p * 16 < a.D * M::SZ && (C::TILE >= STEP || key < C::TILE);
+  }
   __device__ __forceinline__ void fetch(const Args &a, const char *kb, const char *vb, const unsigned char *km, int t0, int k1) {
-    using M = typename C::M;
+    const char *kt = kb + t0 * a.k_rs, *vt = vb + t0 * a.v_rs;
+    if (km == nullptr && t0 + C::TILE <= k1) {
 #pragma unroll
-    for (int j = 0; j < C::NP; ++j) {
-      const int e = threadIdx.x + 256 * j, key = e / M::PPR, p = e % M::PPR, s = t0 + key;
-      k[j] = v[j] = u4{0, 0, 0, 0};
-      bool ok = s < k1 && key < C::TILE && p * 16 < a.D * M::SZ;
-      if (km != nullptr && ok) ok = km[s] != 0;
-      if (ok) {
-        k[j] = *reinterpret_cast<const u4 *>(kb + s * a.k_rs + p * 16);
-        v[j] = *reinterpret_cast<const u4 *>(vb + s * a.v_rs + p * 16);
+      for (int j = 0; j < C::NP; ++j) {
+        k[j] = v[j] = u4{0, 0, 0, 0};
+        if (in) {
+          k[j] = *reinterpret_cast<const u4 *>(kt + j * STEP * a.k_rs + ko);
+          v[j] = *reinterpret_cast<const u4 *>(vt + j * STEP * a.v_rs + vo);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::NP; ++j) {
+        const int s = t0 + key + j * STEP;
+        k[j] = v[j] = u4{0, 0, 0, 0};
+        if (in && s < k1 && (km == nullptr || km[s] != 0)) {
+          k[j] = *reinterpret_cast<const u4 *>(kt + j * STEP * a.k_rs + ko);
+          v[j] = *reinterpret_cast<const u4 *>(vt + j * STEP * a.v_rs + vo);
+        }
       }
     }
   }
   __device__ __forceinline__ void commit(char *lds, int kstride, int vstride, int v_at) {
-    using M = typename C::M;
+    const int p = threadIdx.x % M::PPR;
+    if (C::TILE >= STEP || key < C::TILE) {
 #pragma unroll
-    for (int j = 0; j < C::NP; ++j) {
-      const int e = threadIdx.x + 256 * j, key = e / M::PPR, p = e % M::PPR;
-      if (C::TILE * M::PPR % 256 == 0 || key < C::TILE) {
-        *reinterpret_cast<u4 *>(lds + key * kstride + p * 16) = k[j];
-        *reinterpret_cast<u4 *>(lds + v_at + key * vstride + p * 16) = v[j];
+      for (int j = 0; j < C::NP; ++j) {
+        *reinterpret_cast<u4 *>(lds + (key + j * STEP) * kstride + p * 16) = k[j];
+        *reinterpret_cast<u4 *>(lds + v_at + (key + j * STEP) * vstride + p * 16) = v[j];
       }
     }
   }
@@ -67,16 +88,25 @@ struct KeyStage {
 // a score.  A NaN score loses the comparison but stays a NaN in the exponential.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 
-// 4 keys x 1 row of the (row, key) mask; keys past the end count as allowed (their scores are excluded by the bias)
-__device__ __forceinline__ void exclude(const unsigned char *row, int key, int S, f4 &s) {
+// 4 keys x 1 row of the (row, key) mask; keys past the end count as allowed (their scores are excluded by the bias).  `words`: rows
+// start on 4 bytes, and key is a multiple of 4
+__device__ __forceinline__ void exclude(const unsigned char *row, int key, int S, bool words, f4 &s) {
+  unsigned w = 0x01010101u;
+  if (words && key + 4 <= S) {
+    w = *reinterpret_cast<const unsigned *>(row + key);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (key + r < S && row[key + r] == 0) w &= ~(0xffu << (8 * r));
+  }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (key + r < S && row[key + r] == 0) s[r] = -INFINITY;
+    if ((w >> (8 * r) & 0xffu) == 0) s[r] = -INFINITY;
 }
 
 // FULL: with a key mask, a (query, key) mask or dropout; without them only the last tile of a range is tested key by key
 template <int TY, int DP, int MT, int WQ, bool FULL>
-__global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
+__global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attention_fwd_kernel(Args a) {
   using C = FwdCfg<TY, DP, MT, WQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
@@ -140,7 +170,7 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
-            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, s[t][u]);
+            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words, s[t][u]);
         }
       }
       float mx[MT];
@@ -199,6 +229,7 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
   };
 
   KeyStage<C> st;
+  st.init(a);
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
   for (int t0 = k0; t0 < k1; t0 += C::TILE) {
     __syncthreads();                                            // the last tile's reads are done
@@ -277,39 +308,37 @@ __global__ __launch_bounds__(256) void attention_fwd_kernel(Args a) {
   }
 }
 
-// The ranges' sums of a row joined: a wavefront per row, 4 head dims a lane, the other lanes on further ranges.  STATS: forward,
+// The ranges' sums of a row joined: `group` lanes per row, 4 head dims a lane, the other lanes on further ranges.  STATS: forward,
 // every range has its own maximum and sum; otherwise gq, plain sums.
 template <int TY, bool STATS>
-__global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
+__global__ __launch_bounds__(256) void attention_join_kernel(Args a, int nd, int group) {
   using M = Mm<TY, 16>;
-  const int lane = threadIdx.x & 63;
-  const int rows = a.G * a.L, nd = a.D <= 16 ? 4 : a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32;      // lanes across the head dim
-  const long long all = (long long)a.B * a.Hk * rows, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= all) return;
+  const int lane = threadIdx.x % group;
+  const int rows = a.G * a.L;
+  const long long all = (long long)a.B * a.Hk * rows, id = ((long long)blockIdx.x * 256 + threadIdx.x) / group;
+  if (id >= all) return;                                        // whole groups leave: the exchanges below stay inside a group
   const int r = (int)(id % rows), hk = (int)(id / rows % a.Hk), b = (int)(id / rows / a.Hk);
   const int n = min(a.splits, (keys_of(a, b) + a.range - 1) / a.range);
   float top = kLowest, l = 0.f;
   if (STATS) {
-    for (int s = lane; s < n; s += 64) top = fmaxf(top, a.part_ml[2 * (s * all + id)]);
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    for (int s = lane; s < n; s += 64) {
+    for (int s = lane; s < n; s += group) top = fmaxf(top, a.part_ml[2 * (s * all + id)]);
+    for (int x = 1; x < group; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    for (int s = lane; s < n; s += group) {
       const float *p = a.part_ml + 2 * (s * all + id);
       l = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - top), l);
     }
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+    for (int x = 1; x < group; x *= 2) l += __shfl_xor(l, x);
     if (a.lse != nullptr && lane == 0) a.lse[id] = l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l);
   }
   const int d = 4 * (lane % nd);
   f4 o = {0.f, 0.f, 0.f, 0.f};
   if (d < a.D)
-    for (int s = lane / nd; s < n; s += 64 / nd) {
+    for (int s = lane / nd; s < n; s += group / nd) {
       const f4 p = *reinterpret_cast<const f4 *>(a.part + (s * all + id) * a.D + d);
       if (STATS) o += p * __builtin_amdgcn_exp2f(a.part_ml[2 * (s * all + id)] - top);
       else o += p;
     }
-  for (int x = nd; x < 64; x *= 2)
+  for (int x = nd; x < group; x *= 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
   if (lane >= nd || d >= a.D) return;

@@ -16,6 +16,16 @@ static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &
   return check_launch(name);
 }
 
+template <int TY, bool STATS>
+static int join(const Args &a, hipStream_t s) {
+  const int nd = padded(a.D) / 4;                               // lanes across the head dim
+  int group = nd;
+  while (group < 64 && group / nd < a.splits) group *= 2;
+  const long long all = (long long)a.B * a.Hk * a.G * a.L;
+  hipLaunchKernelGGL((attention_join_kernel<TY, STATS>), dim3((unsigned)((all * group + 255) / 256)), dim3(256), 0, s, a, nd, group);
+  return check_launch("attention_join");
+}
+
 template <int TY, int DP, int MT, int WQ>
 static int fwd(const Args &a, hipStream_t s) {
   static LdsRaised plain, full;
@@ -36,9 +46,11 @@ template <int TY, int DP, int NT>
 static int gkv(const Args &a, hipStream_t s) {
   static LdsRaised plain, full;
   const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
-  constexpr int lds = GkvCfg<TY, DP, NT>::LDS;
-  return needs_full(a) ? go(attention_gkv_kernel<TY, DP, NT, true>, full, lds, grid, a, s, "attention_gkv")
-                       : go(attention_gkv_kernel<TY, DP, NT, false>, plain, lds, grid, a, s, "attention_gkv");
+  constexpr bool GQ = one_launch(DP);
+  constexpr int lds = GkvCfg<TY, DP, NT, GQ>::LDS;
+  static_assert(GkvCfg<TY, DP, NT, GQ>::BR == tile_rows(TY, DP), "the plan's tiles");
+  return needs_full(a) ? go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, lds, grid, a, s, "attention_gkv")
+                       : go(attention_gkv_kernel<TY, DP, NT, GQ, false>, plain, lds, grid, a, s, "attention_gkv");
 }
 
 static void take(Args &a, const Plan &p) {
@@ -62,37 +74,34 @@ int launch_fwd(const Args &args, const Plan &p, hipStream_t s) {
   }
 #undef DI_AT_FWD
   if (rc != DI_OK || p.splits == 1) return rc;
-  const long long all = (long long)a.B * a.Hk * a.G * a.L;
-  hipLaunchKernelGGL((attention_join_kernel<TY, true>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, a);
-  return check_launch("attention_join");
+  return join<TY, true>(a, s);
 }
 
 template <int TY>
 int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) {
   Args a = args;
   int rc = DI_OK;
-  take(a, pq);
+  if (!one_launch(padded(a.D))) {
+    take(a, pq);
 #define DI_AT_GQ(DP) \
   rc = pq.big == 0 ? gq<TY, DP, 1, 1>(a, s) : pq.big == 1 ? gq<TY, DP, 1, 4>(a, s) : gq<TY, DP, row_tiles(DP), 4>(a, s)
-  if (a.L > 0) switch (padded(a.D)) {
-    case 16: DI_AT_GQ(16); break;
-    case 32: DI_AT_GQ(32); break;
-    case 64: DI_AT_GQ(64); break;
-    default: DI_AT_GQ(128); break;
-  }
+    if (a.L > 0) {
+      if (padded(a.D) == 64) DI_AT_GQ(64);
+      else DI_AT_GQ(128);
+    }
 #undef DI_AT_GQ
-  if (rc != DI_OK) return rc;
-  if (pq.splits > 1) {
-    const long long all = (long long)a.B * a.Hk * a.G * a.L;
-    hipLaunchKernelGGL((attention_join_kernel<TY, false>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, a);
-    if ((rc = check_launch("attention_gq_join")) != DI_OK) return rc;
+    if (rc != DI_OK) return rc;
+    if (a.L > 0 && pq.splits > 1 && (rc = join<TY, false>(a, s)) != DI_OK) return rc;
+    if (a.S == 0) return DI_OK;
   }
-  if (a.S == 0) return DI_OK;
   take(a, pk);
-#define DI_AT_GKV(DP)                                                                                                 \
-  rc = pk.big == 4 && key_tiles(TY, DP) >= 4   ? gkv<TY, DP, key_tiles(TY, DP) >= 4 ? 4 : 1>(a, s)                     \
-       : pk.big == 2 && key_tiles(TY, DP) >= 2 ? gkv<TY, DP, key_tiles(TY, DP) >= 2 ? 2 : 1>(a, s)                     \
-                                               : gkv<TY, DP, 1>(a, s)
+#define DI_AT_GKV(DP)                                                                                                      \
+  do {                                                                                                                     \
+    constexpr int most = key_tiles(TY, DP), least = least_key_tiles(DP);                                                   \
+    rc = pk.big >= 4 && most >= 4 ? gkv<TY, DP, most >= 4 ? 4 : least>(a, s)                                               \
+         : pk.big >= 2 && most >= 2 ? gkv<TY, DP, most >= 2 ? 2 : least>(a, s)                                             \
+                                    : gkv<TY, DP, least>(a, s);                                                            \
+  } while (0)
   switch (padded(a.D)) {
     case 16: DI_AT_GKV(16); break;
     case 32: DI_AT_GKV(32); break;
@@ -100,7 +109,14 @@ int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) 
     default: DI_AT_GKV(128); break;
   }
 #undef DI_AT_GKV
-  if (rc != DI_OK || pk.splits == 1) return rc;
+  if (rc != DI_OK) return rc;
+  if (one_launch(padded(a.D)) && pk.blocks > 1 && a.L > 0) {
+    Args j = a;                                                 // the join's ranges are the key blocks
+    j.splits = pk.blocks;
+    j.range = 64 * pk.big;
+    if ((rc = join<TY, false>(j, s)) != DI_OK) return rc;
+  }
+  if (pk.splits == 1 || a.S == 0) return DI_OK;
   const long long n = (long long)a.B * a.Hk * a.S * (a.D / 4);
   hipLaunchKernelGGL((attention_gkv_join_kernel<TY>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
   return check_launch("attention_gkv_join");

@@ -1231,13 +1231,15 @@ def _bool_bytes(t, name):
 
 
 def _seq_view(t):
-    """(B, N, E) as it is when its columns are contiguous and its rows start on 16 bytes, else a dense copy; an expanded batch
-    (stride 0) is read in place."""
+    """(tensor, batch stride, row stride) of (B, N, E): as it is when its columns are contiguous and its rows start on 16 bytes (less
+    than 16 MB apart), else a dense copy; an expanded batch (stride 0) is read in place.  The stride of a dim of size 1 is not used."""
     n = t.element_size()
-    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * n % 16 == 0 and t.stride(1) * n % 16 == 0 \
-            and t.stride(0) >= 0 and t.stride(1) >= 0:
-        return t
-    return t.contiguous()
+    sb, sr, sc = t.stride()
+    B, N, E = t.shape
+    sb, sr = sb if B > 1 else 0, sr if N > 1 else 0
+    if sc == 1 and t.data_ptr() % 16 == 0 and sb * n % 16 == 0 and sr * n % 16 == 0 and sr * n < 1 << 24:
+        return t, sb, sr
+    return t.clone(memory_format=torch.contiguous_format), N * E, E
 
 
 def _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed):
@@ -1262,12 +1264,9 @@ def _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropou
         raise ValueError(f'cross_attention: scale {scale} (positive and finite)')
     if not 0.0 <= dropout_p < 1.0:
         raise ValueError(f'cross_attention: dropout_p {dropout_p} (0 <= p < 1)')
-    q, k, v = _seq_view(q), _seq_view(k), _seq_view(v)
+    (q, t.q_bs, t.q_rs), (k, t.k_bs, t.k_rs), (v, t.v_bs, t.v_rs) = _seq_view(q), _seq_view(k), _seq_view(v)
     keep = [q, k, v]
     t.q, t.k, t.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    t.q_bs, t.q_rs, _ = q.stride()
-    t.k_bs, t.k_rs, _ = k.stride()
-    t.v_bs, t.v_rs, _ = v.stride()
     if key_lengths is not None:
         if key_lengths.shape != (B,) or key_lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f'cross_attention: key_lengths {key_lengths.dtype} {tuple(key_lengths.shape)}, int32 ({B},) expected')
@@ -1350,19 +1349,19 @@ def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None
         raise ValueError(f'cross_attention: out {tuple(out.shape)}, grad_out {tuple(grad_out.shape)}, q {tuple(q.shape)}')
     if lse.shape != (t.B, t.heads, t.L) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError('cross_attention: lse is the tensor that the forward returned')
-    out, go = out.contiguous(), _seq_view(grad_out.to(q.dtype))
+    out, (go, go_bs, go_rs) = out.contiguous(), _seq_view(grad_out.to(q.dtype))
     gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if grads_kv is None:
         gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
     else:
         gk, gv = grads_kv
         for x in (gk, gv):
-            if x.shape != k.shape or x.dtype != k.dtype or _seq_view(x) is not x or (t.B > 1 and x.stride(0) == 0):
+            if x.shape != k.shape or x.dtype != k.dtype or _seq_view(x)[0] is not x or (t.B > 1 and x.stride(0) == 0):
                 raise ValueError('cross_attention: grads_kv have the shape and type of k, contiguous columns and rows on 16 bytes')
     ref = ctypes.addressof(t)
     ws = _attention_workspace('di_attention_bwd_workspace_floats', ref, q)
-    _launch('attention_bwd', t.B, q, ref, out.data_ptr(), lse.data_ptr(), go.data_ptr(), go.stride(0), go.stride(1), gq.data_ptr(),
-            gk.data_ptr(), gk.stride(0), gk.stride(1), gv.data_ptr(), gv.stride(0), gv.stride(1), 0 if ws is None else ws.data_ptr())
+    _launch('attention_bwd', t.B, q, ref, out.data_ptr(), lse.data_ptr(), go.data_ptr(), go_bs, go_rs, gq.data_ptr(),
+            gk.data_ptr(), *_seq_view(gk)[1:], gv.data_ptr(), *_seq_view(gv)[1:], 0 if ws is None else ws.data_ptr())
     return gq, gk, gv
 
 
