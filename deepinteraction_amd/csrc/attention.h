@@ -44,7 +44,10 @@ struct Mm {
   static constexpr int NK = DP / KD, ND = DP / 16;
   static constexpr int CH = WIDE ? 16 : 32, NT = CH / 16;       // rows (keys / queries) per contraction over rows
   static constexpr int PPR = DP * SZ / 16;                      // 16-byte pieces of a tile row
-  // tile row strides in bytes: + 16 keeps the 16-byte row fragments of 16 rows in different banks, + 32 (16-bit) the transposing reads
+  // tile row strides in bytes.  ROWS (read in rows only): + 16 keeps the fragments of 16 rows in different banks.  TRS (read transposed,
+  // or both ways): float32 the same; 16-bit + 32, the stride that spreads the transposing reads of 8 rows over all banks.  Head dim 16 (no
+  // padding): the two 16-byte pieces of every other 8 rows are exchanged (`x` on their offsets), which does the same for the 8-byte row
+  // fragments (1200 x 60 x 112: conflicts 9.4 -> 3.9 million cycles); wider rows had no conflicts, and lost time to the addresses
   static constexpr int ROWS = DP * SZ + 16;
   static constexpr int TRS = WIDE ? DP * 4 + 16 : (DP == 16 ? 32 : DP * 2 + 32);
   struct RF {
@@ -57,6 +60,8 @@ struct Mm {
     u4 v;
   };
 
+  static __device__ __forceinline__ int x(int row) { return WIDE || DP != 16 ? 0 : (row & 8) << 1; }
+
   static __device__ __forceinline__ int d0(int kk, int g) { return KD * kk + (WIDE || DP == 16 ? 4 : 8) * g; }
   static __device__ __forceinline__ RF row_frag(const char *row, int kk, int g) {
     RF f;
@@ -67,6 +72,23 @@ struct Mm {
       f.v = *reinterpret_cast<const u4 *>(row + SZ * d0(kk, g));
     }
     return f;
+  }
+  // row i (mod 16) of a TRS tile
+  static __device__ __forceinline__ RF row_frag_x(const char *row, int kk, int g, int i) {
+    RF f;
+    const char *at = row + ((SZ * d0(kk, g)) ^ x(i));
+    if constexpr (!WIDE && DP == 16) {
+      const u2 t = *reinterpret_cast<const u2 *>(at);
+      f.v = u4{t[0], t[1], 0, 0};
+    } else {
+      f.v = *reinterpret_cast<const u4 *>(at);
+    }
+    return f;
+  }
+  static __device__ __forceinline__ void put_x(char *row, int kk, int g, int i, const RF &f) {
+    char *at = row + ((SZ * d0(kk, g)) ^ x(i));
+    if constexpr (!WIDE && DP == 16) *reinterpret_cast<u2 *>(at) = u2{f.v[0], f.v[1]};
+    else *reinterpret_cast<u4 *>(at) = f.v;
   }
   // from global memory: dims past D and rows that are not there are zeros
   static __device__ __forceinline__ RF row_frag_of(const char *row, int kk, int g, int D, bool ok) {
@@ -92,14 +114,14 @@ struct Mm {
       return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a.v), __builtin_bit_cast(b8, b.v), c, 0, 0, 0);
     }
   }
-  // columns 16 dt .. + 15 of the CH rows from row0 of a tile
+  // columns 16 dt .. + 15 of the CH rows from row0 (a multiple of 16) of a TRS tile
   static __device__ __forceinline__ TF tr_frag(const char *tile, int stride, int row0, int dt, int i, int g) {
     TF f;
     if constexpr (WIDE) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) f.v[r] = *reinterpret_cast<const unsigned *>(tile + (row0 + 4 * g + r) * stride + 4 * (16 * dt + i));
     } else {
-      const char *at = tile + (row0 + 4 * g + (i >> 2)) * stride + 32 * dt + 8 * (i & 3);
+      const char *at = tile + (row0 + 4 * g + (i >> 2)) * stride + 32 * dt + ((8 * (i & 3)) ^ x(4 * g));
       const tr4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4 __attribute__((address_space(3))) *)at);
       const tr4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4 __attribute__((address_space(3))) *)(at + 16 * stride));
       const u2 a = __builtin_bit_cast(u2, lo), b = __builtin_bit_cast(u2, hi);
@@ -182,6 +204,25 @@ __device__ __forceinline__ unsigned drop_pair(unsigned row, unsigned k4, bool se
   return second ? mix(x + 0x68bc21ebu) : x;
 }
 
+// n / d for 0 <= n < 2^31 by one multiplication (d fixed for the launch): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// n / d = (mulhi(n, m) + n) >> s
+struct Div {
+  unsigned d, m, s;
+  __host__ __device__ __forceinline__ unsigned of(unsigned n) const {
+#ifdef __HIP_DEVICE_COMPILE__
+    return (__umulhi(n, m) + n) >> s;
+#else
+    return (unsigned)((((unsigned long long)n * m >> 32) + n) >> s);
+#endif
+  }
+};
+inline Div div_by(unsigned d) {
+  Div v = {d < 1 ? 1 : d, 0, 0};
+  while ((1ull << v.s) < v.d) ++v.s;
+  v.m = (unsigned)((((1ull << v.s) - v.d) << 32) / v.d + 1);
+  return v;
+}
+
 struct Args {
   const char *q, *k, *v;
   char *o;                               // forward: (B, L, H D); backward: the forward's output
@@ -197,6 +238,8 @@ struct Args {
   int splits, range;                     // key (or row) ranges of a split grid
   int blocks;                            // row blocks (or key blocks)
   bool allowed_words;                    // every row of `allowed` starts on 4 bytes
+  Div by_unit, by_blocks, by_hk, by_splits, by_L;              // unit = blocks * Hk
+  int even;                              // blocks of the whole turns of 8 units
   float scale2;                          // softmax scale * log2(e)
   float scale;
   unsigned drop;                         // threshold of 65536; 0 = no dropout
@@ -214,19 +257,23 @@ struct Where {
   int blk, hk, sp, b;
 };
 __device__ __forceinline__ Where where(const Args &a) {
-  const int unit = a.blocks * a.Hk, units = a.B * a.splits, even = units / 8 * 8 * unit;
+  const int unit = a.blocks * a.Hk;
   int id = blockIdx.x;
-  if (id < even) {
-    const int xcd = id % 8, j = id / 8;
-    id = (j / unit * 8 + xcd) * unit + j % unit;
+  if (id < a.even) {
+    const int xcd = id % 8, j = id / 8, turn = a.by_unit.of(j);
+    id = (turn * 8 + xcd) * unit + (j - turn * unit);
   } else {
-    id = even + xcd_remap(id - even, units * unit - even);
+    id = a.even + xcd_remap(id - a.even, gridDim.x - a.even);
   }
   Where w;
-  w.blk = id % a.blocks; id /= a.blocks;
-  w.hk = id % a.Hk; id /= a.Hk;
-  w.sp = id % a.splits;
-  w.b = id / a.splits;
+  int next = a.by_blocks.of(id);
+  w.blk = id - next * a.blocks;
+  id = next;
+  next = a.by_hk.of(id);
+  w.hk = id - next * a.Hk;
+  id = next;
+  w.b = a.by_splits.of(id);
+  w.sp = id - w.b * a.splits;
   return w;
 }
 

@@ -2,7 +2,6 @@
 // Reference: the decoder layer's attention to the BEV map (decoder_utils.py:96-103, :421-485), the RoI blocks' attention among the
 // queries of a view (:743-746) and the ray decoder's attention to an image column (fusion_transformerv4.py:715-769).
 #include <math.h>
-#include <stdlib.h>
 
 #include "attention_plan.h"
 
@@ -23,22 +22,27 @@ static void cut(Plan &p, long long problems, int rows, int per_block, int walked
   p.splits = (tiles + per - 1) / per;
 }
 
-static int plan_rows(const di_attention &t, Plan &p) {
+// Rows per workgroup and ranges of the keys.  Up to 16 rows (single queries): 24 workgroups a CU, the memory streams best through many
+// short ranges (16 samples x 8 key heads of 128, up to 32 768 keys, with the join: 8 a CU 246 us, 16 229, 24 220).  More rows: what is
+// resident - two workgroups a CU, one for gq of 128 dims (2048 x 8192 x 16 heads of 128, forward: 1 a CU 263 us, 2 211, 3 229; gq: 1 a
+// CU 290, 2 317) - and three times that where the samples' lengths differ, so that short ones make room (4 x 511 x up to 4100, four heads
+// of 64 to a key head, forward + gq: 2 a CU 161 us, 4 154, 6 123, 8 132).  Too few row blocks for the CUs: 64 rows a workgroup.
+static int plan_rows(const di_attention &t, bool forward, Plan &p) {
   const int cus = device_cus();
   if (cus <= 0) return DI_ERR_LAUNCH;
-  static const int W = getenv("AT_W") ? atoi(getenv("AT_W")) : 2, W1 = getenv("AT_W1") ? atoi(getenv("AT_W1")) : 4;
   const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
   const long long problems = (long long)t.B * t.kv_heads;
   if (rows <= 16) {
     p.big = 0;
-    cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, (long long)W1 * cus);
+    cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, 24ll * cus);
     return DI_OK;
   }
+  const long long want = (forward || DP < 128 ? 2ll : 1ll) * cus * (t.key_lengths != nullptr ? 3 : 1);
   p.big = 2;
-  cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, (long long)W * cus * (t.key_lengths ? 2 : 1));
+  cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, want);
   if (rows <= 64 || problems * p.blocks * p.splits < cus) {
     p.big = 1;
-    cut(p, problems, rows, 64, t.S, 64, 4, (long long)W * cus * (t.key_lengths ? 2 : 1));
+    cut(p, problems, rows, 64, t.S, 64, 4, want);
   }
   return DI_OK;
 }
@@ -49,14 +53,13 @@ static int plan_keys(const di_attention &t, Plan &p) {
   const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L, least = least_key_tiles(DP);
   const int tile = tile_rows(t.dtype, DP);
   const long long problems = (long long)t.B * t.kv_heads;
-  static const int W = getenv("AT_WK") ? atoi(getenv("AT_WK")) : 2;
   const int S = t.S > 0 ? t.S : 1;                              // without keys, one block still writes gq's zeros
   for (p.big = key_tiles(t.dtype, DP); p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
     if (32 * p.big >= t.S) continue;
-    cut(p, problems, S, 64 * p.big, rows, tile, 4, (long long)W * cus);
+    cut(p, problems, S, 64 * p.big, rows, tile, 4, 2ll * cus);
     if (problems * p.blocks * p.splits >= cus) return DI_OK;
   }
-  cut(p, problems, S, 64 * p.big, rows, tile, 4, (long long)W * cus);
+  cut(p, problems, S, 64 * p.big, rows, tile, 4, 2ll * cus);
   return DI_OK;
 }
 
@@ -89,8 +92,8 @@ static int check(const di_attention *t) {
   DI_REQUIRE(t->dropout_p >= 0.f && t->dropout_p < 1.f, "attention: dropout probability %f", (double)t->dropout_p);
   const long long rows = (long long)(t->heads / t->kv_heads) * t->L;
   DI_REQUIRE(rows <= 0x3fffffff && t->S <= 0x3fffffff, "attention: more than 2^30 rows or keys");
-  // every grid: problems x blocks x splits, and the joins' rows x head_dim / 4 / 256
-  const long long most = (long long)t->B * t->kv_heads * ((rows > t->S ? rows : t->S) / 16 + 2);
+  // every grid: problems x blocks x splits (few problems), and the joins' four rows and more per workgroup
+  const long long most = (long long)t->B * t->kv_heads * ((rows > t->S ? rows : t->S) / 4 + 2);
   DI_REQUIRE(most <= 0x7fffffff / 2, "attention: too many rows for one launch");
   const int sz = t->dtype == DI_F32 ? 4 : 2;
   if (t->B == 0) return DI_OK;
@@ -133,7 +136,7 @@ long long di_attention_fwd_workspace_floats(const di_attention *t) {
   using namespace di::at;
   if (check(t) != DI_OK) return -1;
   Plan p;
-  if (plan_rows(*t, p) != DI_OK) return -1;
+  if (plan_rows(*t, true, p) != DI_OK) return -1;
   return p.splits == 1 ? 0 : (long long)p.splits * t->B * t->heads * t->L * (t->head_dim + 2);
 }
 
@@ -141,7 +144,7 @@ long long di_attention_bwd_workspace_floats(const di_attention *t) {
   using namespace di::at;
   if (check(t) != DI_OK) return -1;
   Plan p, k;
-  if (plan_rows(*t, p) != DI_OK || plan_keys(*t, k) != DI_OK) return -1;
+  if (plan_rows(*t, false, p) != DI_OK || plan_keys(*t, k) != DI_OK) return -1;
   const Room r = room_of(*t, p, k);
   return ((long long)t->B * t->heads * t->L + 3) / 4 * 4 + r.gq + r.gkv;
 }
@@ -152,7 +155,7 @@ int di_attention_fwd(const di_attention *t, void *out, float *lse, float *worksp
   if (t->B == 0 || t->L == 0) return DI_OK;
   DI_REQUIRE(out != nullptr && ((uintptr_t)out & 15) == 0, "attention: the output must start on 16 bytes");
   Plan p;
-  if (int rc = plan_rows(*t, p)) return rc;
+  if (int rc = plan_rows(*t, true, p)) return rc;
   Args a = args_of(t);
   a.o = (char *)out;
   a.lse = lse;
@@ -178,7 +181,7 @@ int di_attention_bwd(const di_attention *t, const void *out, const float *lse, c
              "attention: grad_k and grad_v must start and step on 16 bytes");
   DI_REQUIRE((workspace != nullptr || t->L == 0) && ((uintptr_t)workspace & 15) == 0, "attention: workspace");   // no rows: one range, no sums
   Plan p, k;
-  if (int rc = plan_rows(*t, p)) return rc;
+  if (int rc = plan_rows(*t, false, p)) return rc;
   if (int rc = plan_keys(*t, k)) return rc;
   Args a = args_of(t);
   a.o = (char *)const_cast<void *>(out);

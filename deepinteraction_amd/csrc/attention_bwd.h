@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
     const int tile = (at.blk * MT + t) * WQ + wq;
     row[t] = tile < ntile ? 16 * tile + i : rows;
     const bool ok = row[t] < rows;
-    const int r = min(row[t], rows - 1), head = a.G == 1 ? 0 : r / a.L;
+    const int r = min(row[t], rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(r);
     query[t] = r - head * a.L;
     const long long col = (long long)(at.hk * a.G + head) * a.D * M::SZ;
     const char *qp = a.q + at.b * a.q_bs + query[t] * a.q_rs + col, *gp = a.go + at.b * a.go_bs + query[t] * a.go_rs + col;
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         for (int t = 0; t < MT; ++t) s[t][u] = dp[t][u] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < M::NK; ++kk) {
-          const typename M::RF kf = M::row_frag(lds + (kc + 16 * u + i) * M::TRS, kk, g);
+          const typename M::RF kf = M::row_frag_x(lds + (kc + 16 * u + i) * M::TRS, kk, g, i);
           const typename M::RF vf = M::row_frag(lds + C::V_AT + (kc + 16 * u + i) * M::ROWS, kk, g);
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
   for (int t0 = k0; t0 < k1; t0 += C::TILE) {
     __syncthreads();
-    st.commit(lds, M::TRS, M::ROWS, C::V_AT);
+    st.template commit<true, false>(lds, C::V_AT);
     const bool edge = FULL || t0 + C::TILE > k1;
     if (edge && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
       for (int d = 0; d < M::ND; ++d)
         if (16 * d + 4 * g < a.D) *reinterpret_cast<f4 *>(p + 16 * d + 4 * g) = acc[t][d];
     } else {
-      const int head = a.G == 1 ? 0 : row[t] / a.L;
+      const int head = a.G == 1 ? 0 : (int)a.by_L.of(row[t]);
       char *p = a.gq + (((long long)at.b * a.L + query[t]) * a.Hk * a.G + at.hk * a.G + head) * a.D * M::SZ;
 #pragma unroll
       for (int d = 0; d < M::ND; ++d)
@@ -212,7 +212,7 @@ struct GkvCfg {
   static constexpr int NP = (BR * M::PPR + 255) / 256;
   // P of a normalised row is about 1 / S: in float16 it is scaled by 2^14 (the largest power of two whose product with 1 is finite
   // with room to spare) so that probabilities down to 2^-28 keep their 11 bits; exact to undo
-  static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f;
+  static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f, P_LOG2 = TY == DI_F16 ? 14.f : 0.f;
 };
 
 template <int TY, int DP, int NT, bool GQ, bool FULL>
@@ -232,33 +232,6 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
   const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
 
-  typename M::RF kf[NT][M::NK], vf[NT][M::NK];
-  f4 gk[NT][M::ND], gv[NT][M::ND];
-  bool valid[NT];
-  int key[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    key[n] = key0 + (wave * NT + n) * 16 + i;
-    valid[n] = key[n] < nkeys && (!FULL || a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
-#pragma unroll
-    for (int kk = 0; kk < M::NK; ++kk) {
-      kf[n][kk] = M::row_frag_of(kb + key[n] * a.k_rs, kk, g, a.D, valid[n]);
-      vf[n][kk] = M::row_frag_of(vb + key[n] * a.v_rs, kk, g, a.D, valid[n]);
-    }
-#pragma unroll
-    for (int d = 0; d < M::ND; ++d) gk[n][d] = gv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
-  }
-  const unsigned long long seed = FULL && a.drop ? seed_of(a) : 0;
-  if constexpr (GQ) {                                           // the keys once more, for the products that contract over them
-    for (int e = tid; e < C::KEYS * M::PPR; e += 256) {
-      const int k = e / M::PPR, p = e % M::PPR, s = key0 + k;
-      u4 x = {0, 0, 0, 0};
-      if (s < nkeys && p * 16 < a.D * M::SZ && (!FULL || a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + s] != 0))
-        x = *reinterpret_cast<const u4 *>(kb + s * a.k_rs + p * 16);
-      *reinterpret_cast<u4 *>(lds + C::K_AT + k * M::TRS + p * 16) = x;
-    }
-  }
-
   // rows of Q and go as KeyStage holds keys; a tile that lies in one head has a uniform base
   constexpr int STEP = 256 / M::PPR;
   u4 qs[C::NP], gs[C::NP], os[C::NP];                           // os: GQ forms delta from the forward's output
@@ -271,7 +244,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
   const unsigned oo = (unsigned)(first * o_rs) + piece * 16;
   const char *ob = a.o + at.b * a.L * o_rs;
   auto fetch = [&](int t0) {
-    const int head0 = a.G == 1 ? 0 : t0 / a.L, l0 = t0 - head0 * a.L;
+    const int head0 = a.G == 1 ? 0 : (int)a.by_L.of(t0), l0 = t0 - head0 * a.L;
     if (t0 + C::BR <= r1 && l0 + C::BR <= a.L) {
       const long long col = (long long)(at.hk * a.G + head0) * a.D * M::SZ;
       const char *qt = qb + l0 * a.q_rs + col, *gt = gb + l0 * a.go_rs + col, *ot = ob + l0 * o_rs + col;
@@ -290,7 +263,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         const int r = t0 + first + j * STEP;
         qs[j] = gs[j] = os[j] = u4{0, 0, 0, 0};
         if (in && r < r1) {
-          const int head = a.G == 1 ? 0 : r / a.L, l = r - head * a.L;
+          const int head = a.G == 1 ? 0 : (int)a.by_L.of(r), l = r - head * a.L;
           const long long col = (long long)(at.hk * a.G + head) * a.D * M::SZ + piece * 16;
           qs[j] = *reinterpret_cast<const u4 *>(qb + l * a.q_rs + col);
           gs[j] = *reinterpret_cast<const u4 *>(gb + l * a.go_rs + col);
@@ -305,24 +278,50 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
     }
   };
   if (r0 < r1) fetch(r0);
+
+  typename M::RF kf[NT][M::NK], vf[NT][M::NK];
+  f4 gk[NT][M::ND], gv[NT][M::ND];
+  bool valid[NT];
+  int key[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    key[n] = key0 + (wave * NT + n) * 16 + i;
+    valid[n] = key[n] < nkeys && (!FULL || a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
+#pragma unroll
+    for (int kk = 0; kk < M::NK; ++kk) {
+      kf[n][kk] = M::row_frag_of(kb + key[n] * a.k_rs, kk, g, a.D, valid[n]);
+      vf[n][kk] = M::row_frag_of(vb + key[n] * a.v_rs, kk, g, a.D, valid[n]);
+    }
+#pragma unroll
+    for (int d = 0; d < M::ND; ++d) gk[n][d] = gv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const unsigned long long seed = FULL && a.drop ? seed_of(a) : 0;
+  if constexpr (GQ) {                                           // the keys once more, for the products that contract over them
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int kk = 0; kk < M::NK; ++kk) M::put_x(lds + C::K_AT + ((wave * NT + n) * 16 + i) * M::TRS, kk, g, i, kf[n][kk]);
+  }
+
   for (int t0 = r0; t0 < r1; t0 += C::BR) {
     __syncthreads();
     if (C::BR >= STEP || first < C::BR) {
 #pragma unroll
       for (int j = 0; j < C::NP; ++j) {
-        *reinterpret_cast<u4 *>(lds + (first + j * STEP) * M::TRS + piece * 16) = qs[j];
-        *reinterpret_cast<u4 *>(lds + C::G_AT + (first + j * STEP) * M::TRS + piece * 16) = gs[j];
+        const int at_row = (first + j * STEP) * M::TRS + ((piece * 16) ^ M::x(first + j * STEP));
+        *reinterpret_cast<u4 *>(lds + at_row) = qs[j];
+        *reinterpret_cast<u4 *>(lds + C::G_AT + at_row) = gs[j];
         if (GQ) {
           float d = M::widen_dot({gs[j]}, {os[j]});
 #pragma unroll
           for (int x = 1; x < M::PPR; x *= 2) d += __shfl_xor(d, x);
-          if (piece == 0) sdelta[first + j * STEP] = d;
+          if (piece == 0) sdelta[first + j * STEP] = d * (1.f / C::P_SCALE);
         }
       }
     }
     if (tid < C::BR) {
-      slse[tid] = ls == -INFINITY ? INFINITY : ls;
-      if (!GQ) sdelta[tid] = de;
+      slse[tid] = ls == -INFINITY ? INFINITY : ls - C::P_LOG2;
+      if (!GQ) sdelta[tid] = de * (1.f / C::P_SCALE);
     }
     __syncthreads();
     if (t0 + C::BR < r1) fetch(t0 + C::BR);
@@ -338,7 +337,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int rr = min(rfirst + r, rows - 1), head = a.G == 1 ? 0 : rr / a.L;
+            const int rr = min(rfirst + r, rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(rr);
             const unsigned char *line = a.allowed + at.b * a.allowed_bs + (rr - head * a.L) * a.allowed_rs;
 #pragma unroll
             for (int n = 0; n < NT; ++n) may[n][r] = line[min(key[n], a.S - 1)];
@@ -349,8 +348,8 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         for (int n = 0; n < NT; ++n) s[n] = dp[n] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < M::NK; ++kk) {
-          const typename M::RF qf = M::row_frag(lds + (rc + 16 * u + i) * M::TRS, kk, g);
-          const typename M::RF gf = M::row_frag(lds + C::G_AT + (rc + 16 * u + i) * M::TRS, kk, g);
+          const typename M::RF qf = M::row_frag_x(lds + (rc + 16 * u + i) * M::TRS, kk, g, i);
+          const typename M::RF gf = M::row_frag_x(lds + C::G_AT + (rc + 16 * u + i) * M::TRS, kk, g, i);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             s[n] = M::dot(qf, kf[n][kk], s[n]);
@@ -367,16 +366,17 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             // (a column is one key: whatever the column of an excluded key holds stays there, and is dropped at the end)
+            // pr = P_SCALE p, ds = pr ((dp - delta) / P_SCALE): the scale sits in the rows' two numbers
             const float pr = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale2, -l4[r]));
             if (FULL && a.drop) {
               const unsigned x = drop_pair(drop_row(seed, row_id + rfirst + r), (unsigned)key[n] >> 2, (key[n] & 2) != 0);
               const bool kept = ((key[n] & 1) ? x >> 16 : x & 0xffffu) >= a.drop;
-              p[n][u][r] = kept ? pr * C::P_SCALE : 0.f;          // the kept ones' scale: at the end
+              p[n][u][r] = kept ? pr : 0.f;                        // the kept ones' scale: at the end
               dp[n][r] = kept ? dp[n][r] * a.keep_scale : 0.f;
             } else {
-              p[n][u][r] = pr * C::P_SCALE;
+              p[n][u][r] = pr;
             }
-            ds[n][u][r] = pr * (dp[n][r] - d4[r]);
+            ds[n][u][r] = pr * fmaf(dp[n][r], 1.f / C::P_SCALE, -d4[r]);
           }
         }
       }
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         char *mine = lds + C::DS_AT + wave * C::DS_WAVE;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          char *at_key = mine + (16 * n + i) * C::DS_ROW + 4 * g * M::SZ;
+          char *at_key = mine + (16 * n + i) * C::DS_ROW + ((4 * g * M::SZ) ^ M::x(i));
           if constexpr (M::WIDE) {
             *reinterpret_cast<u4 *>(at_key) = df[n].v;
           } else {
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         if (a.blocks > 1) {
           *reinterpret_cast<f4 *>(a.part + ((long long)at.blk * a.B * a.Hk * rows + row_id + r) * a.D + d) = x;
         } else {
-          const int head = a.G == 1 ? 0 : r / a.L;
+          const int head = a.G == 1 ? 0 : (int)a.by_L.of(r);
           M::store4(a.gq + (((long long)at.b * a.L + (r - head * a.L)) * o_rs) + ((at.hk * a.G + head) * a.D + d) * M::SZ, x * a.scale);
         }
       }

@@ -72,13 +72,16 @@ struct KeyStage {
       }
     }
   }
-  __device__ __forceinline__ void commit(char *lds, int kstride, int vstride, int v_at) {
+  // KX / VX: the tile of K / V is a TRS tile
+  template <bool KX, bool VX>
+  __device__ __forceinline__ void commit(char *lds, int v_at) {
     const int p = threadIdx.x % M::PPR;
     if (C::TILE >= STEP || key < C::TILE) {
 #pragma unroll
       for (int j = 0; j < C::NP; ++j) {
-        *reinterpret_cast<u4 *>(lds + (key + j * STEP) * kstride + p * 16) = k[j];
-        *reinterpret_cast<u4 *>(lds + v_at + (key + j * STEP) * vstride + p * 16) = v[j];
+        const int row = key + j * STEP, x = M::x(row);
+        *reinterpret_cast<u4 *>(lds + row * (KX ? M::TRS : M::ROWS) + ((p * 16) ^ (KX ? x : 0))) = k[j];
+        *reinterpret_cast<u4 *>(lds + v_at + row * (VX ? M::TRS : M::ROWS) + ((p * 16) ^ (VX ? x : 0))) = v[j];
       }
     }
   }
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attent
   for (int t = 0; t < MT; ++t) {
     const int tile = (at.blk * MT + t) * WQ + wq;               // row tiles dealt out to the wavefronts in turn
     row[t] = tile < ntile ? 16 * tile + i : rows;
-    const int r = min(row[t], rows - 1), head = a.G == 1 ? 0 : r / a.L;
+    const int r = min(row[t], rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(r);
     query[t] = r - head * a.L;
     const char *qp = a.q + at.b * a.q_bs + query[t] * a.q_rs + (long long)(at.hk * a.G + head) * a.D * M::SZ;
 #pragma unroll
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attent
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
   for (int t0 = k0; t0 < k1; t0 += C::TILE) {
     __syncthreads();                                            // the last tile's reads are done
-    st.commit(lds, M::ROWS, M::TRS, C::V_AT);
+    st.template commit<false, true>(lds, C::V_AT);
     const bool edge = FULL || t0 + C::TILE > k1;
     if (edge && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attent
     } else {
       const float inv = l[t] == 0.f ? 0.f : a.keep_scale / l[t];         // an empty row: zeros
       if (a.lse != nullptr && g == 0) a.lse[row_id + row[t]] = l[t] == 0.f ? -INFINITY : m[t] + __builtin_amdgcn_logf(l[t]);
-      const int head = a.G == 1 ? 0 : row[t] / a.L;
+      const int head = a.G == 1 ? 0 : (int)a.by_L.of(row[t]);
       char *p = a.o + (((long long)at.b * a.L + query[t]) * a.Hk * a.G + at.hk * a.G + head) * a.D * M::SZ;
 #pragma unroll
       for (int d = 0; d < M::ND; ++d)
@@ -308,41 +311,60 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attent
   }
 }
 
-// The ranges' sums of a row joined: `group` lanes per row, 4 head dims a lane, the other lanes on further ranges.  STATS: forward,
-// every range has its own maximum and sum; otherwise gq, plain sums.
+// The ranges' sums of a row joined: `group` lanes per row, 4 head dims a lane, the other lanes on further ranges, four ranges of a lane
+// in flight (with their statistics).  by_unit: workgroups per (sample, key head).  STATS: forward, every range has its own maximum and
+// sum; otherwise gq, plain sums.
 template <int TY, bool STATS>
 __global__ __launch_bounds__(256) void attention_join_kernel(Args a, int nd, int group) {
   using M = Mm<TY, 16>;
-  const int lane = threadIdx.x % group;
-  const int rows = a.G * a.L;
-  const long long all = (long long)a.B * a.Hk * rows, id = ((long long)blockIdx.x * 256 + threadIdx.x) / group;
-  if (id >= all) return;                                        // whole groups leave: the exchanges below stay inside a group
-  const int r = (int)(id % rows), hk = (int)(id / rows % a.Hk), b = (int)(id / rows / a.Hk);
+  const int lane = threadIdx.x % group, rows = a.G * a.L;
+  const int pr = a.by_unit.of(blockIdx.x), b = a.by_hk.of(pr), hk = pr - b * a.Hk;
+  const int r = (int)((blockIdx.x - pr * a.by_unit.d) * (256 / group) + threadIdx.x / group);
+  if (r >= rows) return;                                        // whole groups leave: the exchanges below stay inside a group
+  const long long all = (long long)a.B * a.Hk * rows, id = (long long)pr * rows + r;
   const int n = min(a.splits, (keys_of(a, b) + a.range - 1) / a.range);
+  const int d = 4 * (lane % nd), step = group / nd;
   float top = kLowest, l = 0.f;
-  if (STATS) {
-    for (int s = lane; s < n; s += group) top = fmaxf(top, a.part_ml[2 * (s * all + id)]);
-    for (int x = 1; x < group; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    for (int s = lane; s < n; s += group) {
-      const float *p = a.part_ml + 2 * (s * all + id);
-      l = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - top), l);
-    }
-    for (int x = 1; x < group; x *= 2) l += __shfl_xor(l, x);
-    if (a.lse != nullptr && lane == 0) a.lse[id] = l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l);
-  }
-  const int d = 4 * (lane % nd);
   f4 o = {0.f, 0.f, 0.f, 0.f};
-  if (d < a.D)
-    for (int s = lane / nd; s < n; s += group / nd) {
-      const f4 p = *reinterpret_cast<const f4 *>(a.part + (s * all + id) * a.D + d);
-      if (STATS) o += p * __builtin_amdgcn_exp2f(a.part_ml[2 * (s * all + id)] - top);
-      else o += p;
-    }
-  for (int x = nd; x < group; x *= 2)
+  auto merge = [&](float m2, float l2, const f4 &o2) {
+    const float x = fmaxf(top, m2), f = __builtin_amdgcn_exp2f(top - x), f2 = __builtin_amdgcn_exp2f(m2 - x);
+    l = l * f + l2 * f2;
+    o = o * f + o2 * f2;
+    top = x;
+  };
+  for (int s0 = lane / nd; s0 < n; s0 += 4 * step) {
+    f4 p[4];
+    float m2[4], l2[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * step;
+      p[u] = f4{0.f, 0.f, 0.f, 0.f};
+      m2[u] = kLowest;
+      l2[u] = 0.f;
+      if (s < n) {
+        if (d < a.D) p[u] = *reinterpret_cast<const f4 *>(a.part + (s * all + id) * a.D + d);
+        if (STATS) {
+          m2[u] = a.part_ml[2 * (s * all + id)];
+          l2[u] = a.part_ml[2 * (s * all + id) + 1];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (STATS) merge(m2[u], l2[u], p[u]);
+      else o += p[u];
+    }
+  }
+  for (int x = nd; x < group; x *= 2) {
+    f4 p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = __shfl_xor(o[e], x);
+    if (STATS) merge(__shfl_xor(top, x), __shfl_xor(l, x), p);
+    else o += p;
+  }
+  if (STATS && a.lse != nullptr && lane == 0) a.lse[id] = l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l);
   if (lane >= nd || d >= a.D) return;
-  const int head = r / a.L;
+  const int head = a.by_L.of(r);
   char *out = (STATS ? a.o : a.gq) + ((((long long)b * a.L + (r - head * a.L)) * a.Hk * a.G + hk * a.G + head) * a.D + d) * M::SZ;
   M::store4(out, o * (STATS ? (l == 0.f ? 0.f : a.keep_scale / l) : a.scale));
 }

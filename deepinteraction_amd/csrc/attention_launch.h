@@ -17,12 +17,14 @@ static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &
 }
 
 template <int TY, bool STATS>
-static int join(const Args &a, hipStream_t s) {
+static int join(const Args &args, hipStream_t s) {
+  Args a = args;
   const int nd = padded(a.D) / 4;                               // lanes across the head dim
   int group = nd;
-  while (group < 64 && group / nd < a.splits) group *= 2;
-  const long long all = (long long)a.B * a.Hk * a.G * a.L;
-  hipLaunchKernelGGL((attention_join_kernel<TY, STATS>), dim3((unsigned)((all * group + 255) / 256)), dim3(256), 0, s, a, nd, group);
+  while (group < 64 && 4 * (group / nd) < a.splits) group *= 2;
+  const int per = 256 / group, blocks = (a.G * a.L + per - 1) / per;
+  a.by_unit = div_by(blocks);
+  hipLaunchKernelGGL((attention_join_kernel<TY, STATS>), dim3((unsigned)(a.B * a.Hk * blocks)), dim3(256), 0, s, a, nd, group);
   return check_launch("attention_join");
 }
 
@@ -57,6 +59,13 @@ static void take(Args &a, const Plan &p) {
   a.blocks = p.blocks;
   a.splits = p.splits;
   a.range = p.range;
+  const int unit = a.blocks * a.Hk, units = a.B * a.splits;
+  a.even = units / 8 * 8 * unit;
+  a.by_unit = div_by(unit);
+  a.by_blocks = div_by(a.blocks);
+  a.by_hk = div_by(a.Hk);
+  a.by_splits = div_by(a.splits);
+  a.by_L = div_by(a.L);
 }
 
 template <int TY>
