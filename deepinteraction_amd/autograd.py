@@ -201,6 +201,54 @@ class AddLayerNorm(torch.autograd.Function):
                 None, None, None)
 
 
+class CrossAttention(torch.autograd.Function):
+    """softmax(scale q k^T) v per head (csrc/attention*.hip); k alone, (B, S, 2 Ek), is [K | V] of one projection and receives one
+    packed gradient.  Gradients: q, k, v; lengths and masks have none."""
+
+    @staticmethod
+    @_fwd
+    def forward(ctx, q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed):
+        Ek = k.shape[-1] // 2
+        ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
+        out, lse = ops.cross_attention_train_fwd(q, ks, vs, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+        ctx.save_for_backward(q, k, v, out, lse, key_lengths, key_mask, allowed)
+        ctx.args = (num_heads, scale, dropout_p, seed)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    @_bwd
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, key_lengths, key_mask, allowed = ctx.saved_tensors
+        num_heads, scale, dropout_p, seed = ctx.args
+        Ek = k.shape[-1] // 2
+        packed = None if v is not None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
+        gq, gk, gv = ops.cross_attention_train_bwd(q, ks, vs, out, grad_out, lse, num_heads, scale, key_lengths, key_mask, allowed,
+                                                   dropout_p, seed,
+                                                   grads_kv=None if packed is None else (packed[..., :Ek], packed[..., Ek:]))
+        return gq, gk if packed is None else packed, gv if packed is None else None, None, None, None, None, None, None, None
+
+
+def cross_attention_usable(q, k, num_heads):
+    """Whether `cross_attention` takes these projections: on the GPU, one of float32 / float16 / bfloat16, a head dim of 8 .. 128 in
+    steps of 8."""
+    D = q.shape[-1] // num_heads
+    return q.is_cuda and q.dtype == k.dtype and q.dtype in (torch.float32, torch.float16, torch.bfloat16) and D % 8 == 0 and 8 <= D <= 128
+
+
+def cross_attention(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None, dropout_p=0.0):
+    """`ops.cross_attention`, differentiable where a gradient is asked for; v None: k is [K | V] of one projection.  dropout_p: of the
+    attention weights, with a fresh seed from torch's CPU generator (inside a captured step: plus the word of
+    `ops.set_i2p_seed_tensor`)."""
+    if dropout_p > 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v))):
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if dropout_p > 0 else 0
+        return CrossAttention.apply(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+    if v is None:
+        k, v = k.chunk(2, -1)
+    return ops.cross_attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed)
+
+
 # ---------------------------------------------------------------------------------- DeepInteraction++ samplers
 class MSDeformAttn(torch.autograd.Function):
     """mmcv MultiScaleDeformableAttention core on the packed [offsets | logits] projection (csrc/plusplus.hip /

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   for (int t0 = k0; t0 < k1; t0 += C::TILE) {
     __syncthreads();
     st.template commit<true, false>(lds, C::V_AT);
-    const bool edge = FULL || t0 + C::TILE > k1;
+    const bool edge = km != nullptr || t0 + C::TILE > k1;
     if (edge && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
       bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;

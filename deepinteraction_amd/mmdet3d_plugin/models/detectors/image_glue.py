@@ -339,7 +339,18 @@ class FrozenSwinFPN(_FrozenImageNet):
 
     # ------------------------------------------------------------------ forward
     def _ln(self, x, name):
+        if x.is_cuda and x.dtype != torch.float64:
+            from .... import ops
+            return ops.layernorm(x, self._p(name + '.weight'), self._p(name + '.bias'))
         return F.layer_norm(x, x.shape[-1:], self._p(name + '.weight'), self._p(name + '.bias'), 1e-5)
+
+    def _add_ln(self, x, branch, name):
+        """(x + branch, its norm) in one pass."""
+        if x.is_cuda and x.dtype != torch.float64:
+            from .... import ops
+            return ops.layernorm(x, self._p(name + '.weight'), self._p(name + '.bias'), branch, with_sum=True)[::-1]
+        x = x + branch
+        return x, self._ln(x, name)
 
     def _region_mask(self, Hp, Wp, device):
         """(nW, 49, 49): 0 inside a region of the cyclically shifted map, -100 across regions (swin.py:195-217)."""
@@ -393,8 +404,7 @@ class FrozenSwinFPN(_FrozenImageNet):
             y = torch.roll(y, shifts=(shift, shift), dims=(1, 2))
         if pad_r or pad_b:
             y = y[:, :H, :Wd]
-        x = x + y
-        y = self._ln(x, b + 'norm2')
+        x, y = self._add_ln(x, y, b + 'norm2')
         y = F.gelu(F.linear(y, self._p(b + 'ffn.layers.0.0.weight'), self._p(b + 'ffn.layers.0.0.bias')))
         return x + F.linear(y, self._p(b + 'ffn.layers.1.weight'), self._p(b + 'ffn.layers.1.bias'))
 

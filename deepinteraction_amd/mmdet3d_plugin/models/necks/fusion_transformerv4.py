@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .... import ops, utils
-from ....autograd import GridGather, PolarBEVSample
+from ....autograd import GridGather, PolarBEVSample, cross_attention, cross_attention_usable
 from ....geometry import PC_RANGE, aug_affine
 from ....registry import ATTENTION, NECKS, TRANSFORMER_LAYER
 from ..utils import encoder_utils as eu
@@ -134,7 +134,7 @@ def sine_position_tokens(n_x, n_y, num_feats, temperature=10000, x_major=False):
 
 class PackedMHA(nn.Module):
     """Parameters of the reference's `FlashMultiheadAttention` (:715-760): `in_proj_weight`, `in_proj_bias`,
-    `out_proj.*`.  The attention itself is `ops.mha_small`."""
+    `out_proj.*`.  The attention itself is `ops.mha_small` (inference) or `autograd.cross_attention` (training)."""
 
     def __init__(self, embed_dim, num_heads, dropout=0.0):
         super().__init__()
@@ -146,10 +146,15 @@ class PackedMHA(nn.Module):
         nn.init.constant_(self.out_proj.bias, 0.)
 
     def _attend(self, q, k, v):
-        if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-            return ops.mha_small(q, k, v, self.num_heads)
-        # training: scores materialised per (sequence, head) through library GEMMs and their autograd (what
-        # flash-attn's backward recomputes); attention dropout as in FlashAttention(attention_dropout=dropout)
+        """v None: k is [K | V] of one projection."""
+        if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (v is not None and v.requires_grad))):
+            return ops.mha_small(q, *(k.chunk(2, -1) if v is None else (k, v)), self.num_heads)
+        # training; attention dropout as in FlashAttention(attention_dropout=dropout)
+        if cross_attention_usable(q, k, self.num_heads):
+            return cross_attention(q, k, v, self.num_heads, dropout_p=self.dropout if self.training else 0.0)
+        # scores materialised per (sequence, head) through library GEMMs and their autograd
+        if v is None:
+            k, v = k.chunk(2, -1)
         N, T, E = q.shape
         h, d = self.num_heads, E // self.num_heads
         qh = q.reshape(N, T, h, d).transpose(1, 2) * (float(d) ** -0.5)
@@ -163,13 +168,14 @@ class PackedMHA(nn.Module):
     def self_attention(self, x):
         E = self.embed_dim
         qkv = F.linear(x, self.in_proj_weight, self.in_proj_bias)               # (N,T,3E): q | k | v in place
-        return self.out_proj(self._attend(qkv[..., :E], qkv[..., E:2 * E], qkv[..., 2 * E:]))
+        q, kv = qkv.split((E, 2 * E), -1)
+        return self.out_proj(self._attend(q, kv, None))
 
     def cross_attention(self, x, memory):
         E = self.embed_dim
         q = F.linear(x, self.in_proj_weight[:E], self.in_proj_bias[:E])
         kv = F.linear(memory, self.in_proj_weight[E:], self.in_proj_bias[E:])   # (N,S,2E): k | v
-        return self.out_proj(self._attend(q, kv[..., :E], kv[..., E:]))
+        return self.out_proj(self._attend(q, kv, None))
 
     # ---- fp16 inference: every projection through the fused chain kernels, the output projection with the residual and the
     # layer's LayerNorm as its epilogue (ops.linear_ln)

@@ -24,7 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .... import ops
-from ....autograd import PixelLinear, RoIAlign, WideLinear
+from ....autograd import PixelLinear, RoIAlign, WideLinear, cross_attention, cross_attention_usable
 from ....geometry import aug_affine
 from ....utils import param_key
 
@@ -141,7 +141,8 @@ def _post_norm(norm, x, branch=None):
 def mha_tokens(q_in, k_in, v_in, w, b, out_proj, H, dropout_p=0.0, key_allowed=None):
     """Batch-first multi-head attention on small token sets with library GEMMs.
     q_in (B,L,E), k_in/v_in (B,S,E); key_allowed: optional bool (B,L,S) - query l attends only to the
-    keys s with key_allowed[b,l,s] (a row without any allowed key yields NaN; callers drop it).
+    keys s with key_allowed[b,l,s] (a row without any allowed key yields out_proj's bias on the GPU, NaN in
+    the torch formulation; callers drop it).
     Returns (B,L,E)."""
     B, L, E = q_in.shape
     S = k_in.shape[1]
@@ -153,6 +154,8 @@ def mha_tokens(q_in, k_in, v_in, w, b, out_proj, H, dropout_p=0.0, key_allowed=N
         q = F.linear(q_in, w[:E], b[:E])
         k = F.linear(k_in, w[E:2 * E], b[E:2 * E])
         v = F.linear(v_in, w[2 * E:], b[2 * E:])
+    if cross_attention_usable(q, k, H):
+        return out_proj(cross_attention(q, k, v, H, allowed=key_allowed, dropout_p=dropout_p))
     q = q.view(B, L, H, D).transpose(1, 2) * (float(D) ** -0.5)
     k = k.view(B, S, H, D).transpose(1, 2)
     v = v.view(B, S, H, D).transpose(1, 2)
@@ -222,9 +225,11 @@ class TransformerDecoderLayer(nn.Module):
             kv = F.linear(kin, ca.in_proj_weight[E:], ca.in_proj_bias[E:])     # (B,Pk,2C) = [K | V]
         if x.is_cuda and not (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad)):
             o = ops.mha_decode(q, kv, ca.num_heads, float(ca.head_dim) ** -0.5)
+        elif cross_attention_usable(q, kv, ca.num_heads):
+            # training: one pass over the keys per direction, the (B,H,Q,32400) scores (:471-485) never reach memory
+            o = cross_attention(q, kv, None, ca.num_heads, dropout_p=ca.dropout if self.training else 0.0)
         else:
-            # training: the (B,H,Q,32400) score tensor is materialised, as in the reference (:471-485),
-            # through library GEMMs and their autograd
+            # the (B,H,Q,32400) score tensor is materialised, as in the reference (:471-485), through library GEMMs and their autograd
             Bq, Lq, _ = q.shape
             H, D = ca.num_heads, ca.head_dim
             qh = q.view(Bq, Lq, H, D).transpose(1, 2) * (float(D) ** -0.5)

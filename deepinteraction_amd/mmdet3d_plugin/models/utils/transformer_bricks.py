@@ -9,19 +9,44 @@ import torch.nn.functional as F
 from torch import nn
 
 from .... import ops
-from ....autograd import MSDeformAttn
+from ....autograd import AddLayerNorm, MSDeformAttn
 from ....utils import param_key
 
 
+_NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _norm_type(norm, x, branch):
+    """The type of `norm(x + branch)` where the LayerNorm kernels take it, None elsewhere: autocast evaluates the norm in float32
+    whatever its operands are; without it the operands' common type has to be the norm's own."""
+    if not (x.is_cuda and isinstance(norm, nn.LayerNorm) and norm.elementwise_affine and norm.bias is not None
+            and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= ops.LAYERNORM_MAX_C
+            and (branch is None or branch.shape == x.shape)):
+        return None
+    halves = {t for t in (x.dtype, x.dtype if branch is None else branch.dtype, norm.weight.dtype) if t != torch.float32}
+    if len(halves) > 1 or not halves <= set(_NORM_TYPES) or norm.weight.dtype != norm.bias.dtype:
+        return None
+    if torch.is_autocast_enabled('cuda'):
+        return torch.float32
+    dt = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)
+    return dt if dt == norm.weight.dtype else None
+
+
 def post_norm(norm, x, branch=None):
-    """`norm(x + branch)` (branch may be None) - the post-norm step.  One fused kernel at inference for C <= 128
-    fp16/fp32 tokens on the GPU (ops.add_layernorm), the plain modules otherwise."""
+    """`norm(x + branch)` (branch may be None) - the post-norm step - in one pass on the GPU: training through
+    autograd.AddLayerNorm, inference through ops.add_layernorm (fp16/fp32 tokens, C <= 128) or ops.layernorm; the plain modules
+    on the CPU and for norms the kernels do not take."""
     if (x.is_cuda and not torch.is_grad_enabled() and isinstance(norm, nn.LayerNorm) and norm.elementwise_affine
             and x.shape[-1] <= 128 and x.shape[-1] % 8 == 0 and x.dtype in (torch.float16, torch.float32)
             and norm.weight.dtype == x.dtype):
         return ops.add_layernorm(x.contiguous(), None if branch is None else branch.contiguous(), norm.weight,
                                  norm.bias, norm.eps)
-    return norm(x if branch is None else x + branch)
+    dt = _norm_type(norm, x, branch)
+    if dt is None:
+        return norm(x if branch is None else x + branch)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, branch, norm.weight, norm.bias)):
+        return AddLayerNorm.apply(x, branch, norm.weight, norm.bias, norm.eps, dt, False)
+    return ops.layernorm(x, norm.weight, norm.bias, branch, norm.eps, out_dtype=dt)
 
 
 def fused_tokens_ok(x, *mods):

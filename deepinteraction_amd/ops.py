@@ -557,7 +557,7 @@ _I2P_SEED_REF = [None]
 
 
 def set_i2p_seed_tensor(t):
-    """Register (or clear with None) the device int64 word that every pillar-attention launch adds to its dropout seed when
+    """Register (or clear with None) the device int64 word that every pillar- and cross-attention launch adds to its dropout seed when
     it runs - what a graph-replayed training step rewrites before each replay (`train_step.GraphedTrainer`)."""
     if t is not None:
         assert t.is_cuda and t.dtype == torch.int64 and t.numel() == 1
