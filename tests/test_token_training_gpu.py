@@ -1,0 +1,201 @@
+"""The training paths that the LayerNorm and attention operators carry, as modules: the decoder layer, a RoI block's masked attention, a
+ray decoder layer; against the same modules in float64 on the CPU (torch formulation, materialised scores).
+
+Tolerance: the float32 torch formulation of the same module on the GPU is the yardstick - two float32 evaluations of one chain differ
+from float64 by errors of one size; the operators are given twice its largest error (and 2^-20 of the tensor's largest value, the level
+of a dozen roundings, where the yardstick is exact).  Half precision the same, with 2^-10."""
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from deepinteraction_amd import autograd, ops
+from deepinteraction_amd.mmdet3d_plugin.models.necks import fusion_transformerv4 as ft
+from deepinteraction_amd.mmdet3d_plugin.models.utils import decoder_utils as du, transformer_bricks as tb
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    """Switches the modules to their torch formulation (and back with plain(False))."""
+    def switch(on):
+        if on:
+            monkeypatch.setattr(du, 'cross_attention_usable', lambda *a: False)
+            monkeypatch.setattr(ft, 'cross_attention_usable', lambda *a: False)
+            monkeypatch.setattr(tb, '_norm_type', lambda *a: None)
+        else:
+            monkeypatch.undo()
+    return switch
+
+
+def grads(module, run, dev, dtype, amp=False):
+    m = copy.deepcopy(module).to(dev, dtype)
+    leaves, out = run(m, dev, dtype)
+    g = torch.Generator().manual_seed(4)
+    w = torch.randn(out.shape, generator=g).to(dev, torch.float64 if dtype == torch.float64 else torch.float32)
+    with torch.autocast('cuda', enabled=False):
+        (out.to(w.dtype) * w).sum().backward()
+    named = {'out': out.detach()}
+    named |= {f'd input {i}': t.grad for i, t in enumerate(leaves) if t.grad is not None}
+    named |= {n: p.grad for n, p in m.named_parameters() if p.grad is not None}
+    return {n: t.double().cpu() for n, t in named.items()}
+
+
+def compare(module, run, plain, floor, amp=False):
+    ref = grads(module, run, 'cpu', torch.float64)
+    with torch.autocast('cuda', enabled=amp):
+        plain(True)
+        yard = grads(module, run, 'cuda', torch.float32)
+        plain(False)
+        calls = []
+        fwd, norm = ops.cross_attention_train_fwd, ops.layernorm_train_fwd
+        ops.cross_attention_train_fwd = lambda *a, **k: (calls.append('a'), fwd(*a, **k))[1]
+        ops.layernorm_train_fwd = lambda *a, **k: (calls.append('n'), norm(*a, **k))[1]
+        try:
+            own = grads(module, run, 'cuda', torch.float32)
+        finally:
+            ops.cross_attention_train_fwd, ops.layernorm_train_fwd = fwd, norm
+    assert set(own) == set(ref) == set(yard)
+    for n, r in ref.items():
+        top = float(r.abs().max())
+        e, y = float((own[n] - r).abs().max()), float((yard[n] - r).abs().max())
+        # a bias that feeds only a softmax's constant (the keys'), or a norm: exact gradient 0, round-off on both sides
+        assert e <= 2 * y + floor * max(top, 1e-3), (n, e, y, top)
+    return calls
+
+
+def tokens(shape, dev, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(dev, dtype)
+
+
+def decoder_layer(dev, dropout=0.0):
+    torch.manual_seed(0)
+    return du.TransformerDecoderLayer(128, 8, 256, dropout, 'relu', self_posembed=du.PositionEmbeddingLearned(2, 128),
+                                      cross_posembed=du.PositionEmbeddingLearned(2, 128)).train()
+
+
+def run_decoder(m, dev, dtype):
+    q, k = (tokens(s, dev, dtype, i).requires_grad_(True) for i, s in enumerate(((2, 128, 40), (2, 128, 600))))
+    qp, kp = tokens((2, 40, 2), dev, dtype, 5), tokens((2, 600, 2), dev, dtype, 6)
+    return (q, k), m(q, k, qp, kp)
+
+
+@pytest.mark.parametrize('amp', [False, True])
+def test_decoder_layer(plain, amp):
+    calls = compare(decoder_layer('cpu'), run_decoder, plain, 2.0 ** -10 if amp else 2.0 ** -20, amp)
+    assert calls.count('a') == 2 and calls.count('n') == 3
+
+
+@pytest.mark.parametrize('amp', [False, True])
+def test_ray_decoder_layer(plain, amp):
+    torch.manual_seed(1)
+    m = ft._RayDecoderLayer(128, 8, 256, dropout=0.0).train()
+
+    def run(m, dev, dtype):
+        t, mem = (tokens(s, dev, dtype, i).requires_grad_(True) for i, s in enumerate(((7, 60, 128), (7, 112, 128))))
+        return (t, mem), m(t, mem)
+    calls = compare(m, run, plain, 2.0 ** -10 if amp else 2.0 ** -20, amp)
+    assert calls.count('a') == 2 and calls.count('n') == 3
+
+
+def test_attention_among_the_queries_of_a_view(plain):
+    """mha_tokens with the RoI blocks' mask; queries of no view have an empty row and are dropped, as by the blocks."""
+    torch.manual_seed(2)
+    m = du.MultiheadAttention(128, 8).train()
+    view = torch.randint(-1, 3, (2, 50), generator=torch.Generator().manual_seed(3))
+    allowed = (view[:, :, None] == view[:, None, :]) & (view[:, :, None] >= 0)
+
+    def run(m, dev, dtype):
+        x = tokens((2, 50, 128), dev, dtype, 1).requires_grad_(True)
+        y = du.mha_tokens(x, x, x, m.in_proj_weight, m.in_proj_bias, m.out_proj, 8, 0.0, allowed.to(dev))
+        return (x,), torch.where((view >= 0)[..., None].to(dev), y, torch.zeros_like(y))
+
+    ref = grads(m, lambda m, dev, dtype: run(m, dev, dtype), 'cuda', torch.float32)
+    assert all(torch.isfinite(t).all() for t in ref.values())
+    # the torch formulation gives NaN for the empty rows, and NaN * 0 in its gradients: the oracle attends with one key for them
+    ids = torch.arange(50)
+    patched = allowed | ((view < 0)[:, :, None] & (ids[None, :, None] == ids[None, None, :]))
+
+    def run_patched(m, dev, dtype):
+        x = tokens((2, 50, 128), dev, dtype, 1).requires_grad_(True)
+        y = du.mha_tokens(x, x, x, m.in_proj_weight, m.in_proj_bias, m.out_proj, 8, 0.0, patched.to(dev))
+        return (x,), torch.where((view >= 0)[..., None].to(dev), y, torch.zeros_like(y))
+    want = grads(m, run_patched, 'cpu', torch.float64)
+    plain(True)
+    yard = grads(m, run_patched, 'cuda', torch.float32)
+    plain(False)
+    for n, r in want.items():
+        e, y = float((ref[n] - r).abs().max()), float((yard[n] - r).abs().max())
+        assert e <= 2 * y + 2.0 ** -20 * max(float(r.abs().max()), 1e-3), (n, e, y)
+
+
+def test_dropout_reaches_the_attention_and_its_seed_is_torch_s(plain):
+    """Training with dropout: the same CPU seed gives the same step, another seed another; evaluation has none."""
+    m = decoder_layer('cpu', dropout=0.3).cuda()
+
+    def step(seed):
+        torch.manual_seed(seed)
+        for p in m.parameters():
+            p.grad = None
+        (q, _), out = run_decoder(m, 'cuda', torch.float32)
+        out.square().sum().backward()
+        return out.detach().clone(), q.grad.clone()
+    a, b, c = step(1), step(1), step(2)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and not torch.equal(a[0], c[0])
+    q = tokens((2, 30, 128), 'cuda', torch.float32, 0)
+    kv = tokens((2, 90, 256), 'cuda', torch.float32, 1)
+    torch.manual_seed(5)
+    x = autograd.cross_attention(q, kv, None, 8, dropout_p=0.5)
+    y = autograd.cross_attention(q, kv, None, 8, dropout_p=0.5)
+    torch.manual_seed(5)
+    assert torch.equal(x, autograd.cross_attention(q, kv, None, 8, dropout_p=0.5)) and not torch.equal(x, y)
+
+
+def test_packed_and_separate_projections_agree():
+    q = tokens((2, 33, 64), 'cuda', torch.float16, 0)
+    kv = tokens((2, 77, 64), 'cuda', torch.float16, 1)
+    outs = []
+    for packed in (True, False):
+        a, b = q.clone().requires_grad_(True), kv.clone().requires_grad_(True)
+        o = autograd.cross_attention(a, b, None, 4) if packed else autograd.cross_attention(a, *b.chunk(2, -1), 4)
+        o.backward(tokens((2, 33, 64), 'cuda', torch.float16, 2))
+        outs.append((o.detach(), a.grad, b.grad))
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+    with torch.no_grad():
+        assert torch.equal(autograd.cross_attention(q, kv, None, 4), outs[0][0])
+
+
+def test_captured_training_step_of_a_layer():
+    """Forward and backward of the decoder layer in one graph, replayed with new inputs between eager steps."""
+    m = decoder_layer('cpu').cuda()
+    q, k = torch.empty(1, 128, 40, device='cuda'), torch.empty(1, 128, 600, device='cuda')
+    qp, kp = tokens((1, 40, 2), 'cuda', torch.float32, 5), tokens((1, 600, 2), 'cuda', torch.float32, 6)
+    params = [p for p in m.parameters()]
+
+    def step():
+        out = m(q, k, qp, kp)
+        return (out,) + torch.autograd.grad(out.square().mean(), params, allow_unused=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    q.normal_(), k.normal_()
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = [None if t is None else t for t in step()]
+    bn = [b for mod in m.modules() if isinstance(mod, torch.nn.BatchNorm1d) for b in (mod.running_mean, mod.running_var, mod.num_batches_tracked)]
+    for n in range(3):
+        q.normal_(), k.normal_()
+        keep = [b.clone() for b in bn]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [None if t is None else t.detach().clone() for t in static]
+        for b, v in zip(bn, keep):
+            b.copy_(v)
+        for a, b in zip(got, step()):
+            # library products may be chosen differently inside and outside a capture: a few roundings of the largest value
+            assert (a is None) == (b is None) and (a is None or float((a - b).abs().max()) <= 2.0 ** -18 * max(float(b.abs().max()), 1e-6)), n
