@@ -1105,6 +1105,14 @@ def _same_device(first, *ts):
             raise ValueError(f'tensors on {first.device} and {t.device} in one call')
 
 
+def _on_device(q, f):
+    """f() with q's device current: plans ask for its number of compute units."""
+    if q.get_device() == torch.cuda.current_device():
+        return f()
+    with torch.cuda.device(q.device):
+        return f()
+
+
 def _launch(name, n, t, *args):
     """`_lib.call` on the device of `t`, on that device's current stream (appended to the arguments)."""
     at = t.get_device()
@@ -1156,9 +1164,9 @@ def _layernorm_fwd(x, weight, bias, res, eps, with_sum, out_dtype, stats):
         out_dtype = x.dtype if res is None else torch.promote_types(x.dtype, res.dtype)
     codes = [_code3(x), _code3(x if res is None else res), _code3(weight), _code3(out_dtype)]
     rows = x.numel() // C
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_sum else None
-    mean, rstd = (torch.empty(rows, dtype=torch.float32, device=x.device) for _ in range(2)) if stats else (None, None)
+    y = x.new_empty(x.shape, dtype=out_dtype)
+    total = x.new_empty(x.shape) if with_sum else None
+    mean, rstd = (x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)) if stats else (None, None)
     xv, xs = _row_view(x, C)
     rv, rs = (None, 0) if res is None else _row_view(res, C)
     w, b = weight.contiguous(), bias.contiguous()
@@ -1205,18 +1213,18 @@ def layernorm_train_bwd(grad_y, x, weight, mean, rstd, res=None, grad_sum=None, 
         grad_sum = grad_sum.to(x.dtype)
     if grad_y.dtype != torch.float32 and not x.dtype == (x if res is None else res).dtype == grad_y.dtype:
         grad_y, codes[0] = grad_y.float(), _lib.DI_F32           # a 16-bit gradient of a float32 result: exact in float32
-    gx = torch.empty(x.shape, dtype=grad_dtype, device=x.device)
+    gx = x.new_empty(x.shape, dtype=grad_dtype)
     gres = None
     if res is not None:
-        gres = gx if res.dtype == grad_dtype else torch.empty(res.shape, dtype=res.dtype, device=x.device)
-    gw, gb = (torch.empty(C, dtype=weight.dtype, device=x.device) for _ in range(2))
+        gres = gx if res.dtype == grad_dtype else res.new_empty(res.shape)
+    gw, gb = weight.new_empty(C), weight.new_empty(C)
     gv, gs = _row_view(grad_y, C)
     sv, ss = (None, 0) if grad_sum is None else _row_view(grad_sum, C)
     xv, xs = _row_view(x, C)
     rv, rs = (None, 0) if res is None else _row_view(res, C)
     w = weight.contiguous()
     ptr = lambda t: 0 if t is None else t.data_ptr()
-    ws = torch.empty(max(4, _lib.lib().di_layernorm_bwd_workspace_floats(rows, C)), dtype=torch.float32, device=x.device)
+    ws = x.new_empty(max(4, _on_device(x, lambda: _lib.lib().di_layernorm_bwd_workspace_floats(rows, C))), dtype=torch.float32)
     _launch('layernorm_bwd', rows, x, gv.data_ptr(), gs, codes[0], ptr(sv), ss, xv.data_ptr(), xs, codes[1], ptr(rv), rs, codes[2],
             w.data_ptr(), codes[3], mean.data_ptr(), rstd.data_ptr(), gx.data_ptr(), codes[4], 0 if gres is gx else ptr(gres),
             gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), rows, C)
@@ -1296,25 +1304,17 @@ def _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropou
     return t, keep
 
 
-def _on_device(q, f):
-    """f() with q's device current: plans ask for its number of compute units."""
-    if q.get_device() == torch.cuda.current_device():
-        return f()
-    with torch.cuda.device(q.device):
-        return f()
-
-
 def _attention_workspace(name, ref, q):
     n = _on_device(q, lambda: getattr(_lib.lib(), name)(ref))
     if n < 0:
         raise _lib.HipLibraryError(f'{name}: {_lib.lib().di_last_error().decode()}')
-    return torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    return q.new_empty(n, dtype=torch.float32) if n else None
 
 
 def _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, stats):
     t, keep = _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((t.B, t.heads, t.L), dtype=torch.float32, device=q.device) if stats else None
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((t.B, t.heads, t.L), dtype=torch.float32) if stats else None
     ref = ctypes.addressof(t)
     ws = _attention_workspace('di_attention_fwd_workspace_floats', ref, q)
     _launch('attention_fwd', t.B, q, ref, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr())
@@ -1350,18 +1350,20 @@ def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None
     if lse.shape != (t.B, t.heads, t.L) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError('cross_attention: lse is the tensor that the forward returned')
     out, (go, go_bs, go_rs) = out.contiguous(), _seq_view(grad_out.to(q.dtype))
-    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    gq = q.new_empty(q.shape)
     if grads_kv is None:
-        gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+        gk, gv = k.new_empty(k.shape), k.new_empty(k.shape)
+        k_strides = v_strides = (t.S * k.shape[2], k.shape[2])
     else:
         gk, gv = grads_kv
         for x in (gk, gv):
             if x.shape != k.shape or x.dtype != k.dtype or _seq_view(x)[0] is not x or (t.B > 1 and x.stride(0) == 0):
                 raise ValueError('cross_attention: grads_kv have the shape and type of k, contiguous columns and rows on 16 bytes')
+        k_strides, v_strides = _seq_view(gk)[1:], _seq_view(gv)[1:]
     ref = ctypes.addressof(t)
     ws = _attention_workspace('di_attention_bwd_workspace_floats', ref, q)
     _launch('attention_bwd', t.B, q, ref, out.data_ptr(), lse.data_ptr(), go.data_ptr(), go_bs, go_rs, gq.data_ptr(),
-            gk.data_ptr(), *_seq_view(gk)[1:], gv.data_ptr(), *_seq_view(gv)[1:], 0 if ws is None else ws.data_ptr())
+            gk.data_ptr(), *k_strides, gv.data_ptr(), *v_strides, 0 if ws is None else ws.data_ptr())
     return gq, gk, gv
 
 
