@@ -56,10 +56,10 @@ static int plan_keys(const di_attention &t, Plan &p) {
   const int S = t.S > 0 ? t.S : 1;                              // without keys, one block still writes gq's zeros
   for (p.big = key_tiles(t.dtype, DP); p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
     if (32 * p.big >= t.S) continue;
-    cut(p, problems, S, 64 * p.big, rows, tile, 4, 2ll * cus);
+    cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
     if (problems * p.blocks * p.splits >= cus) return DI_OK;
   }
-  cut(p, problems, S, 64 * p.big, rows, tile, 4, 2ll * cus);
+  cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
   return DI_OK;
 }
 

@@ -87,6 +87,14 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;
       if (EDGE && t0 + kc >= k1) break;
+      unsigned may[MT][M::NT];                                  // in flight behind the products
+      if (FULL && a.allowed != nullptr) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < M::NT; ++u)
+            may[t][u] = look(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words);
+      }
       f4 s[MT][M::NT], dp[MT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
@@ -111,8 +119,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         }
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
-            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words, s[t][u]);
+          for (int t = 0; t < MT; ++t) exclude(may[t][u], s[t][u]);
         }
       }
       typename M::PF df[MT];
@@ -279,6 +286,22 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
   };
   if (r0 < r1) fetch(r0);
 
+  // the (query, key) mask of a chunk's rows: with up to 32 keys a wavefront one chunk ahead of its use (rows clamped into the matrix),
+  // with more - registers - in front of the products
+  constexpr bool MASK_AHEAD = NT <= 2;
+  unsigned char may[M::NT][NT][4];
+  auto look = [&](int row0) {
+#pragma unroll
+    for (int u = 0; u < M::NT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int rr = min(row0 + 16 * u + 4 * g + r, rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(rr);
+        const unsigned char *line = a.allowed + at.b * a.allowed_bs + (rr - head * a.L) * a.allowed_rs;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) may[u][n][r] = line[min(key0 + (wave * NT + n) * 16 + i, a.S - 1)];
+      }
+  };
+
   typename M::RF kf[NT][M::NK], vf[NT][M::NK];
   f4 gk[NT][M::ND], gv[NT][M::ND];
   bool valid[NT];
@@ -328,21 +351,12 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
 #pragma unroll 1
     for (int rc = 0; rc < C::BR; rc += M::CH) {
       if (t0 + rc >= r1 || (GQ && wave >= waves)) break;
+      if (FULL && a.allowed != nullptr && (!MASK_AHEAD || (t0 == r0 && rc == 0))) look(t0 + rc);
       typename M::PF pf[NT], df[NT];
       f4 p[NT][M::NT], ds[NT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
         const int rfirst = t0 + rc + 16 * u + 4 * g;
-        unsigned char may[NT][4];                               // in flight behind the products
-        if (FULL && a.allowed != nullptr) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int rr = min(rfirst + r, rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(rr);
-            const unsigned char *line = a.allowed + at.b * a.allowed_bs + (rr - head * a.L) * a.allowed_rs;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) may[n][r] = line[min(key[n], a.S - 1)];
-          }
-        }
         f4 s[NT], dp[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n] = dp[n] = f4{0.f, 0.f, 0.f, 0.f};
@@ -361,7 +375,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
         for (int n = 0; n < NT; ++n) {
           if (FULL && a.allowed != nullptr) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[n][r] = may[n][r] != 0 ? s[n][r] : -INFINITY;
+            for (int r = 0; r < 4; ++r) s[n][r] = may[u][n][r] != 0 ? s[n][r] : -INFINITY;
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -380,6 +394,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
           }
         }
       }
+      if (FULL && MASK_AHEAD && a.allowed != nullptr) look(t0 + rc + M::CH);
       if (GQ && !whole) {                                       // gq sums over the columns: those of excluded keys have to be zero
 #pragma unroll
         for (int n = 0; n < NT; ++n)

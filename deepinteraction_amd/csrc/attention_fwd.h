@@ -91,17 +91,17 @@ struct KeyStage {
 // a score.  A NaN score loses the comparison but stays a NaN in the exponential.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 
-// 4 keys x 1 row of the (row, key) mask; keys past the end count as allowed (their scores are excluded by the bias).  `words`: rows
-// start on 4 bytes, and key is a multiple of 4
-__device__ __forceinline__ void exclude(const unsigned char *row, int key, int S, bool words, f4 &s) {
+// 4 keys x 1 row of the (row, key) mask as the bytes of a word; keys past the end count as allowed (their scores are excluded by the
+// bias).  `words`: rows start on 4 bytes, and key is a multiple of 4.  A row that is not there reads the last one's mask.
+__device__ __forceinline__ unsigned look(const unsigned char *row, int key, int S, bool words) {
+  if (words && key + 4 <= S) return *reinterpret_cast<const unsigned *>(row + key);
   unsigned w = 0x01010101u;
-  if (words && key + 4 <= S) {
-    w = *reinterpret_cast<const unsigned *>(row + key);
-  } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (key + r < S && row[key + r] == 0) w &= ~(0xffu << (8 * r));
-  }
+  for (int r = 0; r < 4; ++r)
+    if (key + r < S && row[key + r] == 0) w &= ~(0xffu << (8 * r));
+  return w;
+}
+__device__ __forceinline__ void exclude(unsigned w, f4 &s) {
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if ((w >> (8 * r) & 0xffu) == 0) s[r] = -INFINITY;
@@ -109,7 +109,7 @@ __device__ __forceinline__ void exclude(const unsigned char *row, int key, int S
 
 // FULL: with a key mask, a (query, key) mask or dropout; without them only the last tile of a range is tested key by key
 template <int TY, int DP, int MT, int WQ, bool FULL>
-__global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attention_fwd_kernel(Args a) {
+__global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) void attention_fwd_kernel(Args a) {
   using C = FwdCfg<TY, DP, MT, WQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
@@ -152,6 +152,14 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attent
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;                 // first key of the chunk in the tile
       if (EDGE && t0 + kc >= k1) break;
+      unsigned may[MT][M::NT];                                  // in flight behind the products
+      if (FULL && a.allowed != nullptr) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < M::NT; ++u)
+            may[t][u] = look(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words);
+      }
       f4 s[MT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
@@ -172,8 +180,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 ? 2 : 1) void attent
         }
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
-            if (row[t] < rows) exclude(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words, s[t][u]);
+          for (int t = 0; t < MT; ++t) exclude(may[t][u], s[t][u]);
         }
       }
       float mx[MT];
