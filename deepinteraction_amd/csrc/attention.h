@@ -131,19 +131,17 @@ struct Mm {
   }
   // result tiles (float32) -> operand of the contraction over their rows; 16-bit: rounded to nearest, half a step of the type -
   // the same relative error for every size of probability, and independent from one to the next in the sums that follow
-  static __device__ __forceinline__ PF pack(const f4 (&p)[NT]) {
-    PF f;
+  static __device__ __forceinline__ void pack(PF &f, int t, const f4 &p) {           // tile t of the operand
     if constexpr (WIDE) {
-      f.v = __builtin_bit_cast(u4, p[0]);
+      f.v = __builtin_bit_cast(u4, p);
     } else {
-      s8 s;
+      s4 s;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[4 * t + r] = TY == DI_F16 ? to_half_bits(p[t][r]) : to_bf_bits(p[t][r]);
-      f.v = __builtin_bit_cast(u4, s);
+      for (int r = 0; r < 4; ++r) s[r] = TY == DI_F16 ? to_half_bits(p[r]) : to_bf_bits(p[r]);
+      const u2 w = __builtin_bit_cast(u2, s);
+      f.v[2 * t] = w[0];
+      f.v[2 * t + 1] = w[1];
     }
-    return f;
   }
   static __device__ __forceinline__ f4 acc(const TF &a, const PF &p, f4 c) {
     if constexpr (WIDE) {

@@ -140,8 +140,8 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             ds[u][r] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], a.scale2, -lse[t])) * (dp[t][u][r] - delta[t]);
+          M::pack(df[t], u, ds[u]);
         }
-        df[t] = M::pack(ds);
       }
 #pragma unroll
       for (int d = 0; d < M::ND; ++d) {
@@ -211,8 +211,8 @@ struct GkvCfg {
   static constexpr int KEYS = 64 * NT;
   static constexpr int G_AT = BR * M::TRS, ST_AT = 2 * G_AT;    // both tiles are read in rows and transposed
   static constexpr int K_AT = ST_AT + 2 * BR * 4;               // GQ: the block's keys,
-  static constexpr int DS_AT = K_AT + KEYS * M::TRS;            // each wavefront's score gradients as (key, row),
-  static constexpr int DS_ROW = M::CH * M::SZ + (M::WIDE ? 16 : 32), DS_WAVE = 16 * NT * DS_ROW;
+  static constexpr int DS_AT = K_AT + KEYS * M::TRS;            // each wavefront's score gradients of CH keys as (key, row),
+  static constexpr int DS_ROW = M::CH * M::SZ + (M::WIDE ? 16 : 32), DS_WAVE = M::CH * DS_ROW;
   static constexpr int RED_AT = DS_AT + 4 * DS_WAVE;            // and its share of gq of the tile's rows, float32
   static constexpr int RED_ROW = DP + 4;
   static constexpr int LDS = GQ ? RED_AT + 4 * BR * RED_ROW * 4 : K_AT;
@@ -223,7 +223,7 @@ struct GkvCfg {
 };
 
 template <int TY, int DP, int NT, bool GQ, bool FULL>
-__global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
+__global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attention_gkv_kernel(Args a) {
   using C = GkvCfg<TY, DP, NT, GQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
@@ -353,7 +353,6 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
       if (t0 + rc >= r1 || (GQ && wave >= waves)) break;
       if (FULL && a.allowed != nullptr && (!MASK_AHEAD || (t0 == r0 && rc == 0))) look(t0 + rc);
       typename M::PF pf[NT], df[NT];
-      f4 p[NT][M::NT], ds[NT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
         const int rfirst = t0 + rc + 16 * u + 4 * g;
@@ -377,6 +376,7 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[n][r] = may[u][n][r] != 0 ? s[n][r] : -INFINITY;
           }
+          f4 p, ds;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             // (a column is one key: whatever the column of an excluded key holds stays there, and is dropped at the end)
@@ -385,69 +385,72 @@ __global__ __launch_bounds__(256) void attention_gkv_kernel(Args a) {
             if (FULL && a.drop) {
               const unsigned x = drop_pair(drop_row(seed, row_id + rfirst + r), (unsigned)key[n] >> 2, (key[n] & 2) != 0);
               const bool kept = ((key[n] & 1) ? x >> 16 : x & 0xffffu) >= a.drop;
-              p[n][u][r] = kept ? pr : 0.f;                        // the kept ones' scale: at the end
+              p[r] = kept ? pr : 0.f;                        // the kept ones' scale: at the end
               dp[n][r] = kept ? dp[n][r] * a.keep_scale : 0.f;
             } else {
-              p[n][u][r] = pr;
+              p[r] = pr;
             }
-            ds[n][u][r] = pr * fmaf(dp[n][r], 1.f / C::P_SCALE, -d4[r]);
+            ds[r] = pr * fmaf(dp[n][r], 1.f / C::P_SCALE, -d4[r]);
           }
+          if (GQ && !whole) {                                   // gq sums over the columns: those of excluded keys have to be zero
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ds[r] = valid[n] ? ds[r] : 0.f;
+          }
+          M::pack(pf[n], u, p);
+          M::pack(df[n], u, ds);
         }
       }
       if (FULL && MASK_AHEAD && a.allowed != nullptr) look(t0 + rc + M::CH);
-      if (GQ && !whole) {                                       // gq sums over the columns: those of excluded keys have to be zero
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int u = 0; u < M::NT; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) ds[n][u][r] = valid[n] ? ds[n][u][r] : 0.f;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        pf[n] = M::pack(p[n]);
-        df[n] = M::pack(ds[n]);
-      }
-      if constexpr (GQ) {
-        // dS leaves as (key, row) rows of the wavefront's own buffer - a lane holds four rows of one key - and comes back transposed as
-        // the operand of gq^T = K^T dS^T; LDS serves a wavefront in order, no barrier
-        char *mine = lds + C::DS_AT + wave * C::DS_WAVE;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          char *at_key = mine + (16 * n + i) * C::DS_ROW + ((4 * g * M::SZ) ^ M::x(i));
-          if constexpr (M::WIDE) {
-            *reinterpret_cast<u4 *>(at_key) = df[n].v;
-          } else {
-            *reinterpret_cast<u2 *>(at_key) = u2{df[n].v[0], df[n].v[1]};
-            *reinterpret_cast<u2 *>(at_key + 32) = u2{df[n].v[2], df[n].v[3]};
-          }
-        }
-        __builtin_amdgcn_wave_barrier();
-        float *red = reinterpret_cast<float *>(lds + C::RED_AT) + (wave * C::BR + rc) * C::RED_ROW;
+      auto by_rows = [&]() {                                    // gv^T += go^T P, gk^T += Q^T dS
 #pragma unroll
         for (int d = 0; d < M::ND; ++d) {
-          f4 gq[M::NT];
+          const typename M::TF gt = M::tr_frag(lds + C::G_AT, M::TRS, rc, d, i, g);
 #pragma unroll
-          for (int u = 0; u < M::NT; ++u) gq[u] = f4{0.f, 0.f, 0.f, 0.f};
+          for (int n = 0; n < NT; ++n) gv[n][d] = M::acc(gt, pf[n], gv[n][d]);
+          const typename M::TF qt = M::tr_frag(lds, M::TRS, rc, d, i, g);
 #pragma unroll
-          for (int c = 0; c < 16 * NT; c += M::CH) {
-            const typename M::TF kt = M::tr_frag(lds + C::K_AT, M::TRS, wave * 16 * NT + c, d, i, g);
-#pragma unroll
-            for (int u = 0; u < M::NT; ++u) gq[u] = M::acc(kt, {M::tr_frag(mine, C::DS_ROW, c, u, i, g).v}, gq[u]);
-          }
-#pragma unroll
-          for (int u = 0; u < M::NT; ++u) *reinterpret_cast<f4 *>(red + (16 * u + i) * C::RED_ROW + 16 * d + 4 * g) = gq[u];
+          for (int n = 0; n < NT; ++n) gk[n][d] = M::acc(qt, df[n], gk[n][d]);
         }
-        __builtin_amdgcn_wave_barrier();
-      }
+      };
+      if constexpr (!GQ) by_rows();
+      if constexpr (GQ) {
+        // gq^T = K^T dS^T of the wavefront's keys, CH of them at a time: dS leaves as (key, row) rows of the wavefront's own buffer - a lane
+        // holds four rows of one key - and comes back transposed as the operand; LDS serves a wavefront in order, no barrier
+        char *mine = lds + C::DS_AT + wave * C::DS_WAVE;
+        f4 gq[M::NT][M::ND];
 #pragma unroll
-      for (int d = 0; d < M::ND; ++d) {
-        const typename M::TF gt = M::tr_frag(lds + C::G_AT, M::TRS, rc, d, i, g);
+        for (int u = 0; u < M::NT; ++u)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) gv[n][d] = M::acc(gt, pf[n], gv[n][d]);
-        const typename M::TF qt = M::tr_frag(lds, M::TRS, rc, d, i, g);
+          for (int d = 0; d < M::ND; ++d) gq[u][d] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) gk[n][d] = M::acc(qt, df[n], gk[n][d]);
+        for (int c = 0; c < NT / M::NT; ++c) {
+#pragma unroll
+          for (int h = 0; h < M::NT; ++h) {
+            const int n = c * M::NT + h;
+            char *at_key = mine + (16 * h + i) * C::DS_ROW + ((4 * g * M::SZ) ^ M::x(i));
+            if constexpr (M::WIDE) {
+              *reinterpret_cast<u4 *>(at_key) = df[n].v;
+            } else {
+              *reinterpret_cast<u2 *>(at_key) = u2{df[n].v[0], df[n].v[1]};
+              *reinterpret_cast<u2 *>(at_key + 32) = u2{df[n].v[2], df[n].v[3]};
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+          if (c == 0) by_rows();                                // products in the shadow of the first round trip
+#pragma unroll
+          for (int u = 0; u < M::NT; ++u) {
+            const typename M::PF st = {M::tr_frag(mine, C::DS_ROW, 0, u, i, g).v};
+#pragma unroll
+            for (int d = 0; d < M::ND; ++d)
+              gq[u][d] = M::acc(M::tr_frag(lds + C::K_AT, M::TRS, wave * 16 * NT + c * M::CH, d, i, g), st, gq[u][d]);
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+        float *red = reinterpret_cast<float *>(lds + C::RED_AT) + (wave * C::BR + rc) * C::RED_ROW;
+#pragma unroll
+        for (int u = 0; u < M::NT; ++u)
+#pragma unroll
+          for (int d = 0; d < M::ND; ++d) *reinterpret_cast<f4 *>(red + (16 * u + i) * C::RED_ROW + 16 * d + 4 * g) = gq[u][d];
       }
     }
     if constexpr (GQ) {                                         // the wavefronts' shares of the tile's gq

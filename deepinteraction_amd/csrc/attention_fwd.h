@@ -226,8 +226,8 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
               p[u][2 * h + 1] = (x >> 16) >= a.drop ? p[u][2 * h + 1] : 0.f;
             }
           }
+          M::pack(pf[t], u, p[u]);
         }
-        pf[t] = M::pack(p);
       }
 #pragma unroll
       for (int d = 0; d < M::ND; ++d) {
