@@ -39,8 +39,8 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   extern __shared__ __align__(16) char lds[];
   float *bias = reinterpret_cast<float *>(lds + C::BIAS_AT);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int wq = wave % WQ, wk = wave / WQ;
   const Where at = where(a);
+  const int wq = WQ == 1 ? 0 : (wave + at.sp + at.hk + at.b) % WQ, wk = wave / WQ;
   const int rows = a.G * a.L, ntile = (rows + 15) / 16;
   const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;

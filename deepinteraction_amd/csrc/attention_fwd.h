@@ -115,8 +115,9 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
   extern __shared__ __align__(16) char lds[];
   float *bias = reinterpret_cast<float *>(lds + C::BIAS_AT);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int wq = wave % WQ, wk = wave / WQ;
   const Where at = where(a);
+  // the wavefront that gets one row tile more than the others is not the same SIMD's in every workgroup
+  const int wq = WQ == 1 ? 0 : (wave + at.sp + at.hk + at.b) % WQ, wk = wave / WQ;
   const int rows = a.G * a.L, ntile = (rows + 15) / 16;
   const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
   if (a.splits > 1 && k0 >= k1) return;                         // the join knows the sample's keys, too
@@ -145,9 +146,10 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
     drow[t] = FULL && a.drop ? drop_row(seed_of(a), row_id + r) : 0;
   }
 
-  // one tile of keys; EDGE: keys are tested
-  auto tile = [&](auto edge, int t0) {
+  // one tile of keys for the wavefront's first N row tiles; EDGE: keys are tested
+  auto tile = [&](auto edge, auto count, int t0) {
     constexpr bool EDGE = decltype(edge)::value;
+    constexpr int N = decltype(count)::value;
 #pragma unroll
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;                 // first key of the chunk in the tile
@@ -155,7 +157,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
       unsigned may[MT][M::NT];                                  // in flight behind the products
       if (FULL && a.allowed != nullptr) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < N; ++t)
 #pragma unroll
           for (int u = 0; u < M::NT; ++u)
             may[t][u] = look(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words);
@@ -164,29 +166,29 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) s[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < N; ++t) s[t][u] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < M::NK; ++kk) {
           const typename M::RF kf = M::row_frag(lds + (kc + 16 * u + i) * M::ROWS, kk, g);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
+          for (int t = 0; t < N; ++t) s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
         }
         if (EDGE) {
           const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
+          for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][u][r] = bb[r] == 0.f ? s[t][u][r] : -INFINITY;
         }
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t) exclude(may[t][u], s[t][u]);
+          for (int t = 0; t < N; ++t) exclude(may[t][u], s[t][u]);
         }
       }
       float mx[MT];
       bool over = false;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int t = 0; t < N; ++t) {
         mx[t] = kLowest;
 #pragma unroll
         for (int u = 0; u < M::NT; ++u)
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
       }
       if (__any(over)) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
+        for (int t = 0; t < N; ++t) {
           float x = fmaxf(mx[t], __shfl_xor(mx[t], 16));
           x = fmaxf(x, __shfl_xor(x, 32));
           x = fmaxf(x, m[t]);
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
       }
       typename M::PF pf[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int t = 0; t < N; ++t) {
         f4 p[M::NT];
 #pragma unroll
         for (int u = 0; u < M::NT; ++u) {
@@ -233,10 +235,18 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
       for (int d = 0; d < M::ND; ++d) {
         const typename M::TF vf = M::tr_frag(lds + C::V_AT, M::TRS, kc, d, i, g);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) o[t][d] = M::acc(vf, pf[t], o[t][d]);
+        for (int t = 0; t < N; ++t) o[t][d] = M::acc(vf, pf[t], o[t][d]);
       }
     }
   };
+
+  auto each = [&](auto count, bool edge, int t0) {
+    if (edge) tile(std::true_type(), count, t0);
+    else tile(std::false_type(), count, t0);
+  };
+  // row tiles that are there: absent ones are left out where a wavefront has four (200 rows x 32 400 of 16 dims: float32 52 -> 49 us, half
+  // 37.9 -> 37.0); with two, the second copy of the loop cost more than it saved (511 x 4100 of 64 dims: 45 -> 50)
+  const int first = at.blk * MT * WQ + wq, mine = first < ntile ? min(MT, (ntile - first + WQ - 1) / WQ) : 0;
 
   KeyStage<C> st;
   st.init(a);
@@ -251,8 +261,9 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
     }
     __syncthreads();
     if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
-    if (edge) tile(std::true_type(), t0);
-    else tile(std::false_type(), t0);
+    if (MT <= 2 || mine == MT) each(std::integral_constant<int, MT>(), edge, t0);
+    else if (mine == MT - 1) each(std::integral_constant<int, (MT > 2 ? MT - 1 : 1)>(), edge, t0);
+    else if (mine > 0) each(std::integral_constant<int, (MT > 2 ? MT - 2 : 1)>(), edge, t0);
   }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
