@@ -100,16 +100,20 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
       for (int u = 0; u < M::NT; ++u) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) s[t][u] = dp[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+        typename M::RF kf[M::NK], vf[M::NK];                    // the tile's fragments before its first product
 #pragma unroll
         for (int kk = 0; kk < M::NK; ++kk) {
-          const typename M::RF kf = M::row_frag_x(lds + (kc + 16 * u + i) * M::TRS, kk, g, i);
-          const typename M::RF vf = M::row_frag(lds + C::V_AT + (kc + 16 * u + i) * M::ROWS, kk, g);
+          kf[kk] = M::row_frag_x(lds + (kc + 16 * u + i) * M::TRS, kk, g, i);
+          vf[kk] = M::row_frag(lds + C::V_AT + (kc + 16 * u + i) * M::ROWS, kk, g);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < M::NK; ++kk)
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
-            s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
-            dp[t][u] = M::dot(vf, gf[t][kk], dp[t][u]);
+            s[t][u] = M::dot(kf[kk], qf[t][kk], s[t][u]);
+            dp[t][u] = M::dot(vf[kk], gf[t][kk], dp[t][u]);
           }
-        }
         if (EDGE) {
           const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
 #pragma unroll
@@ -122,6 +126,10 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
           for (int t = 0; t < MT; ++t) exclude(may[t][u], s[t][u]);
         }
       }
+      typename M::TF kt[M::ND];                                 // in flight behind the exponentials
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d) kt[d] = M::tr_frag(lds, M::TRS, kc, d, i, g);
+      __builtin_amdgcn_sched_barrier(0);
       typename M::PF df[MT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
@@ -144,30 +152,30 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         }
       }
 #pragma unroll
-      for (int d = 0; d < M::ND; ++d) {
-        const typename M::TF kf = M::tr_frag(lds, M::TRS, kc, d, i, g);
+      for (int d = 0; d < M::ND; ++d)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t][d] = M::acc(kf, df[t], acc[t][d]);
-      }
+        for (int t = 0; t < MT; ++t) acc[t][d] = M::acc(kt[d], df[t], acc[t][d]);
     }
   };
 
   KeyStage<C> st;
   st.init(a);
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
-  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
+  auto step = [&](auto edge, int t0) {
     __syncthreads();
     st.template commit<true, false>(lds, C::V_AT);
-    const bool edge = km != nullptr || t0 + C::TILE > k1;
-    if (edge && threadIdx.x < C::TILE) {
+    if (decltype(edge)::value && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
       bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
     }
     __syncthreads();
     if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
-    if (edge) tile(std::true_type(), t0);
-    else tile(std::false_type(), t0);
-  }
+    tile(edge, t0);
+  };
+  int t0 = k0;
+  if (km == nullptr)
+    for (; t0 + C::TILE <= k1; t0 += C::TILE) step(std::false_type(), t0);
+  for (; t0 < k1; t0 += C::TILE) step(std::true_type(), t0);
 
   if constexpr (WQ == 1) {                                      // add the four wavefronts (MT = 1)
     float *j = reinterpret_cast<float *>(lds);

@@ -150,6 +150,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
   auto tile = [&](auto edge, auto count, int t0) {
     constexpr bool EDGE = decltype(edge)::value;
     constexpr int N = decltype(count)::value;
+    constexpr bool EARLY = true;
 #pragma unroll
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;                 // first key of the chunk in the tile
@@ -162,17 +163,21 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
           for (int u = 0; u < M::NT; ++u)
             may[t][u] = look(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words);
       }
+      typename M::RF kf[M::NT][M::NK];                          // all of the chunk's before its first product: one wait, not one each
+#pragma unroll
+      for (int u = 0; u < M::NT; ++u)
+#pragma unroll
+        for (int kk = 0; kk < M::NK; ++kk) kf[u][kk] = M::row_frag(lds + (kc + 16 * u + i) * M::ROWS, kk, g);
+      if (EARLY) __builtin_amdgcn_sched_barrier(0);
       f4 s[MT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
 #pragma unroll
         for (int t = 0; t < N; ++t) s[t][u] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < M::NK; ++kk) {
-          const typename M::RF kf = M::row_frag(lds + (kc + 16 * u + i) * M::ROWS, kk, g);
+        for (int kk = 0; kk < M::NK; ++kk)
 #pragma unroll
-          for (int t = 0; t < N; ++t) s[t][u] = M::dot(kf, qf[t][kk], s[t][u]);
-        }
+          for (int t = 0; t < N; ++t) s[t][u] = M::dot(kf[u][kk], qf[t][kk], s[t][u]);
         if (EDGE) {
           const f4 bb = *reinterpret_cast<const f4 *>(bias + kc + 16 * u + 4 * g);
 #pragma unroll
@@ -210,6 +215,10 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
           for (int d = 0; d < M::ND; ++d) o[t][d] *= f;
         }
       }
+      typename M::TF vf[M::ND];                                 // in flight behind the exponentials
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d) vf[d] = M::tr_frag(lds + C::V_AT, M::TRS, kc, d, i, g);
+      if (EARLY) __builtin_amdgcn_sched_barrier(0);
       typename M::PF pf[MT];
 #pragma unroll
       for (int t = 0; t < N; ++t) {
@@ -232,18 +241,12 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
         }
       }
 #pragma unroll
-      for (int d = 0; d < M::ND; ++d) {
-        const typename M::TF vf = M::tr_frag(lds + C::V_AT, M::TRS, kc, d, i, g);
+      for (int d = 0; d < M::ND; ++d)
 #pragma unroll
-        for (int t = 0; t < N; ++t) o[t][d] = M::acc(vf, pf[t], o[t][d]);
-      }
+        for (int t = 0; t < N; ++t) o[t][d] = M::acc(vf[d], pf[t], o[t][d]);
     }
   };
 
-  auto each = [&](auto count, bool edge, int t0) {
-    if (edge) tile(std::true_type(), count, t0);
-    else tile(std::false_type(), count, t0);
-  };
   // row tiles that are there: absent ones are left out where a wavefront has four (200 rows x 32 400 of 16 dims: float32 52 -> 49 us, half
   // 37.9 -> 37.0); with two, the second copy of the loop cost more than it saved (511 x 4100 of 64 dims: 45 -> 50)
   const int first = at.blk * MT * WQ + wq, mine = first < ntile ? min(MT, (ntile - first + WQ - 1) / WQ) : 0;
@@ -251,20 +254,23 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
   KeyStage<C> st;
   st.init(a);
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
-  for (int t0 = k0; t0 < k1; t0 += C::TILE) {
+  auto step = [&](auto edge, int t0) {
     __syncthreads();                                            // the last tile's reads are done
     st.template commit<false, true>(lds, C::V_AT);
-    const bool edge = km != nullptr || t0 + C::TILE > k1;
-    if (edge && threadIdx.x < C::TILE) {
+    if (decltype(edge)::value && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
       bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
     }
     __syncthreads();
     if (t0 + C::TILE < k1) st.fetch(a, kb, vb, km, t0 + C::TILE, k1);
-    if (MT <= 2 || mine == MT) each(std::integral_constant<int, MT>(), edge, t0);
-    else if (mine == MT - 1) each(std::integral_constant<int, (MT > 2 ? MT - 1 : 1)>(), edge, t0);
-    else if (mine > 0) each(std::integral_constant<int, (MT > 2 ? MT - 2 : 1)>(), edge, t0);
-  }
+    if (MT <= 2 || mine == MT) tile(edge, std::integral_constant<int, MT>(), t0);
+    else if (mine == MT - 1) tile(edge, std::integral_constant<int, (MT > 2 ? MT - 1 : 1)>(), t0);
+    else if (mine > 0) tile(edge, std::integral_constant<int, (MT > 2 ? MT - 2 : 1)>(), t0);
+  };
+  int t0 = k0;
+  if (km == nullptr)
+    for (; t0 + C::TILE <= k1; t0 += C::TILE) step(std::false_type(), t0);
+  for (; t0 < k1; t0 += C::TILE) step(std::true_type(), t0);
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     l[t] += __shfl_xor(l[t], 16);
