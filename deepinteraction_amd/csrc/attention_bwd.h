@@ -361,23 +361,33 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
       if (t0 + rc >= r1 || (GQ && wave >= waves)) break;
       if (FULL && a.allowed != nullptr && (!MASK_AHEAD || (t0 == r0 && rc == 0))) look(t0 + rc);
       typename M::PF pf[NT], df[NT];
+      typename M::TF gt_[M::ND];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
         const int rfirst = t0 + rc + 16 * u + 4 * g;
         f4 s[NT], dp[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n] = dp[n] = f4{0.f, 0.f, 0.f, 0.f};
+        typename M::RF qf[M::NK], gf[M::NK];                    // the tile's fragments before its first product
 #pragma unroll
         for (int kk = 0; kk < M::NK; ++kk) {
-          const typename M::RF qf = M::row_frag_x(lds + (rc + 16 * u + i) * M::TRS, kk, g, i);
-          const typename M::RF gf = M::row_frag_x(lds + C::G_AT + (rc + 16 * u + i) * M::TRS, kk, g, i);
+          qf[kk] = M::row_frag_x(lds + (rc + 16 * u + i) * M::TRS, kk, g, i);
+          gf[kk] = M::row_frag_x(lds + C::G_AT + (rc + 16 * u + i) * M::TRS, kk, g, i);
+        }
+        if (!GQ) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < M::NK; ++kk)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            s[n] = M::dot(qf, kf[n][kk], s[n]);
-            dp[n] = M::dot(gf, vf[n][kk], dp[n]);
+            s[n] = M::dot(qf[kk], kf[n][kk], s[n]);
+            dp[n] = M::dot(gf[kk], vf[n][kk], dp[n]);
           }
-        }
         const f4 l4 = *reinterpret_cast<const f4 *>(slse + rc + 16 * u + 4 * g), d4 = *reinterpret_cast<const f4 *>(sdelta + rc + 16 * u + 4 * g);
+        if (!GQ && u == M::NT - 1) {                            // go^T in flight behind the last exponentials
+#pragma unroll
+          for (int d = 0; d < M::ND; ++d) gt_[d] = M::tr_frag(lds + C::G_AT, M::TRS, rc, d, i, g);
+          __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (FULL && a.allowed != nullptr) {
@@ -412,9 +422,12 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
       auto by_rows = [&]() {                                    // gv^T += go^T P, gk^T += Q^T dS
 #pragma unroll
         for (int d = 0; d < M::ND; ++d) {
-          const typename M::TF gt = M::tr_frag(lds + C::G_AT, M::TRS, rc, d, i, g);
+          const typename M::TF gt = GQ ? M::tr_frag(lds + C::G_AT, M::TRS, rc, d, i, g) : gt_[d];
 #pragma unroll
           for (int n = 0; n < NT; ++n) gv[n][d] = M::acc(gt, pf[n], gv[n][d]);
+        }
+#pragma unroll
+        for (int d = 0; d < M::ND; ++d) {
           const typename M::TF qt = M::tr_frag(lds, M::TRS, rc, d, i, g);
 #pragma unroll
           for (int n = 0; n < NT; ++n) gk[n][d] = M::acc(qt, df[n], gk[n][d]);
