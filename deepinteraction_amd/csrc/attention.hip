@@ -96,11 +96,19 @@ static int check(const di_attention *t) {
   const long long most = (long long)t->B * t->kv_heads * ((rows > t->S ? rows : t->S) / 4 + 2);
   DI_REQUIRE(most <= 0x7fffffff / 2, "attention: too many rows for one launch");
   const int sz = t->dtype == DI_F32 ? 4 : 2;
+  // rows of the output - and of the keys' gradients - are addressed as those of the inputs
+  DI_REQUIRE((long long)t->heads * t->head_dim * sz < (1ll << 24), "attention: %d heads of %d (rows of 16 MB and more)", t->heads, t->head_dim);
   if (t->B == 0) return DI_OK;
   DI_REQUIRE(t->L == 0 || (t->q != nullptr && aligned(t->q, t->q_bs, t->q_rs, sz)), "attention: q must start and step on 16 bytes, its rows less than 16 MB apart");
   DI_REQUIRE(t->S == 0 || (t->k != nullptr && t->v != nullptr && aligned(t->k, t->k_bs, t->k_rs, sz) && aligned(t->v, t->v_bs, t->v_rs, sz)),
              "attention: k and v must start and step on 16 bytes, their rows less than 16 MB apart");
   return DI_OK;
+}
+
+// rows of a gradient lie apart: each is written once
+static bool apart(const di_attention &t, long long bs, long long rs) {
+  const long long E = (long long)t.kv_heads * t.head_dim;
+  return (t.S == 1 || rs >= E) && (t.B == 1 || bs >= E || bs <= -E);
 }
 
 static Args args_of(const di_attention *t) {
@@ -179,6 +187,7 @@ int di_attention_bwd(const di_attention *t, const void *out, const float *lse, c
              "attention: out, grad_out and grad_q must start (and grad_out step) on 16 bytes");
   DI_REQUIRE(t->S == 0 || (gk && gv && aligned(gk, gk_bs, gk_rs, sz) && aligned(gv, gv_bs, gv_rs, sz)),
              "attention: grad_k and grad_v must start and step on 16 bytes");
+  DI_REQUIRE(t->S == 0 || (apart(*t, gk_bs, gk_rs) && apart(*t, gv_bs, gv_rs)), "attention: rows of grad_k or grad_v overlap");
   DI_REQUIRE((workspace != nullptr || t->L == 0) && ((uintptr_t)workspace & 15) == 0, "attention: workspace");   // no rows: one range, no sums
   Plan p, k;
   if (int rc = plan_rows(*t, false, p)) return rc;

@@ -1357,7 +1357,7 @@ def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None
     else:
         gk, gv = grads_kv
         for x in (gk, gv):
-            if x.shape != k.shape or x.dtype != k.dtype or _seq_view(x)[0] is not x or (t.B > 1 and x.stride(0) == 0):
+            if x.shape != k.shape or x.dtype != k.dtype or (x.numel() and _seq_view(x)[0] is not x):
                 raise ValueError('cross_attention: grads_kv have the shape and type of k, contiguous columns and rows on 16 bytes')
         k_strides, v_strides = _seq_view(gk)[1:], _seq_view(gv)[1:]
     ref = ctypes.addressof(t)
