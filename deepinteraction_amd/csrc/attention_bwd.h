@@ -71,9 +71,10 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
     }
     d += __shfl_xor(d, 16);
     d += __shfl_xor(d, 32);
-    delta[t] = d;
     const float e = ok ? a.lse[row_id + r] : INFINITY;
-    lse[t] = e == -INFINITY ? INFINITY : e;                     // an empty row: every probability 0
+    lse[t] = e == -INFINITY ? INFINITY : e;                     // an empty row: every probability 0, and no gradient whatever it holds
+    if (e == -INFINITY) d = 0.f;
+    delta[t] = d;
     if (ok && at.sp == 0 && wk == 0 && g == 0) a.delta[row_id + row[t]] = d;
 #pragma unroll
     for (int j = 0; j < M::ND; ++j) acc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
@@ -177,6 +178,14 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
     for (; t0 + C::TILE <= k1; t0 += C::TILE) step(std::false_type(), t0);
   for (; t0 < k1; t0 += C::TILE) step(std::true_type(), t0);
 
+  if (FULL) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int d = 0; d < M::ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[t][d][r] = lse[t] == INFINITY ? 0.f : acc[t][d][r];
+  }
   if constexpr (WQ == 1) {                                      // add the four wavefronts (MT = 1)
     float *j = reinterpret_cast<float *>(lds);
     __syncthreads();
@@ -227,6 +236,7 @@ struct GkvCfg {
   static constexpr int NP = (BR * M::PPR + 255) / 256;
   // P of a normalised row is about 1 / S: in float16 it is scaled by 2^14 (the largest power of two whose product with 1 is finite
   // with room to spare) so that probabilities down to 2^-28 keep their 11 bits; exact to undo
+  // Score gradients are rounded as they are: they follow grad_out's size, which a loss scale sets, down to float16's 2^-25 absolute
   static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f, P_LOG2 = TY == DI_F16 ? 14.f : 0.f;
 };
 
@@ -251,6 +261,8 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
   constexpr int STEP = 256 / M::PPR;
   u4 qs[C::NP], gs[C::NP], os[C::NP];                           // os: GQ forms delta from the forward's output
   float ls = INFINITY, de = 0.f;
+  bool empty[C::NP];                                            // (query, key) mask: rows that it leaves without keys become zeros, so that
+                                                                // what they hold - a NaN - meets no product over the rows
   const int piece = tid % M::PPR, first = tid / M::PPR;
   const bool in = piece * 16 < a.D * M::SZ && (C::BR >= STEP || first < C::BR);
   const unsigned qo = (unsigned)(first * a.q_rs) + piece * 16, go = (unsigned)(first * a.go_rs) + piece * 16;
@@ -284,6 +296,13 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
           gs[j] = *reinterpret_cast<const u4 *>(gb + l * a.go_rs + col);
           if (GQ) os[j] = *reinterpret_cast<const u4 *>(ob + l * o_rs + col);
         }
+      }
+    }
+    if (FULL && a.allowed != nullptr) {
+#pragma unroll
+      for (int j = 0; j < C::NP; ++j) {
+        const int r = t0 + first + j * STEP;
+        empty[j] = r < r1 && a.lse[row_id + r] == -INFINITY;
       }
     }
     if (tid < C::BR) {
@@ -339,6 +358,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
     if (C::BR >= STEP || first < C::BR) {
 #pragma unroll
       for (int j = 0; j < C::NP; ++j) {
+        if (FULL && a.allowed != nullptr && empty[j]) qs[j] = gs[j] = os[j] = u4{0, 0, 0, 0};
         const int at_row = (first + j * STEP) * M::TRS + ((piece * 16) ^ M::x(first + j * STEP));
         *reinterpret_cast<u4 *>(lds + at_row) = qs[j];
         *reinterpret_cast<u4 *>(lds + C::G_AT + at_row) = gs[j];

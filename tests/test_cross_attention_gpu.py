@@ -162,6 +162,39 @@ def test_excluded_keys_may_hold_anything(t, L, S, D):
     assert not got[3][dead].any() and not got[4][dead].any()
 
 
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('L,S,D', [(1, 300, 16), (70, 300, 16), (200, 40, 32), (40, 130, 64), (150, 200, 128), (5, 700, 128)])
+def test_queries_without_keys_may_hold_anything(t, L, S, D):
+    """A padded query: nothing allowed, NaN in its projection and its incoming gradient.  It gives zeros and reaches no other gradient."""
+    B, H = 2, 2
+    q, k, v, go = make(B, L, S, H, 1, D, t)
+    allowed = torch.rand(B, L, S, device='cuda') < 0.6
+    pad = torch.rand(B, L, device='cuda') < 0.4
+    pad[0, 0], pad[1, 0] = True, False
+    allowed &= ~pad[..., None]
+    allowed[..., 0] |= ~pad
+    q, go = q.clone(), go.clone()
+    go[pad] = 0
+    clean = check(q, k, v, go, H, allowed, allowed=allowed)
+    q[pad], go[pad] = float('nan'), float('nan')
+    go[0, 0] = float('inf')
+    o, lse = ops.cross_attention_train_fwd(q, k, v, H, allowed=allowed)
+    got = (o, lse) + ops.cross_attention_train_bwd(q, k, v, o, go, lse, H, allowed=allowed)
+    assert all(torch.equal(a, b) for a, b in zip(got, clean))
+    assert not got[0][pad].any() and not got[2][pad].any()
+
+
+@pytest.mark.parametrize('D', [16, 64])
+def test_gradients_that_would_overlap_are_refused(D):
+    q, k, v, go = make(2, 5, 9, 2, 2, D, F16)
+    o, lse = ops.cross_attention_train_fwd(q, k, v, 2)
+    for bad in (k.new_empty(2, 1, 2 * D).expand(2, 9, 2 * D), k.new_empty(1, 9, 2 * D).expand(2, 9, 2 * D),
+                k.new_empty(64 * D).as_strided((2, 9, 2 * D), (24 * D, D, 1))):
+        for pair in ((bad, v), (v, bad)):
+            with pytest.raises((ValueError, ops._lib.HipLibraryError)):
+                ops.cross_attention_train_bwd(q, k, v, o, go, lse, 2, grads_kv=pair)
+
+
 def test_nothing_to_attend_to():
     for t in TYPES:
         for B, L, S in ((2, 5, 0), (2, 0, 7), (0, 3, 4), (2, 100, 0)):
