@@ -238,6 +238,8 @@ struct Args {
   bool allowed_words;                    // every row of `allowed` starts on 4 bytes
   Div by_unit, by_blocks, by_hk, by_splits, by_L;              // unit = blocks * Hk
   int even;                              // blocks of the whole turns of 8 units
+  bool ragged;                           // key lengths, few samples, more workgroups than CUs: blocks with keys first (where_ragged)
+  Div by_walk, by_inner;                 // ragged: keys per step of a sample's blocks, blocks per step
   float scale2;                          // softmax scale * log2(e)
   float scale;
   unsigned drop;                         // threshold of 65536; 0 = no dropout
@@ -254,7 +256,66 @@ __device__ __forceinline__ unsigned long long seed_of(const Args &a) { return a.
 struct Where {
   int blk, hk, sp, b;
 };
+
+__device__ __forceinline__ int keys_of(const Args &a, int b) {
+  if (a.klen == nullptr) return a.S;
+  const int n = a.klen[b];
+  return n < 0 ? 0 : (n < a.S ? n : a.S);
+}
+
+// Samples of different lengths: the workgroups that have keys come first - dealt out to the XCDs as above, key blocks (equal work) in
+// equal consecutive shares - and those without behind them.  Every wavefront finds its sample from the running sum of the samples' workgroups with keys (a lane each, so up
+// to 64 samples).  A sample's workgroups are ordered by what its length cuts off: key ranges (row blocks), key blocks (KEYS).
+// (4 x 511 x 4100, 2733, 1366, 0, four heads of 64 to a key head: gk and gv 121 -> 80 us, gq 54 -> 46, forward 41 -> 33; single
+// queries of 16 samples with 0 .. 32 768 keys: 205 -> 196)
+template <bool KEYS>
+__device__ __forceinline__ Where where_ragged(const Args &a) {
+  const int lane = threadIdx.x & 63, steps = KEYS ? a.blocks : a.splits, inner = (int)a.by_inner.d, all = steps * inner;
+  int mine = 0;
+  if (lane < a.B) mine = min(steps, (int)a.by_walk.of(keys_of(a, lane) + a.by_walk.d - 1)) * inner;
+  int upto = mine;
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) {
+    const int y = __shfl_up(upto, x);
+    if (lane >= x) upto += y;
+  }
+  const int with = __builtin_amdgcn_readlane(upto, 63);
+  int id = blockIdx.x, b;
+  if (id < with) {
+    if (KEYS) {
+      id = xcd_remap(id, with);
+    } else {                                                    // ranges of unequal length: whole units in turn, the last few in chunks
+      const int even = (int)a.by_inner.of(with) / 8 * 8 * inner, xcd = id % 8, j = id / 8, turn = a.by_inner.of(j);
+      id = id < even ? (turn * 8 + xcd) * inner + (j - turn * inner) : even + xcd_remap(id - even, with - even);
+    }
+    b = __builtin_popcountll(__ballot(upto <= id));            // samples that end before it (lanes behind the last one end at `with`)
+    id -= __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(mine, b);
+  } else {
+    id -= with;
+    const int none = (lane + 1) * all - upto;
+    b = __builtin_popcountll(__ballot(lane < a.B && none <= id));
+    const int has = __builtin_amdgcn_readlane(mine, b);
+    id += has - (__builtin_amdgcn_readlane(none, b) - (all - has));
+  }
+  Where w;
+  w.b = b;
+  if (KEYS) {
+    w.blk = a.by_inner.of(id);
+    const int at = id - w.blk * inner;
+    w.sp = a.by_hk.of(at);
+    w.hk = at - w.sp * a.Hk;
+  } else {
+    const int next = a.by_blocks.of(id);
+    w.blk = id - next * a.blocks;
+    w.sp = a.by_hk.of(next);
+    w.hk = next - w.sp * a.Hk;
+  }
+  return w;
+}
+
+template <bool KEYS>
 __device__ __forceinline__ Where where(const Args &a) {
+  if (a.ragged) return where_ragged<KEYS>(a);
   const int unit = a.blocks * a.Hk;
   int id = blockIdx.x;
   if (id < a.even) {
@@ -273,12 +334,6 @@ __device__ __forceinline__ Where where(const Args &a) {
   w.b = a.by_splits.of(id);
   w.sp = id - w.b * a.splits;
   return w;
-}
-
-__device__ __forceinline__ int keys_of(const Args &a, int b) {
-  if (a.klen == nullptr) return a.S;
-  const int n = a.klen[b];
-  return n < 0 ? 0 : (n < a.S ? n : a.S);
 }
 
 }  // namespace at

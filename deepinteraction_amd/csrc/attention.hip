@@ -25,8 +25,15 @@ static void cut(Plan &p, long long problems, int rows, int per_block, int walked
 // Rows per workgroup and ranges of the keys.  Up to 16 rows (single queries): 24 workgroups a CU, the memory streams best through many
 // short ranges (16 samples x 8 key heads of 128, up to 32 768 keys, with the join: 8 a CU 246 us, 16 229, 24 220).  More rows: what is
 // resident - two workgroups a CU, one for gq of 128 dims (2048 x 8192 x 16 heads of 128, forward: 1 a CU 263 us, 2 211, 3 229; gq: 1 a
-// CU 290, 2 317) - and three times that where the samples' lengths differ, so that short ones make room (4 x 511 x up to 4100, four heads
-// of 64 to a key head, forward + gq: 2 a CU 161 us, 4 154, 6 123, 8 132).  Too few row blocks for the CUs: 64 rows a workgroup.
+// CU 290, 2 317) - and twice that where the samples' lengths differ and some ranges have no keys (4 x 511 x 4100, 2733, 1366, 0, four
+// heads of 64 to a key head, forward + gq with their joins: 2 a CU 127 us, 4 95, 6 100, 8 118; four lengths of 1025 .. 4100: 132, 113,
+// 119, 128).  Too few row blocks for the CUs: 64 rows a workgroup.
+// Key lengths: the samples of an unbalanced batch load the XCDs evenly (where_ragged in attention.h) - if there is more than one workgroup
+// a CU to place, and no more samples than lanes to look them up.
+static bool ragged(const di_attention &t, const Plan &p, int cus) {
+  return t.key_lengths != nullptr && t.B <= 64 && (long long)t.B * t.kv_heads * p.blocks * p.splits > cus;
+}
+
 static int plan_rows(const di_attention &t, bool forward, Plan &p) {
   const int cus = device_cus();
   if (cus <= 0) return DI_ERR_LAUNCH;
@@ -35,15 +42,17 @@ static int plan_rows(const di_attention &t, bool forward, Plan &p) {
   if (rows <= 16) {
     p.big = 0;
     cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, 24ll * cus);
+    p.ragged = ragged(t, p, cus);
     return DI_OK;
   }
-  const long long want = (forward || DP < 128 ? 2ll : 1ll) * cus * (t.key_lengths != nullptr ? 3 : 1);
+  const long long want = (forward || DP < 128 ? 2ll : 1ll) * cus * (t.key_lengths != nullptr ? 2 : 1);
   p.big = 2;
   cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, want);
   if (rows <= 64 || problems * p.blocks * p.splits < cus) {
     p.big = 1;
     cut(p, problems, rows, 64, t.S, 64, 4, want);
   }
+  p.ragged = ragged(t, p, cus);
   return DI_OK;
 }
 
@@ -57,9 +66,10 @@ static int plan_keys(const di_attention &t, Plan &p) {
   for (p.big = key_tiles(t.dtype, DP); p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
     if (32 * p.big >= t.S) continue;
     cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
-    if (problems * p.blocks * p.splits >= cus) return DI_OK;
+    if (problems * p.blocks * p.splits >= cus) break;
   }
-  cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
+  if (p.big <= least) cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
+  p.ragged = ragged(t, p, cus);
   return DI_OK;
 }
 

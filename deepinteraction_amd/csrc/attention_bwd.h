@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   extern __shared__ __align__(16) char lds[];
   float *bias = reinterpret_cast<float *>(lds + C::BIAS_AT);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const Where at = where(a);
+  const Where at = where<false>(a);
   const int wq = WQ == 1 ? 0 : (wave + at.sp + at.hk + at.b) % WQ, wk = wave / WQ;
   const int rows = a.G * a.L, ntile = (rows + 15) / 16;
   const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
   extern __shared__ __align__(16) char lds[];
   float *slse = reinterpret_cast<float *>(lds + C::ST_AT), *sdelta = slse + C::BR;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
-  const Where at = where(a);
+  const Where at = where<true>(a);
   const int rows = a.G * a.L, nkeys = keys_of(a, at.b);
   const int key0 = at.blk * C::KEYS;
   // a block without keys: zeros (the only block: gq's zeros, too)

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
   extern __shared__ __align__(16) char lds[];
   float *bias = reinterpret_cast<float *>(lds + C::BIAS_AT);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const Where at = where(a);
+  const Where at = where<false>(a);
   // the wavefront that gets one row tile more than the others is not the same SIMD's in every workgroup
   const int wq = WQ == 1 ? 0 : (wave + at.sp + at.hk + at.b) % WQ, wk = wave / WQ;
   const int rows = a.G * a.L, ntile = (rows + 15) / 16;

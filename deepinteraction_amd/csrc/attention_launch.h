@@ -55,7 +55,8 @@ static int gkv(const Args &a, hipStream_t s) {
                        : go(attention_gkv_kernel<TY, DP, NT, GQ, false>, plain, lds, grid, a, s, "attention_gkv");
 }
 
-static void take(Args &a, const Plan &p) {
+// walk: the keys per range (row blocks) or per block (key blocks)
+static void take(Args &a, const Plan &p, int walk, int inner) {
   a.blocks = p.blocks;
   a.splits = p.splits;
   a.range = p.range;
@@ -66,12 +67,15 @@ static void take(Args &a, const Plan &p) {
   a.by_hk = div_by(a.Hk);
   a.by_splits = div_by(a.splits);
   a.by_L = div_by(a.L);
+  a.ragged = p.ragged;
+  a.by_walk = div_by(walk);
+  a.by_inner = div_by(inner);
 }
 
 template <int TY>
 int launch_fwd(const Args &args, const Plan &p, hipStream_t s) {
   Args a = args;
-  take(a, p);
+  take(a, p, p.range, p.blocks * a.Hk);
   int rc;
 #define DI_AT_FWD(DP) \
   rc = p.big == 0 ? fwd<TY, DP, 1, 1>(a, s) : p.big == 1 ? fwd<TY, DP, 1, 4>(a, s) : fwd<TY, DP, row_tiles(DP), 4>(a, s)
@@ -91,7 +95,7 @@ int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) 
   Args a = args;
   int rc = DI_OK;
   if (!one_launch(padded(a.D))) {
-    take(a, pq);
+    take(a, pq, pq.range, pq.blocks * a.Hk);
 #define DI_AT_GQ(DP) \
   rc = pq.big == 0 ? gq<TY, DP, 1, 1>(a, s) : pq.big == 1 ? gq<TY, DP, 1, 4>(a, s) : gq<TY, DP, row_tiles(DP), 4>(a, s)
     if (a.L > 0) {
@@ -103,7 +107,7 @@ int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) 
     if (a.L > 0 && pq.splits > 1 && (rc = join<TY, false>(a, s)) != DI_OK) return rc;
     if (a.S == 0) return DI_OK;
   }
-  take(a, pk);
+  take(a, pk, 64 * pk.big, pk.splits * a.Hk);
 #define DI_AT_GKV(DP)                                                                                                      \
   do {                                                                                                                     \
     constexpr int most = key_tiles(TY, DP), least = least_key_tiles(DP);                                                   \

@@ -8,6 +8,7 @@ namespace at {
 struct Plan {
   int big;                               // rows: 0 = up to 16, 1 = up to 64, 2 = more; keys: tiles per wavefront
   int blocks, splits, range;
+  bool ragged;                           // workgroups with keys first
 };
 
 template <int TY>

@@ -144,6 +144,19 @@ def test_masks(t, D, H, Hk, L, S):
     check(q, k, v, go, H, allowed[:1].expand(B, L, S), allowed=allowed[:1].expand(B, L, S))
 
 
+@pytest.mark.parametrize('t', [F32, F16], ids=str)
+@pytest.mark.parametrize('B,L,S,H,Hk,D', [(5, 200, 1500, 8, 8, 64), (16, 1, 1400, 8, 4, 64), (64, 40, 130, 4, 2, 64), (65, 40, 130, 4, 2, 64), (9, 90, 700, 8, 8, 16),
+                                          (3, 600, 900, 4, 4, 128), (1, 300, 5000, 8, 8, 32), (6, 70, 400, 16, 16, 128), (64, 1, 600, 8, 8, 16)])
+def test_batches_of_different_lengths(B, L, S, H, Hk, D, t):
+    """More workgroups than compute units: those with keys are put first; no key at all, one, a range's worth, all of them."""
+    q, k, v, go = make(B, L, S, H, Hk, D, t)
+    for kind in range(3):
+        n = [[S, 0, 1, S - 1, 64, 65, S // 2, 128, 17][(3 * b + kind) % 9] if kind < 2 else 0 for b in range(B)]
+        n = torch.tensor(n, dtype=torch.int32, device='cuda')
+        keep = (torch.arange(S, device='cuda')[None, None] < n[:, None, None]).expand(B, L, S)
+        check(q, k, v, go, H, keep, key_lengths=n)
+
+
 @pytest.mark.parametrize('t', TYPES, ids=str)
 @pytest.mark.parametrize('L,S,D', [(1, 300, 16), (70, 300, 16), (1, 300, 128), (40, 130, 64)])
 def test_excluded_keys_may_hold_anything(t, L, S, D):
