@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
 template <int TY, int DP, int NT, bool GQ>
 struct GkvCfg {
   using M = Mm<TY, DP>;
-  static constexpr int BR = DP * M::SZ >= 256 || (GQ && DP > 16) ? 32 : 64;        // rows per tile
+  static constexpr int BR = DP * M::SZ >= 512 || (GQ && DP > 16) ? 32 : 64;        // rows per tile
   static constexpr int KEYS = 64 * NT;
   static constexpr int G_AT = BR * M::TRS, ST_AT = 2 * G_AT;    // both tiles are read in rows and transposed
   static constexpr int K_AT = ST_AT + 2 * BR * 4;               // GQ: the block's keys,

@@ -21,7 +21,7 @@ constexpr int row_tiles(int DP) { return DP <= 32 ? 4 : 2; }                    
 constexpr bool one_launch(int DP) { return DP <= 32; }                              // the backward's key-block kernel forms gq as well
 constexpr int key_tiles(int TY, int DP) { return DP == 16 ? 4 : DP == 32 ? (TY == DI_F32 ? 2 : 4) : (TY == DI_F32 && DP == 128 ? 1 : 2); }   // most NT
 constexpr int least_key_tiles(int DP) { return one_launch(DP) ? 2 : 1; }            // 16-bit products contract over 32 keys
-constexpr int tile_rows(int TY, int DP) { return DP * (TY == DI_F32 ? 4 : 2) >= 256 || DP == 32 ? 32 : 64; }
+constexpr int tile_rows(int TY, int DP) { return DP * (TY == DI_F32 ? 4 : 2) >= 512 || DP == 32 ? 32 : 64; }
 
 }  // namespace at
 }  // namespace di
