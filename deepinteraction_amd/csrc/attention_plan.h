@@ -19,7 +19,9 @@ int launch_bwd(const Args &a, const Plan &gq, const Plan &gkv, hipStream_t s);
 constexpr int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 constexpr int row_tiles(int DP) { return DP <= 32 ? 4 : 2; }                       // MT of the large variant
 constexpr bool one_launch(int DP) { return DP <= 32; }                              // the backward's key-block kernel forms gq as well
-constexpr int key_tiles(int TY, int DP) { return DP == 16 ? 4 : DP == 32 ? (TY == DI_F32 ? 2 : 4) : (TY == DI_F32 && DP == 128 ? 1 : 2); }   // most NT
+// Key tiles per wavefront at the most.  Heads of 128: one, two wavefronts a SIMD (2048 x 8192 x 16 heads, bf16: 380 us; two tiles, whose
+// sums leave room for one: 394).  Heads of 64: two (161 us; one: 189)
+constexpr int key_tiles(int TY, int DP) { return DP == 16 ? 4 : DP == 32 ? (TY == DI_F32 ? 2 : 4) : DP == 64 ? 2 : 1; }
 constexpr int least_key_tiles(int DP) { return one_launch(DP) ? 2 : 1; }            // 16-bit products contract over 32 keys
 constexpr int tile_rows(int TY, int DP) { return DP * (TY == DI_F32 ? 4 : 2) >= 512 || DP == 32 ? 32 : 64; }
 
