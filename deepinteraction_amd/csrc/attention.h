@@ -235,7 +235,6 @@ struct Args {
   int B, L, S, Hk, G, D;
   int splits, range;                     // key (or row) ranges of a split grid
   int blocks;                            // row blocks (or key blocks)
-  bool allowed_words;                    // every row of `allowed` starts on 4 bytes
   Div by_unit, by_blocks, by_hk, by_splits, by_L;              // unit = blocks * Hk
   int even;                              // blocks of the whole turns of 8 units
   bool ragged;                           // key lengths, few samples, more workgroups than CUs: blocks with keys first (where_ragged)

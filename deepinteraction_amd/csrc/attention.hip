@@ -63,7 +63,10 @@ static int plan_keys(const di_attention &t, Plan &p) {
   const int tile = tile_rows(t.dtype, DP);
   const long long problems = (long long)t.B * t.kv_heads;
   const int S = t.S > 0 ? t.S : 1;                              // without keys, one block still writes gq's zeros
-  for (p.big = key_tiles(t.dtype, DP); p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
+  const bool full = t.key_mask != nullptr || t.allowed != nullptr || t.dropout_p > 0.f;
+  p.big = key_tiles(t.dtype, DP);
+  if (full && p.big > most_masked_key_tiles) p.big = most_masked_key_tiles;
+  for (; p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
     if (32 * p.big >= t.S) continue;
     cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
     if (problems * p.blocks * p.splits >= cus) break;
@@ -131,7 +134,6 @@ static Args args_of(const di_attention *t) {
   a.klen = t->key_lengths;
   if (t->S > 0) {                                              // no keys: nothing that a mask could exclude
     a.kmask = t->key_mask; a.kmask_bs = t->key_mask_bs;
-    a.allowed_words = ((uintptr_t)t->allowed & 3) == 0 && t->allowed_bs % 4 == 0 && t->allowed_rs % 4 == 0;
     a.allowed = t->allowed; a.allowed_bs = t->allowed_bs; a.allowed_rs = t->allowed_rs;
   }
   a.B = t->B; a.L = t->L; a.S = t->S; a.Hk = t->kv_heads; a.G = t->heads / t->kv_heads; a.D = t->head_dim;

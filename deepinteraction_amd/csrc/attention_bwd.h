@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int u = 0; u < M::NT; ++u)
-            may[t][u] = look(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words);
+            may[t][u] = look<EDGE>(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S);
       }
       f4 s[MT][M::NT], dp[MT][M::NT];
 #pragma unroll
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
         }
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t) exclude(may[t][u], s[t][u]);
+          for (int t = 0; t < MT; ++t) exclude(moved<EDGE>(may[t][u], t0 + kc + 16 * u + 4 * g, a.S), s[t][u]);
         }
       }
       typename M::TF kt[M::ND];                                 // in flight behind the exponentials
@@ -234,14 +234,22 @@ struct GkvCfg {
   static constexpr int RED_ROW = DP + 4;
   static constexpr int LDS = GQ ? RED_AT + 4 * BR * RED_ROW * 4 : K_AT;
   static constexpr int NP = (BR * M::PPR + 255) / 256;
+  // behind them, with a (query, key) mask: a bit per row and key, 16 keys of a row in a word, the words of a key tile's rows side by side.
+  // A thread loads 16 keys of a row at a time, with the rows' next tile (7 x 197 x 1062 x 32 heads of 24, bf16: 88 us; every lane
+  // its own bytes from the lines of four rows, two key tiles each: 111)
+  static constexpr int CELLS = (BR * 4 * NT + 255) / 256, MASK = 2 * BR * 4 * NT, DROP = 4 * BR;   // DROP: the rows' dropout hashes
   // P of a normalised row is about 1 / S: in float16 it is scaled by 2^14 (the largest power of two whose product with 1 is finite
   // with room to spare) so that probabilities down to 2^-28 keep their 11 bits; exact to undo
   // Score gradients are rounded as they are: they follow grad_out's size, which a loss scale sets, down to float16's 2^-25 absolute
   static constexpr float P_SCALE = TY == DI_F16 ? 16384.f : 1.f, P_LOG2 = TY == DI_F16 ? 14.f : 0.f;
 };
 
+struct __attribute__((packed)) MaskCell {
+  u4 v;
+};
+
 template <int TY, int DP, int NT, bool GQ, bool FULL>
-__global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attention_gkv_kernel(Args a) {
+__global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY != DI_F32 && FULL ? 2 : 1) void attention_gkv_kernel(Args a) {
   using C = GkvCfg<TY, DP, NT, GQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
@@ -261,6 +269,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
   constexpr int STEP = 256 / M::PPR;
   u4 qs[C::NP], gs[C::NP], os[C::NP];                           // os: GQ forms delta from the forward's output
   float ls = INFINITY, de = 0.f;
+  u4 cells[C::CELLS];                                           // the mask of one row and 16 keys each
   bool empty[C::NP];                                            // (query, key) mask: rows that it leaves without keys become zeros, so that
                                                                 // what they hold - a NaN - meets no product over the rows
   const int piece = tid % M::PPR, first = tid / M::PPR;
@@ -300,6 +309,20 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
     }
     if (FULL && a.allowed != nullptr) {
 #pragma unroll
+      for (int j = 0; j < C::CELLS; ++j) {
+        const int e = tid + 256 * j, r = min(t0 + e / (4 * NT), rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(r);
+        const int at_key = key0 + 16 * (e % (4 * NT));
+        const unsigned char *line = a.allowed + at.b * a.allowed_bs + (r - head * a.L) * a.allowed_rs;
+        cells[j] = u4{0, 0, 0, 0};
+        if (C::CELLS * 256 > C::BR * 4 * NT && e >= C::BR * 4 * NT) continue;
+        if (a.S >= 16) {                                        // the row's last 16 keys: moved up when they become bits
+          cells[j] = reinterpret_cast<const MaskCell *>(line + min(at_key, a.S - 16))->v;
+        } else {                                                // (a single key block: the other key tiles' keys are not there)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) cells[j][k] = look<true>(line, 4 * k, a.S);
+        }
+      }
+#pragma unroll
       for (int j = 0; j < C::NP; ++j) {
         const int r = t0 + first + j * STEP;
         empty[j] = r < r1 && a.lse[row_id + r] == -INFINITY;
@@ -312,22 +335,6 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
     }
   };
   if (r0 < r1) fetch(r0);
-
-  // the (query, key) mask of a chunk's rows: with up to 32 keys a wavefront one chunk ahead of its use (rows clamped into the matrix),
-  // with more - registers - in front of the products
-  constexpr bool MASK_AHEAD = NT <= 2;
-  unsigned char may[M::NT][NT][4];
-  auto look = [&](int row0) {
-#pragma unroll
-    for (int u = 0; u < M::NT; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int rr = min(row0 + 16 * u + 4 * g + r, rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(rr);
-        const unsigned char *line = a.allowed + at.b * a.allowed_bs + (rr - head * a.L) * a.allowed_rs;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) may[u][n][r] = line[min(key0 + (wave * NT + n) * 16 + i, a.S - 1)];
-      }
-  };
 
   typename M::RF kf[NT][M::NK], vf[NT][M::NK];
   f4 gk[NT][M::ND], gv[NT][M::ND];
@@ -370,22 +377,56 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
         }
       }
     }
+    if (FULL && a.allowed != nullptr) {
+#pragma unroll
+      for (int j = 0; j < C::CELLS; ++j) {
+        const int e = tid + 256 * j;
+        unsigned bits = 0;
+        if (a.S < 16) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) cells[j][k] = moved<true>(cells[j][k], 4 * k, a.S);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                           // bytes != 0 -> their top bits -> four adjacent bits (no two of the product's terms meet)
+          const unsigned w = cells[j][k], top = (((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) & 0x80808080u;
+          bits |= ((top >> 7) * 0x01020408u >> 24 & 0xfu) << (4 * k);
+        }
+        if (C::CELLS * 256 > C::BR * 4 * NT && e >= C::BR * 4 * NT) continue;
+        const int at_key = key0 + 16 * (e % (4 * NT)), up = a.S >= 16 ? min(max(at_key - (a.S - 16), 0), 16) : 0;
+        *reinterpret_cast<unsigned short *>(lds + C::LDS + 2 * ((e % (4 * NT)) * C::BR + e / (4 * NT))) = (unsigned short)(bits >> up);
+      }
+    }
     if (tid < C::BR) {
       slse[tid] = ls == -INFINITY ? INFINITY : ls - C::P_LOG2;
       if (!GQ) sdelta[tid] = de * (1.f / C::P_SCALE);
+      if (FULL && a.drop) *reinterpret_cast<unsigned *>(lds + C::LDS + C::MASK + 4 * tid) = drop_row(seed, row_id + t0 + tid);
     }
     __syncthreads();
     if (t0 + C::BR < r1) fetch(t0 + C::BR);
 #pragma unroll 1
     for (int rc = 0; rc < C::BR; rc += M::CH) {
       if (t0 + rc >= r1 || (GQ && wave >= waves)) break;
-      if (FULL && a.allowed != nullptr && (!MASK_AHEAD || (t0 == r0 && rc == 0))) look(t0 + rc);
       typename M::PF pf[NT], df[NT];
       typename M::TF gt_[M::ND];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
-        const int rfirst = t0 + rc + 16 * u + 4 * g;
         f4 s[NT], dp[NT];
+        unsigned keep[NT];                                      // dropout: bit 4 r = row 4 g + r keeps the lane's key
+        if (FULL && a.drop) {
+          // four lanes share four keys: lane j of them hashes row 4 g + j's four numbers, the four rows' decisions are put together (2 x 200 x
+          // 32 400 x 8 heads of 16, half precision: 166 us; every lane its four rows' numbers, 236; without dropout 66)
+          const unsigned dr = *reinterpret_cast<const unsigned *>(lds + C::LDS + C::MASK + 4 * (rc + 16 * u + 4 * g + (i & 3)));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const unsigned k4 = (unsigned)key[n] >> 2, x = drop_pair(dr, k4, false), y = drop_pair(dr, k4, true);
+            unsigned w = ((x & 0xffffu) >= a.drop ? 1u : 0u) | ((x >> 16) >= a.drop ? 2u : 0u) | ((y & 0xffffu) >= a.drop ? 4u : 0u) |
+                         ((y >> 16) >= a.drop ? 8u : 0u);
+            w <<= 4 * (i & 3);
+            w |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)w, 0xb1, 0xf, 0xf, true);       // lanes 1 0 3 2
+            w |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)w, 0x4e, 0xf, 0xf, true);       // lanes 2 3 0 1
+            keep[n] = w >> (i & 3);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n] = dp[n] = f4{0.f, 0.f, 0.f, 0.f};
         typename M::RF qf[M::NK], gf[M::NK];                    // the tile's fragments before its first product
@@ -410,9 +451,10 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if (FULL && a.allowed != nullptr) {
+          if (FULL && a.allowed != nullptr) {                   // bit i of the words of rows 4 g .. + 3
+            const u2 may = *reinterpret_cast<const u2 *>(lds + C::LDS + 2 * ((wave * NT + n) * C::BR + rc + 16 * u + 4 * g));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[n][r] = may[u][n][r] != 0 ? s[n][r] : -INFINITY;
+            for (int r = 0; r < 4; ++r) s[n][r] = (may[r >> 1] >> (16 * (r & 1) + i) & 1u) != 0 ? s[n][r] : -INFINITY;
           }
           f4 p, ds;
 #pragma unroll
@@ -421,8 +463,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
             // pr = P_SCALE p, ds = pr ((dp - delta) / P_SCALE): the scale sits in the rows' two numbers
             const float pr = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale2, -l4[r]));
             if (FULL && a.drop) {
-              const unsigned x = drop_pair(drop_row(seed, row_id + rfirst + r), (unsigned)key[n] >> 2, (key[n] & 2) != 0);
-              const bool kept = ((key[n] & 1) ? x >> 16 : x & 0xffffu) >= a.drop;
+              const bool kept = (keep[n] >> (4 * r) & 1u) != 0;
               p[r] = kept ? pr : 0.f;                        // the kept ones' scale: at the end
               dp[n][r] = kept ? dp[n][r] * a.keep_scale : 0.f;
             } else {
@@ -438,7 +479,6 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : 1) void attentio
           M::pack(df[n], u, ds);
         }
       }
-      if (FULL && MASK_AHEAD && a.allowed != nullptr) look(t0 + rc + M::CH);
       auto by_rows = [&]() {                                    // gv^T += go^T P, gk^T += Q^T dS
 #pragma unroll
         for (int d = 0; d < M::ND; ++d) {

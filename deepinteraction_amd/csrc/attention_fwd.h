@@ -91,15 +91,25 @@ struct KeyStage {
 // a score.  A NaN score loses the comparison but stays a NaN in the exponential.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 
-// 4 keys x 1 row of the (row, key) mask as the bytes of a word; keys past the end count as allowed (their scores are excluded by the
-// bias).  `words`: rows start on 4 bytes, and key is a multiple of 4.  A row that is not there reads the last one's mask.
-__device__ __forceinline__ unsigned look(const unsigned char *row, int key, int S, bool words) {
-  if (words && key + 4 <= S) return *reinterpret_cast<const unsigned *>(row + key);
-  unsigned w = 0x01010101u;
+// 4 keys x 1 row of the (row, key) mask as the bytes of a word, one load wherever the row starts (53 x 721 x 651, 4 heads of 32, forward:
+// four byte loads 430 us, one of a word 96).  EDGE: keys may lie behind the row's end - its last word is taken, which `exclude` moves up
+// once it has arrived; what it then holds for those keys does not matter, they are excluded anyway.  A row that is not there reads the
+// last one's mask.
+struct __attribute__((packed)) MaskWord {
+  unsigned w;
+};
+template <bool EDGE>
+__device__ __forceinline__ unsigned look(const unsigned char *row, int key, int S) {
+  if (!EDGE) return reinterpret_cast<const MaskWord *>(row + key)->w;
+  if (S >= 4) return reinterpret_cast<const MaskWord *>(row + min(key, S - 4))->w;
+  unsigned w = 0;
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (key + r < S && row[key + r] == 0) w &= ~(0xffu << (8 * r));
+  for (int r = 0; r < 4; ++r) w |= (unsigned)row[min(key + r, S - 1)] << (8 * r);
   return w;
+}
+template <bool EDGE>
+__device__ __forceinline__ unsigned moved(unsigned w, int key, int S) {
+  return EDGE && S >= 4 ? w >> (8 * min(max(key - (S - 4), 0), 3)) : w;
 }
 __device__ __forceinline__ void exclude(unsigned w, f4 &s) {
 #pragma unroll
@@ -109,7 +119,7 @@ __device__ __forceinline__ void exclude(unsigned w, f4 &s) {
 
 // FULL: with a key mask, a (query, key) mask or dropout; without them only the last tile of a range is tested key by key
 template <int TY, int DP, int MT, int WQ, bool FULL>
-__global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) void attention_fwd_kernel(Args a) {
+__global__ __launch_bounds__(256, (DP == 128 && TY != DI_F32) || (DP == 32 && FULL) ? 2 : 1) void attention_fwd_kernel(Args a) {
   using C = FwdCfg<TY, DP, MT, WQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
@@ -161,7 +171,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
         for (int t = 0; t < N; ++t)
 #pragma unroll
           for (int u = 0; u < M::NT; ++u)
-            may[t][u] = look(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S, a.allowed_words);
+            may[t][u] = look<EDGE>(a.allowed + at.b * a.allowed_bs + query[t] * a.allowed_rs, t0 + kc + 16 * u + 4 * g, a.S);
       }
       typename M::RF kf[M::NT][M::NK];                          // all of the chunk's before its first product: one wait, not one each
 #pragma unroll
@@ -187,7 +197,7 @@ __global__ __launch_bounds__(256, DP == 128 && TY != DI_F32 && !FULL ? 2 : 1) vo
         }
         if (FULL && a.allowed != nullptr) {
 #pragma unroll
-          for (int t = 0; t < N; ++t) exclude(may[t][u], s[t][u]);
+          for (int t = 0; t < N; ++t) exclude(moved<EDGE>(may[t][u], t0 + kc + 16 * u + 4 * g, a.S), s[t][u]);
         }
       }
       float mx[MT];

@@ -49,10 +49,12 @@ static int gkv(const Args &a, hipStream_t s) {
   static LdsRaised plain, full;
   const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
   constexpr bool GQ = one_launch(DP);
-  constexpr int lds = GkvCfg<TY, DP, NT, GQ>::LDS;
-  static_assert(GkvCfg<TY, DP, NT, GQ>::BR == tile_rows(TY, DP), "the plan's tiles");
-  return needs_full(a) ? go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, lds, grid, a, s, "attention_gkv")
-                       : go(attention_gkv_kernel<TY, DP, NT, GQ, false>, plain, lds, grid, a, s, "attention_gkv");
+  using C = GkvCfg<TY, DP, NT, GQ>;
+  static_assert(C::BR == tile_rows(TY, DP) && C::LDS % 16 == 0, "the plan's tiles; the mask's words");
+  if constexpr (NT <= most_masked_key_tiles) {
+    if (needs_full(a)) return go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, C::LDS + C::MASK + C::DROP, grid, a, s, "attention_gkv");
+  }
+  return go(attention_gkv_kernel<TY, DP, NT, GQ, false>, plain, C::LDS, grid, a, s, "attention_gkv");
 }
 
 // walk: the keys per range (row blocks) or per block (key blocks)

@@ -175,6 +175,24 @@ def test_excluded_keys_may_hold_anything(t, L, S, D):
     assert not got[3][dead].any() and not got[4][dead].any()
 
 
+@pytest.mark.parametrize('D', [16, 24, 64, 128])
+@pytest.mark.parametrize('S', [1, 2, 3, 4, 5, 13, 15, 16, 17, 31, 64, 65, 131, 258, 519])
+def test_mask_rows_that_start_and_end_anywhere(S, D):
+    """(query, key) masks of every width, at odd addresses, of bytes other than 0 and 1, with rows apart or shared."""
+    B, L, H, Hk = 2, 21, 4, 2
+    for t in (F32, F16):
+        q, k, v, go = make(B, L, S, H, Hk, D, t)
+        for lead, rs in ((0, S), (1, S), (3, S + 7)):
+            store = (torch.rand(lead + B * L * rs, device='cuda') < 0.5).to(torch.uint8) * 6
+            allowed = store[lead:].as_strided((B, L, S), (L * rs, rs, 1), lead)
+            check(q, k, v, go, H, allowed != 0, allowed=allowed)
+        lengths = torch.tensor([S, S // 2], dtype=torch.int32, device='cuda')
+        keep = (allowed != 0) & (torch.arange(S, device='cuda') < lengths[:, None, None])
+        check(q, k, v, go, H, keep, allowed=allowed, key_lengths=lengths)
+        shared = allowed[:1, :1].expand(B, L, S)
+        check(q, k, v, go, H, shared != 0, allowed=shared)
+
+
 @pytest.mark.parametrize('t', TYPES, ids=str)
 @pytest.mark.parametrize('L,S,D', [(1, 300, 16), (70, 300, 16), (200, 40, 32), (40, 130, 64), (150, 200, 128), (5, 700, 128)])
 def test_queries_without_keys_may_hold_anything(t, L, S, D):
