@@ -8,14 +8,16 @@
 namespace di {
 namespace at {
 
-// Blocks, and - where they are fewer than `want` - ranges of the walked side (whole tiles, at least `least` of them) so that about
-// `want` workgroups run.
-static void cut(Plan &p, long long problems, int rows, int per_block, int walked, int tile, int least, long long want) {
+// Blocks, and - where they are fewer than `want` - ranges of the walked side (whole tiles) so that about `want` workgroups run: at
+// least `least` tiles each, or up to `some` ranges whatever their length.
+static void cut(Plan &p, long long problems, int rows, int per_block, int walked, int tile, int least, int some, long long want) {
   p.blocks = (rows + per_block - 1) / per_block;
   const long long n = problems * (p.blocks > 0 ? p.blocks : 1);
   const int tiles = walked > 0 ? (int)(((long long)walked + tile - 1) / tile) : 1;
+  int most = tiles / least;
+  if (most < some) most = some < tiles ? some : tiles;
   long long splits = n > 0 ? want / n : 1;
-  if (splits > tiles / least) splits = tiles / least;
+  if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   const int per = (int)((tiles + splits - 1) / splits);
   p.range = per > 0x7fffffff / tile ? 0x7fffffff : per * tile;
@@ -27,7 +29,10 @@ static void cut(Plan &p, long long problems, int rows, int per_block, int walked
 // resident - two workgroups a CU, one for gq of 128 dims (2048 x 8192 x 16 heads of 128, forward: 1 a CU 263 us, 2 211, 3 229; gq: 1 a
 // CU 290, 2 317) - and twice that where the samples' lengths differ and some ranges have no keys (4 x 511 x 4100, 2733, 1366, 0, four
 // heads of 64 to a key head, forward + gq with their joins: 2 a CU 127 us, 4 95, 6 100, 8 118; four lengths of 1025 .. 4100: 132, 113,
-// 119, 128).  Too few row blocks for the CUs: 64 rows a workgroup.
+// 119, 128).  Too few row blocks for the CUs, and gq of 128 dims with a mask or dropout (426 x 375 x 127, 8 heads, key mask: 128 rows,
+// one a CU, 637 us; 64, two a CU, 554): 64 rows a workgroup, and - heads of up to 32 dims, of which more are resident - eight a CU
+// (57 x 20 rows x 19 070, four heads of 24: 564 -> 442; heads of 128 lose, 150 -> 170).  A tile of float32 keys takes 3 - 7 us with 64 and
+// 128 dims: up to 16 ranges of single tiles (300 x 300, 8 heads of 64, forward 16.6 -> 7.4 + 4.9 us for the join; 23 x 598 of 128: 34 -> 10 + 5).
 // Key lengths: the samples of an unbalanced batch load the XCDs evenly (where_ragged in attention.h) - if there is more than one workgroup
 // a CU to place, and no more samples than lanes to look them up.
 static bool ragged(const di_attention &t, const Plan &p, int cus) {
@@ -41,16 +46,18 @@ static int plan_rows(const di_attention &t, bool forward, Plan &p) {
   const long long problems = (long long)t.B * t.kv_heads;
   if (rows <= 16) {
     p.big = 0;
-    cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, 24ll * cus);
+    cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, 1, 24ll * cus);
     p.ragged = ragged(t, p, cus);
     return DI_OK;
   }
-  const long long want = (forward || DP < 128 ? 2ll : 1ll) * cus * (t.key_lengths != nullptr ? 2 : 1);
+  const bool wide = !forward && DP == 128, full = t.key_mask != nullptr || t.allowed != nullptr || t.dropout_p > 0.f;
+  const long long want = 2ll * cus * (t.key_lengths != nullptr ? 2 : 1);
+  const int some = t.dtype == DI_F32 && DP >= 64 ? 16 : 1;
   p.big = 2;
-  cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, want);
-  if (rows <= 64 || problems * p.blocks * p.splits < cus) {
+  cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, some, wide ? want / 2 : want);
+  if (rows <= 64 || (wide && full) || problems * p.blocks * p.splits < cus) {
     p.big = 1;
-    cut(p, problems, rows, 64, t.S, 64, 4, want);
+    cut(p, problems, rows, 64, t.S, 64, 4, some, DP <= 32 ? 4 * want : want);
   }
   p.ragged = ragged(t, p, cus);
   return DI_OK;
@@ -63,15 +70,15 @@ static int plan_keys(const di_attention &t, Plan &p) {
   const int tile = tile_rows(t.dtype, DP);
   const long long problems = (long long)t.B * t.kv_heads;
   const int S = t.S > 0 ? t.S : 1;                              // without keys, one block still writes gq's zeros
-  const bool full = t.key_mask != nullptr || t.allowed != nullptr || t.dropout_p > 0.f;
+  const bool full = t.allowed != nullptr || t.dropout_p > 0.f;
   p.big = key_tiles(t.dtype, DP);
   if (full && p.big > most_masked_key_tiles) p.big = most_masked_key_tiles;
   for (; p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
     if (32 * p.big >= t.S) continue;
-    cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
+    cut(p, problems, S, 64 * p.big, rows, tile, 1, 1, 2ll * cus);
     if (problems * p.blocks * p.splits >= cus) break;
   }
-  if (p.big <= least) cut(p, problems, S, 64 * p.big, rows, tile, 1, 2ll * cus);
+  if (p.big <= least) cut(p, problems, S, 64 * p.big, rows, tile, 1, 1, 2ll * cus);
   p.ragged = ragged(t, p, cus);
   return DI_OK;
 }

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
   auto step = [&](auto edge, int t0) {
     __syncthreads();
-    st.template commit<true, false>(lds, C::V_AT);
+    st.template commit<true, false>(lds, C::V_AT, km != nullptr);
     if (decltype(edge)::value && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
       bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;
@@ -248,6 +248,7 @@ struct __attribute__((packed)) MaskCell {
   u4 v;
 };
 
+// FULL: with a (query, key) mask or dropout
 template <int TY, int DP, int NT, bool GQ, bool FULL>
 __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY != DI_F32 && FULL ? 2 : 1) void attention_gkv_kernel(Args a) {
   using C = GkvCfg<TY, DP, NT, GQ>;
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
   const int key0 = at.blk * C::KEYS;
   // a block without keys: zeros (the only block: gq's zeros, too)
   const int r0 = at.sp * a.range, r1 = key0 < nkeys || (GQ && a.blocks == 1) ? min(r0 + a.range, rows) : r0;
-  const bool whole = key0 + C::KEYS <= nkeys && (!FULL || a.kmask == nullptr);
+  const bool whole = key0 + C::KEYS <= nkeys && a.kmask == nullptr;
   const int waves = min(4, max(1, (nkeys - key0 + 16 * NT - 1) / (16 * NT)));             // wavefronts with keys
   const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     key[n] = key0 + (wave * NT + n) * 16 + i;
-    valid[n] = key[n] < nkeys && (!FULL || a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
+    valid[n] = key[n] < nkeys && (a.kmask == nullptr || a.kmask[at.b * a.kmask_bs + key[n]] != 0);
 #pragma unroll
     for (int kk = 0; kk < M::NK; ++kk) {
       kf[n][kk] = M::row_frag_of(kb + key[n] * a.k_rs, kk, g, a.D, valid[n]);

@@ -39,6 +39,7 @@ struct KeyStage {
   using M = typename C::M;
   static constexpr int STEP = 256 / M::PPR;                     // rows per piece index j
   u4 k[C::NP], v[C::NP];
+  unsigned char part[C::NP];                                    // with a key mask: whether the key takes part
   unsigned ko, vo;
   int key;
   bool in;                                                      // the piece lies within the head dim (and the tile)
@@ -65,7 +66,8 @@ struct KeyStage {
       for (int j = 0; j < C::NP; ++j) {
         const int s = t0 + key + j * STEP;
         k[j] = v[j] = u4{0, 0, 0, 0};
-        if (in && s < k1 && (km == nullptr || km[s] != 0)) {
+        if (km != nullptr) part[j] = km[min(s, k1 - 1)];
+        if (in && s < k1) {                                     // (masked keys are loaded, too: the loads do not wait for the mask)
           k[j] = *reinterpret_cast<const u4 *>(kt + j * STEP * a.k_rs + ko);
           v[j] = *reinterpret_cast<const u4 *>(vt + j * STEP * a.v_rs + vo);
         }
@@ -74,12 +76,13 @@ struct KeyStage {
   }
   // KX / VX: the tile of K / V is a TRS tile
   template <bool KX, bool VX>
-  __device__ __forceinline__ void commit(char *lds, int v_at) {
+  __device__ __forceinline__ void commit(char *lds, int v_at, bool masked) {
     const int p = threadIdx.x % M::PPR;
     if (C::TILE >= STEP || key < C::TILE) {
 #pragma unroll
       for (int j = 0; j < C::NP; ++j) {
         const int row = key + j * STEP, x = M::x(row);
+        if (masked && part[j] == 0) k[j] = v[j] = u4{0, 0, 0, 0};
         *reinterpret_cast<u4 *>(lds + row * (KX ? M::TRS : M::ROWS) + ((p * 16) ^ (KX ? x : 0))) = k[j];
         *reinterpret_cast<u4 *>(lds + v_at + row * (VX ? M::TRS : M::ROWS) + ((p * 16) ^ (VX ? x : 0))) = v[j];
       }
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(256, (DP == 128 && TY != DI_F32) || (DP == 32 && FU
   if (k0 < k1) st.fetch(a, kb, vb, km, k0, k1);
   auto step = [&](auto edge, int t0) {
     __syncthreads();                                            // the last tile's reads are done
-    st.template commit<false, true>(lds, C::V_AT);
+    st.template commit<false, true>(lds, C::V_AT, km != nullptr);
     if (decltype(edge)::value && threadIdx.x < C::TILE) {
       const int s = t0 + threadIdx.x;
       bias[threadIdx.x] = s < k1 && (km == nullptr || km[s] != 0) ? 0.f : -INFINITY;

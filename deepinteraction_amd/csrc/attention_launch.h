@@ -41,8 +41,12 @@ static int gq(const Args &a, hipStream_t s) {
   static LdsRaised plain, full;
   const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
   constexpr int lds = GqCfg<TY, DP, MT, WQ>::LDS;
-  return needs_full(a) ? go(attention_gq_kernel<TY, DP, MT, WQ, true>, full, lds, grid, a, s, "attention_gq")
-                       : go(attention_gq_kernel<TY, DP, MT, WQ, false>, plain, lds, grid, a, s, "attention_gq");
+  if constexpr (DP == 128 && MT > 1) {                          // the plan's: 64 rows with masks and dropout
+    return go(attention_gq_kernel<TY, DP, MT, WQ, false>, plain, lds, grid, a, s, "attention_gq");
+  } else {
+    return needs_full(a) ? go(attention_gq_kernel<TY, DP, MT, WQ, true>, full, lds, grid, a, s, "attention_gq")
+                         : go(attention_gq_kernel<TY, DP, MT, WQ, false>, plain, lds, grid, a, s, "attention_gq");
+  }
 }
 template <int TY, int DP, int NT>
 static int gkv(const Args &a, hipStream_t s) {
@@ -52,7 +56,7 @@ static int gkv(const Args &a, hipStream_t s) {
   using C = GkvCfg<TY, DP, NT, GQ>;
   static_assert(C::BR == tile_rows(TY, DP) && C::LDS % 16 == 0, "the plan's tiles; the mask's words");
   if constexpr (NT <= most_masked_key_tiles) {
-    if (needs_full(a)) return go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, C::LDS + C::MASK + C::DROP, grid, a, s, "attention_gkv");
+    if (a.allowed != nullptr || a.drop != 0) return go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, C::LDS + C::MASK + C::DROP, grid, a, s, "attention_gkv");
   }
   return go(attention_gkv_kernel<TY, DP, NT, GQ, false>, plain, C::LDS, grid, a, s, "attention_gkv");
 }

@@ -22,7 +22,7 @@ constexpr bool one_launch(int DP) { return DP <= 32; }                          
 // Key tiles per wavefront at the most.  Heads of 128: one, two wavefronts a SIMD (2048 x 8192 x 16 heads, bf16: 380 us; two tiles, whose
 // sums leave room for one: 394).  Heads of 64: two (161 us; one: 189)
 constexpr int key_tiles(int TY, int DP) { return DP == 16 ? 4 : DP == 32 ? (TY == DI_F32 ? 2 : 4) : DP == 64 ? 2 : 1; }
-// With a mask or dropout two at the most: their words and hashes take the registers of the second wavefront a SIMD (half precision, with four
+// With a (query, key) mask or dropout two at the most: their words and hashes take the registers of the second wavefront a SIMD (half precision, with four
 // and with two: 2 x 200 x 32 400 x 8 heads of 16 and dropout 228 and 183 us with the join, 53 x 721 x 651 x 4 heads of 32 and a (query, key)
 // mask 322 and 241)
 constexpr int most_masked_key_tiles = 2;
