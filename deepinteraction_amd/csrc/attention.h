@@ -35,7 +35,7 @@ constexpr float kLowest = -3.4028234663852886e38f;
 __device__ __forceinline__ short to_half_bits(float x) { return __builtin_bit_cast(short, (_Float16)x); }
 __device__ __forceinline__ short to_bf_bits(float x) { return __builtin_bit_cast(short, (__bf16)x); }
 
-// TY: DI_F32 / DI_F16 / DI_BF16; DP: the head dim padded to 16, 32, 64 or 128
+// TY: DI_F32 / DI_F16 / DI_BF16; DP: the head dim padded to 16, 32, 64, 96 or 128
 template <int TY, int DP>
 struct Mm {
   static constexpr bool WIDE = TY == DI_F32;
@@ -43,7 +43,7 @@ struct Mm {
   static constexpr int KD = WIDE || DP == 16 ? 16 : 32;         // head dims per row fragment
   static constexpr int NK = DP / KD, ND = DP / 16;
   static constexpr int CH = WIDE ? 16 : 32, NT = CH / 16;       // rows (keys / queries) per contraction over rows
-  static constexpr int PPR = DP * SZ / 16;                      // 16-byte pieces of a tile row
+  static constexpr int PPR = (DP == 96 ? 128 : DP) * SZ / 16;   // threads that stage a tile row's 16-byte pieces (a power of two)
   // tile row strides in bytes.  ROWS (read in rows only): + 16 keeps the fragments of 16 rows in different banks.  TRS (read transposed,
   // or both ways): float32 the same; 16-bit + 32, the stride that spreads the transposing reads of 8 rows over all banks.  Head dim 16 (no
   // padding): the two 16-byte pieces of every other 8 rows are exchanged (`x` on their offsets), which does the same for the 8-byte row
@@ -62,6 +62,7 @@ struct Mm {
 
   static __device__ __forceinline__ int x(int row) { return WIDE || DP != 16 ? 0 : (row & 8) << 1; }
 
+  static __device__ __forceinline__ bool whole(int piece) { return DP != 96 || piece * 16 < DP * SZ; }   // the tile row has the piece
   static __device__ __forceinline__ int d0(int kk, int g) { return KD * kk + (WIDE || DP == 16 ? 4 : 8) * g; }
   static __device__ __forceinline__ RF row_frag(const char *row, int kk, int g) {
     RF f;

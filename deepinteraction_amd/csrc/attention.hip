@@ -29,8 +29,8 @@ static void cut(Plan &p, long long problems, int rows, int per_block, int walked
 // resident - two workgroups a CU, one for gq of 128 dims (2048 x 8192 x 16 heads of 128, forward: 1 a CU 263 us, 2 211, 3 229; gq: 1 a
 // CU 290, 2 317) - and twice that where the samples' lengths differ and some ranges have no keys (4 x 511 x 4100, 2733, 1366, 0, four
 // heads of 64 to a key head, forward + gq with their joins: 2 a CU 127 us, 4 95, 6 100, 8 118; four lengths of 1025 .. 4100: 132, 113,
-// 119, 128).  Too few row blocks for the CUs, and gq of 128 dims with a mask or dropout (426 x 375 x 127, 8 heads, key mask: 128 rows,
-// one a CU, 637 us; 64, two a CU, 554): 64 rows a workgroup, and - heads of up to 32 dims, of which more are resident - eight a CU
+// 119, 128).  Too few row blocks for the CUs, and 16-bit gq of 96 and 128 dims with a mask or dropout (426 x 375 x 127, 8 heads, key mask: 128 rows,
+// one a CU, 637 us; 64, two a CU, 554; 2 x 1000 x 4000, 8 heads of 72: 108 and 90; float32 loses, 347 and 416): 64 rows a workgroup, and - heads of up to 32 dims, of which more are resident - eight a CU
 // (57 x 20 rows x 19 070, four heads of 24: 564 -> 442; heads of 128 lose, 150 -> 170).  A tile of float32 keys takes 3 - 7 us with 64 and
 // 128 dims: up to 16 ranges of single tiles (300 x 300, 8 heads of 64, forward 16.6 -> 7.4 + 4.9 us for the join; 23 x 598 of 128: 34 -> 10 + 5).
 // Key lengths: the samples of an unbalanced batch load the XCDs evenly (where_ragged in attention.h) - if there is more than one workgroup
@@ -55,7 +55,7 @@ static int plan_rows(const di_attention &t, bool forward, Plan &p) {
   const int some = t.dtype == DI_F32 && DP >= 64 ? 16 : 1;
   p.big = 2;
   cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, some, wide ? want / 2 : want);
-  if (rows <= 64 || (wide && full) || problems * p.blocks * p.splits < cus) {
+  if (rows <= 64 || (!forward && DP >= 96 && full && t.dtype != DI_F32) || problems * p.blocks * p.splits < cus) {
     p.big = 1;
     cut(p, problems, rows, 64, t.S, 64, 4, some, DP <= 32 ? 4 * want : want);
   }

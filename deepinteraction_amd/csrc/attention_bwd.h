@@ -13,6 +13,17 @@
 // transposed through LDS, the four shares added per tile of rows, the key blocks' sums joined by the forward's second launch.  The
 // scores are formed once, and rows of few dims make the key blocks' sums small (rows x D floats per 128 - 256 keys); wide heads would
 // write more sums than the second pass over the keys costs.
+//
+// What bounds them, and what they measured:
+//   heads of 128 (2048 x 8192 x 16, bf16): gq 252 us = 818 TFLOP/s, the matrix cores; gk and gv 350 - 380 us = 720 - 790: a SIMD's two
+//     wavefronts hold 16 keys each, so every fragment of Q and go from LDS feeds one product (the fragments take half of LDS's cycles),
+//     and a quarter of the cycles waits for them and at the tiles' barriers
+//   heads of 64, four to a key head (4 x 511 x 4100, 2733, 1366, 0, bf16): gq 46 us, gk and gv 78: 264 workgroups for 256 CUs, one
+//     wavefront a SIMD - its own chain of product, exponential, product is the time of a tile
+//   heads of 16, one launch (200 x 32 400 x 8, float32: 100 us; half precision 2 samples: 66 us; 1200 x 60 x 112: 77 us): the vector unit
+//     (ten instructions and an exponential a pair), in float32 the matrix cores beside it
+// Not taken: the products over a chunk's rows left for the next chunk, to hide behind its exponentials - the registers that this takes
+// cost the second wavefront of the SIMD (4 x 511 x .. of 64: 79 -> 110 us; heads of 128: 410 -> 433).
 #pragma once
 #include "attention_fwd.h"
 
@@ -368,8 +379,10 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
       for (int j = 0; j < C::NP; ++j) {
         if (FULL && a.allowed != nullptr && empty[j]) qs[j] = gs[j] = os[j] = u4{0, 0, 0, 0};
         const int at_row = (first + j * STEP) * M::TRS + ((piece * 16) ^ M::x(first + j * STEP));
-        *reinterpret_cast<u4 *>(lds + at_row) = qs[j];
-        *reinterpret_cast<u4 *>(lds + C::G_AT + at_row) = gs[j];
+        if (M::whole(piece)) {
+          *reinterpret_cast<u4 *>(lds + at_row) = qs[j];
+          *reinterpret_cast<u4 *>(lds + C::G_AT + at_row) = gs[j];
+        }
         if (GQ) {
           float d = M::widen_dot({gs[j]}, {os[j]});
 #pragma unroll

@@ -10,6 +10,15 @@
 // The maximum is corrected only when a score exceeds it by more than 8 (a factor of 256 in exp2's argument, harmless in float32 and
 // in the 16-bit probabilities): the test is one comparison per tile against the lane's own scores, the exchange between lanes and
 // the correction of the sums run when any lane asks for them - a few times per row, not once per tile.
+//
+// What bounds it, and what it measured:
+//   heads of 128 and 64 (2048 x 8192 x 16 heads of 128, bf16: 172 us = 800 TFLOP/s, a large matrix product reaches 1085 on this card):
+//     the matrix cores, then the exponentials of the same wavefronts - both units have their own work, two wavefronts a SIMD share them
+//   heads of 16 (200 x 32 400 x 8, float32: 49 us = 68 TFLOP/s of 149, half precision 2 samples 37 us): a pair of row and key costs 32
+//     multiply-adds and an exponential, so the vector unit (5 instructions and the exponential a score) and, in float32, the matrix cores
+//     in turn.  Writing float32 operands as three bf16 parts would take the products to the 16-bit rate and put the splitting of every
+//     probability, six instructions, on the vector unit: no gain
+//   single queries (16 samples of up to 32 768 keys x 8 key heads of 128, 1.07 GB): the memory, 190 us = 5.6 TB/s
 #pragma once
 #include <type_traits>
 
@@ -83,6 +92,7 @@ struct KeyStage {
       for (int j = 0; j < C::NP; ++j) {
         const int row = key + j * STEP, x = M::x(row);
         if (masked && part[j] == 0) k[j] = v[j] = u4{0, 0, 0, 0};
+        if (!M::whole(p)) continue;
         *reinterpret_cast<u4 *>(lds + row * (KX ? M::TRS : M::ROWS) + ((p * 16) ^ (KX ? x : 0))) = k[j];
         *reinterpret_cast<u4 *>(lds + v_at + row * (VX ? M::TRS : M::ROWS) + ((p * 16) ^ (VX ? x : 0))) = v[j];
       }
@@ -122,7 +132,7 @@ __device__ __forceinline__ void exclude(unsigned w, f4 &s) {
 
 // FULL: with a key mask, a (query, key) mask or dropout; without them only the last tile of a range is tested key by key
 template <int TY, int DP, int MT, int WQ, bool FULL>
-__global__ __launch_bounds__(256, (DP == 128 && TY != DI_F32) || (DP == 32 && FULL) ? 2 : 1) void attention_fwd_kernel(Args a) {
+__global__ __launch_bounds__(256, (DP >= 96 && TY != DI_F32) || (DP == 32 && FULL) ? 2 : 1) void attention_fwd_kernel(Args a) {
   using C = FwdCfg<TY, DP, MT, WQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];

@@ -19,7 +19,7 @@ static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &
 template <int TY, bool STATS>
 static int join(const Args &args, hipStream_t s) {
   Args a = args;
-  const int nd = padded(a.D) / 4;                               // lanes across the head dim
+  const int nd = (padded(a.D) == 96 ? 128 : padded(a.D)) / 4;    // lanes across the head dim: a power of two
   int group = nd;
   while (group < 64 && 4 * (group / nd) < a.splits) group *= 2;
   const int per = 256 / group, blocks = (a.G * a.L + per - 1) / per;
@@ -41,7 +41,7 @@ static int gq(const Args &a, hipStream_t s) {
   static LdsRaised plain, full;
   const long long grid = (long long)a.B * a.splits * a.Hk * a.blocks;
   constexpr int lds = GqCfg<TY, DP, MT, WQ>::LDS;
-  if constexpr (DP == 128 && MT > 1) {                          // the plan's: 64 rows with masks and dropout
+  if constexpr (DP >= 96 && MT > 1 && TY != DI_F32) {                          // the plan: 64 rows with masks and dropout
     return go(attention_gq_kernel<TY, DP, MT, WQ, false>, plain, lds, grid, a, s, "attention_gq");
   } else {
     return needs_full(a) ? go(attention_gq_kernel<TY, DP, MT, WQ, true>, full, lds, grid, a, s, "attention_gq")
@@ -89,6 +89,7 @@ int launch_fwd(const Args &args, const Plan &p, hipStream_t s) {
     case 16: DI_AT_FWD(16); break;
     case 32: DI_AT_FWD(32); break;
     case 64: DI_AT_FWD(64); break;
+    case 96: DI_AT_FWD(96); break;
     default: DI_AT_FWD(128); break;
   }
 #undef DI_AT_FWD
@@ -106,6 +107,7 @@ int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) 
   rc = pq.big == 0 ? gq<TY, DP, 1, 1>(a, s) : pq.big == 1 ? gq<TY, DP, 1, 4>(a, s) : gq<TY, DP, row_tiles(DP), 4>(a, s)
     if (a.L > 0) {
       if (padded(a.D) == 64) DI_AT_GQ(64);
+      else if (padded(a.D) == 96) DI_AT_GQ(96);
       else DI_AT_GQ(128);
     }
 #undef DI_AT_GQ
@@ -125,6 +127,7 @@ int launch_bwd(const Args &args, const Plan &pq, const Plan &pk, hipStream_t s) 
     case 16: DI_AT_GKV(16); break;
     case 32: DI_AT_GKV(32); break;
     case 64: DI_AT_GKV(64); break;
+    case 96: DI_AT_GKV(96); break;
     default: DI_AT_GKV(128); break;
   }
 #undef DI_AT_GKV

@@ -16,10 +16,11 @@ int launch_fwd(const Args &a, const Plan &p, hipStream_t s);
 template <int TY>
 int launch_bwd(const Args &a, const Plan &gq, const Plan &gkv, hipStream_t s);
 
-constexpr int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+// (72 of 96 rather than of 128 dims, 2 x 1000 x 4000 x 8 heads: float32 305 + 430 + 573 -> 257 + 347 + 443 us, bf16 46 + 68 + 92 -> 45 + 52 + 87)
+constexpr int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 constexpr int row_tiles(int DP) { return DP <= 32 ? 4 : 2; }                       // MT of the large variant
 constexpr bool one_launch(int DP) { return DP <= 32; }                              // the backward's key-block kernel forms gq as well
-// Key tiles per wavefront at the most.  Heads of 128: one, two wavefronts a SIMD (2048 x 8192 x 16 heads, bf16: 380 us; two tiles, whose
+// Key tiles per wavefront at the most.  Heads of 96 and 128: one, two wavefronts a SIMD (2048 x 8192 x 16 heads, bf16: 380 us; two tiles, whose
 // sums leave room for one: 394).  Heads of 64: two (161 us; one: 189)
 constexpr int key_tiles(int TY, int DP) { return DP == 16 ? 4 : DP == 32 ? (TY == DI_F32 ? 2 : 4) : DP == 64 ? 2 : 1; }
 // With a (query, key) mask or dropout two at the most: their words and hashes take the registers of the second wavefront a SIMD (half precision, with four

@@ -194,6 +194,20 @@ def test_mask_rows_that_start_and_end_anywhere(S, D):
 
 
 @pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('D', range(8, 129, 8))
+def test_every_head_dim(D, t):
+    """Single queries, few rows and row blocks, ragged lengths and masks, split ranges, dropout."""
+    for B, L, S, H, Hk in ((3, 1, 333, 4, 2), (2, 19, 201, 2, 1), (1, 150, 700, 2, 2)):
+        q, k, v, go = make(B, L, S, H, Hk, D, t)
+        check(q, k, v, go, H)
+        lengths = torch.tensor([S, 0, S - 70][:B], dtype=torch.int32, device='cuda')
+        mask, allowed = torch.rand(B, S, device='cuda') < 0.8, torch.rand(B, L, S, device='cuda') < 0.5
+        keep = (torch.arange(S, device='cuda') < lengths[:, None]) & mask
+        check(q, k, v, go, H, keep[:, None].expand(B, L, S), key_lengths=lengths, key_mask=mask)
+        check(q, k, v, go, H, keep[:, None] & allowed, key_lengths=lengths, key_mask=mask, allowed=allowed)
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
 @pytest.mark.parametrize('L,S,D', [(1, 300, 16), (70, 300, 16), (200, 40, 32), (40, 130, 64), (150, 200, 128), (5, 700, 128)])
 def test_queries_without_keys_may_hold_anything(t, L, S, D):
     """A padded query: nothing allowed, NaN in its projection and its incoming gradient.  It gives zeros and reaches no other gradient."""
