@@ -263,6 +263,16 @@ __device__ __forceinline__ int keys_of(const Args &a, int b) {
   return n < 0 ? 0 : (n < a.S ? n : a.S);
 }
 
+// A row with a single key: its probability is 1 whatever the score, the score's gradient exactly 0 - not the rounding of dp - delta, all
+// that would be left of gq and gk where every row is such a one.  Looked for where there are few keys at all.
+constexpr int kFew = 16;
+__device__ __forceinline__ bool one_key(const Args &a, int b, int query, int n) {
+  int c = 0;
+  for (int k = 0; k < n; ++k)
+    c += (a.kmask == nullptr || a.kmask[b * a.kmask_bs + k] != 0) && (a.allowed == nullptr || a.allowed[b * a.allowed_bs + query * a.allowed_rs + k] != 0);
+  return c <= 1;
+}
+
 // Samples of different lengths: the workgroups that have keys come first - dealt out to the XCDs as above, key blocks (equal work) in
 // equal consecutive shares - and those without behind them.  Every wavefront finds its sample from the running sum of the samples' workgroups with keys (a lane each, so up
 // to 64 samples).  A sample's workgroups are ordered by what its length cuts off: key ranges (row blocks), key blocks (KEYS).

@@ -53,7 +53,8 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
   const Where at = where<false>(a);
   const int wq = WQ == 1 ? 0 : (wave + at.sp + at.hk + at.b) % WQ, wk = wave / WQ;
   const int rows = a.G * a.L, ntile = (rows + 15) / 16;
-  const int k0 = at.sp * a.range, k1 = min(k0 + a.range, keys_of(a, at.b));
+  const int nkeys = keys_of(a, at.b), k0 = at.sp * a.range, k1 = min(k0 + a.range, nkeys);
+  const bool few = a.S <= kFew;
   const char *kb = a.k + at.b * a.k_bs + (long long)at.hk * a.D * M::SZ, *vb = a.v + at.b * a.v_bs + (long long)at.hk * a.D * M::SZ;
   const unsigned char *km = !FULL || a.kmask == nullptr ? nullptr : a.kmask + at.b * a.kmask_bs;
   const long long row_id = ((long long)at.b * a.Hk + at.hk) * rows;
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(256) void attention_gq_kernel(Args a) {
     d += __shfl_xor(d, 32);
     const float e = ok ? a.lse[row_id + r] : INFINITY;
     lse[t] = e == -INFINITY ? INFINITY : e;                     // an empty row: every probability 0, and no gradient whatever it holds
+    if (few && ok && one_key(a, at.b, query[t], nkeys)) lse[t] = INFINITY;
     if (e == -INFINITY) d = 0.f;
     delta[t] = d;
     if (ok && at.sp == 0 && wk == 0 && g == 0) a.delta[row_id + row[t]] = d;
@@ -238,7 +240,7 @@ struct GkvCfg {
   static constexpr int BR = DP * M::SZ >= 512 || (GQ && DP > 16) ? 32 : 64;        // rows per tile
   static constexpr int KEYS = 64 * NT;
   static constexpr int G_AT = BR * M::TRS, ST_AT = 2 * G_AT;    // both tiles are read in rows and transposed
-  static constexpr int K_AT = ST_AT + 2 * BR * 4;               // GQ: the block's keys,
+  static constexpr int K_AT = ST_AT + 3 * BR * 4;               // GQ: the block's keys,
   static constexpr int DS_AT = K_AT + KEYS * M::TRS;            // each wavefront's score gradients of CH keys as (key, row),
   static constexpr int DS_ROW = M::CH * M::SZ + (M::WIDE ? 16 : 32), DS_WAVE = M::CH * DS_ROW;
   static constexpr int RED_AT = DS_AT + 4 * DS_WAVE;            // and its share of gq of the tile's rows, float32
@@ -265,10 +267,11 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
   using C = GkvCfg<TY, DP, NT, GQ>;
   using M = Mm<TY, DP>;
   extern __shared__ __align__(16) char lds[];
-  float *slse = reinterpret_cast<float *>(lds + C::ST_AT), *sdelta = slse + C::BR;
+  float *slse = reinterpret_cast<float *>(lds + C::ST_AT), *sdelta = slse + C::BR, *sone = sdelta + C::BR;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
   const Where at = where<true>(a);
   const int rows = a.G * a.L, nkeys = keys_of(a, at.b);
+  const bool few = NT == (GQ ? 2 : 1) && a.S <= kFew;           // (few keys: the plan's smallest block)
   const int key0 = at.blk * C::KEYS;
   // a block without keys: zeros (the only block: gq's zeros, too)
   const int r0 = at.sp * a.range, r1 = key0 < nkeys || (GQ && a.blocks == 1) ? min(r0 + a.range, rows) : r0;
@@ -413,6 +416,10 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
     if (tid < C::BR) {
       slse[tid] = ls == -INFINITY ? INFINITY : ls - C::P_LOG2;
       if (!GQ) sdelta[tid] = de * (1.f / C::P_SCALE);
+      if (few) {
+        const int r = min(t0 + tid, rows - 1), head = a.G == 1 ? 0 : (int)a.by_L.of(r);
+        sone[tid] = one_key(a, at.b, r - head * a.L, nkeys) ? 0.f : 1.f;
+      }
       if (FULL && a.drop) *reinterpret_cast<unsigned *>(lds + C::LDS + C::MASK + 4 * tid) = drop_row(seed, row_id + t0 + tid);
     }
     __syncthreads();
@@ -485,6 +492,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
             }
             ds[r] = pr * fmaf(dp[n][r], 1.f / C::P_SCALE, -d4[r]);
           }
+          if (few) ds *= *reinterpret_cast<const f4 *>(sone + rc + 16 * u + 4 * g);
           if (GQ && !whole) {                                   // gq sums over the columns: those of excluded keys have to be zero
 #pragma unroll
             for (int r = 0; r < 4; ++r) ds[r] = valid[n] ? ds[r] : 0.f;

@@ -240,6 +240,24 @@ def test_gradients_that_would_overlap_are_refused(D):
                 ops.cross_attention_train_bwd(q, k, v, o, go, lse, 2, grads_kv=pair)
 
 
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('D', [16, 24, 64, 80, 128])
+def test_a_single_key_has_no_score_gradient(D, t):
+    """Exact zeros in gq and gk where every query has one key: S = 1, masks that leave one, another one for every query."""
+    H, Hk = 4, 2
+    for B, L, S in ((3, 70, 1), (2, 1, 1), (2, 33, 2), (1, 150, 16)):
+        q, k, v, go = make(B, L, S, H, Hk, D, t)
+        pick = torch.randint(0, S, (B, L), device='cuda')
+        allowed = torch.zeros(B, L, S, dtype=torch.bool, device='cuda').scatter_(2, pick[..., None], True)
+        allowed[:, -1] &= L == 1                                       # and a query without any
+        mask = torch.zeros(B, S, dtype=torch.bool, device='cuda').scatter_(1, pick[:, :1], True)
+        one = torch.ones(B, dtype=torch.int32, device='cuda')
+        for kw, keep in ((dict(key_lengths=one), torch.arange(S, device='cuda')[None, None] < 1), (dict(key_mask=mask), mask[:, None]),
+                         (dict(allowed=allowed), allowed)) + (((dict(), None),) if S == 1 else ()):
+            _, _, gq, gk, _ = check(q, k, v, go, H, None if keep is None else keep.expand(B, L, S), **kw)
+            assert not gq.any() and not gk.any()
+
+
 def test_nothing_to_attend_to():
     for t in TYPES:
         for B, L, S in ((2, 5, 0), (2, 0, 7), (0, 3, 4), (2, 100, 0)):
