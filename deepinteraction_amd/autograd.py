@@ -4,8 +4,6 @@ Forward = the inference kernels; backward = the float32-atomic scatter kernels o
 feature maps receive gradients: sampling coordinates are functions of points, metas and detached box
 predictions, exactly as in the reference (F.grid_sample's grid at encoder_utils.py:195,:297 is built from
 data; the RoI boxes come from deep-copied, decoded predictions, decoder_utils.py:672-679)."""
-import contextlib
-
 import torch
 from torch.amp import custom_bwd, custom_fwd
 from torch.autograd.function import once_differentiable
@@ -232,25 +230,9 @@ class CrossAttention(torch.autograd.Function):
         return gq, gk if packed is None else packed, gv if packed is None else None, None, None, None, None, None, None, None
 
 
-_LIBRARY_FORMS = [False]
-
-
-@contextlib.contextmanager
-def library_forms():
-    """Modules called inside compute attention and post-norm steps through library products and modules instead of
-    `cross_attention` and `AddLayerNorm` (`train_step.GraphedTrainer` captures its step so)."""
-    before, _LIBRARY_FORMS[0] = _LIBRARY_FORMS[0], True
-    try:
-        yield
-    finally:
-        _LIBRARY_FORMS[0] = before
-
-
 def cross_attention_usable(q, k, num_heads):
     """Whether `cross_attention` takes these projections: on the GPU, one of float32 / float16 / bfloat16, a head dim of 8 .. 128 in
-    steps of 8 (and not inside `library_forms`)."""
-    if _LIBRARY_FORMS[0]:
-        return False
+    steps of 8."""
     D = q.shape[-1] // num_heads
     return q.is_cuda and q.dtype == k.dtype and q.dtype in (torch.float32, torch.float16, torch.bfloat16) and D % 8 == 0 and 8 <= D <= 128
 

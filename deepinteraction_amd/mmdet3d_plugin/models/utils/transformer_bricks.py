@@ -9,7 +9,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .... import ops
-from ....autograd import _LIBRARY_FORMS, AddLayerNorm, MSDeformAttn
+from ....autograd import AddLayerNorm, MSDeformAttn
 from ....utils import param_key
 
 
@@ -19,7 +19,7 @@ _NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 def _norm_type(norm, x, branch):
     """The type of `norm(x + branch)` where the LayerNorm kernels take it, None elsewhere: autocast evaluates the norm in float32
     whatever its operands are; without it the operands' common type has to be the norm's own."""
-    if not (x.is_cuda and not _LIBRARY_FORMS[0] and isinstance(norm, nn.LayerNorm) and norm.elementwise_affine and norm.bias is not None
+    if not (x.is_cuda and isinstance(norm, nn.LayerNorm) and norm.elementwise_affine and norm.bias is not None
             and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= ops.LAYERNORM_MAX_C
             and (branch is None or branch.shape == x.shape)):
         return None

@@ -293,15 +293,11 @@ class GraphedTrainer(Trainer):
         # no garbage collection INSIDE the captures: a collected autograd graph of a warm-up iteration (Python Function nodes are
         # freed by the collector, not by reference counting) releases device memory through calls a capturing process may not make
         import gc
-        from .autograd import library_forms
         gc.collect()
         was_enabled = gc.isenabled()
         gc.disable()
         try:
-            # (library_forms: with the attention and LayerNorm operators inside, the replay of the backward graph ended the process once,
-            # late in a long session; without a known cause they stay out of this capture)
-            with library_forms():
-                self.graphed = torch.cuda.make_graphed_callables(self.module, (h.img_feats, h.pts_feats), allow_unused_input=True)
+            self.graphed = torch.cuda.make_graphed_callables(self.module, (h.img_feats, h.pts_feats), allow_unused_input=True)
         finally:
             ops.set_i2p_seed_tensor(None)
             if was_enabled:

@@ -125,17 +125,3 @@ def test_the_argument_block_s_layout():
     """Three pointers and six strides, five mask words and strides, seven ints, two floats, four bytes of padding, the seed."""
     A = _lib.Attention
     assert (A.q_bs.offset, A.key_lengths.offset, A.B.offset, A.scale.offset, A.seed.offset, ctypes.sizeof(A)) == (24, 72, 120, 148, 160, 168)
-
-
-def test_library_forms_switches_the_operators_off_and_on():
-    class Projection:
-        is_cuda, dtype, shape = True, torch.float32, (1, 2, 32)
-    assert autograd.cross_attention_usable(Projection, Projection, 2)
-    with pytest.raises(ZeroDivisionError):
-        with autograd.library_forms():
-            assert not autograd.cross_attention_usable(Projection, Projection, 2)
-            with autograd.library_forms():
-                pass
-            assert not autograd.cross_attention_usable(Projection, Projection, 2)
-            1 // 0
-    assert autograd.cross_attention_usable(Projection, Projection, 2)
