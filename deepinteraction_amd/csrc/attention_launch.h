@@ -56,7 +56,7 @@ static int gkv(const Args &a, hipStream_t s) {
   using C = GkvCfg<TY, DP, NT, GQ>;
   static_assert(C::BR == tile_rows(TY, DP) && C::LDS % 16 == 0, "the plan's tiles; the mask's words");
   if constexpr (NT <= most_masked_key_tiles) {
-    if (a.allowed != nullptr || a.drop != 0) return go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, C::LDS + C::MASK + C::DROP, grid, a, s, "attention_gkv");
+    if (a.allowed != nullptr || a.drop != 0 || a.S <= kFew) return go(attention_gkv_kernel<TY, DP, NT, GQ, true>, full, C::LDS + C::MASK + C::DROP, grid, a, s, "attention_gkv");
   }
   return go(attention_gkv_kernel<TY, DP, NT, GQ, false>, plain, C::LDS, grid, a, s, "attention_gkv");
 }
