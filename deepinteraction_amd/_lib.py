@@ -124,7 +124,6 @@ class TokHeads(ctypes.Structure):
                 ('nheads', _c_i), ('center_head', _c_i), ('ldo', _c_i), ('col0', _c_i), ('qpos2', _c_p), ('pos2_out', _c_p)]
 
 
-
 class Attention(ctypes.Structure):
     _fields_ = ([(n, _c_p) for n in ('q', 'k', 'v')] + [(n, _c_ll) for n in ('q_bs', 'q_rs', 'k_bs', 'k_rs', 'v_bs', 'v_rs')] +
                 [('key_lengths', _c_p), ('key_mask', _c_p), ('key_mask_bs', _c_ll), ('allowed', _c_p), ('allowed_bs', _c_ll),

@@ -173,7 +173,6 @@ __global__ __launch_bounds__(256, (DP >= 96 && TY != DI_F32) || (DP == 32 && FUL
   auto tile = [&](auto edge, auto count, int t0) {
     constexpr bool EDGE = decltype(edge)::value;
     constexpr int N = decltype(count)::value;
-    constexpr bool EARLY = true;
 #pragma unroll
     for (int c = 0; c < C::CPT; ++c) {
       const int kc = (wk * C::CPT + c) * M::CH;                 // first key of the chunk in the tile
@@ -191,7 +190,7 @@ __global__ __launch_bounds__(256, (DP >= 96 && TY != DI_F32) || (DP == 32 && FUL
       for (int u = 0; u < M::NT; ++u)
 #pragma unroll
         for (int kk = 0; kk < M::NK; ++kk) kf[u][kk] = M::row_frag(lds + (kc + 16 * u + i) * M::ROWS, kk, g);
-      if (EARLY) __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);
       f4 s[MT][M::NT];
 #pragma unroll
       for (int u = 0; u < M::NT; ++u) {
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(256, (DP >= 96 && TY != DI_F32) || (DP == 32 && FUL
       typename M::TF vf[M::ND];                                 // in flight behind the exponentials
 #pragma unroll
       for (int d = 0; d < M::ND; ++d) vf[d] = M::tr_frag(lds + C::V_AT, M::TRS, kc, d, i, g);
-      if (EARLY) __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);
       typename M::PF pf[MT];
 #pragma unroll
       for (int t = 0; t < N; ++t) {
