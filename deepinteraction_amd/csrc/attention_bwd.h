@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256, GQ && DP == 16 && !FULL ? 3 : DP >= 64 && TY !
   const char *qb = a.q + at.b * a.q_bs, *gb = a.go + at.b * a.go_bs;
   const long long o_rs = (long long)a.Hk * a.G * a.D * M::SZ;
   const unsigned oo = (unsigned)(first * o_rs) + piece * 16;
-  const char *ob = a.o + at.b * a.L * o_rs;
+  const char *ob = a.o + (long long)at.b * a.L * o_rs;
   auto fetch = [&](int t0) {
     const int head0 = a.G == 1 ? 0 : (int)a.by_L.of(t0), l0 = t0 - head0 * a.L;
     if (t0 + C::BR <= r1 && l0 + C::BR <= a.L) {

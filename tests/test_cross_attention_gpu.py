@@ -454,3 +454,17 @@ def test_refusals():
             bad()
     with pytest.raises(ops._lib.HipLibraryError):
         ops.cross_attention(q.cpu(), k, v, 4)
+
+
+def test_queries_past_32_bits():
+    """More than 2^31 queries in all: every sample is the same, and so is every sample's result, bit for bit."""
+    B, L, D, S = 2 ** 21 + 3, 1024, 8, 2
+    q, k, v, go = (x[:1].expand(B, -1, -1) for x in make(1, L, S, 1, 1, D, F16))
+    o, lse = ops.cross_attention_train_fwd(q, k, v, 1)
+    gq, gk, gv = ops.cross_attention_train_bwd(q, k, v, o, go, lse, 1)
+    want = ops.cross_attention_train_fwd(q[:1], k[:1], v[:1], 1)
+    want += ops.cross_attention_train_bwd(q[:1], k[:1], v[:1], want[0], go[:1], want[1], 1)
+    for name, got, one in zip(('o', 'lse', 'gq', 'gk', 'gv'), (o, lse, gq, gk, gv), want):
+        for b in range(0, B, 1 << 17):
+            part = got[b:b + (1 << 17)]
+            assert torch.equal(part, one.expand_as(part)), (name, b)
