@@ -39,23 +39,37 @@ static bool ragged(const di_attention &t, const Plan &p, int cus) {
   return t.key_lengths != nullptr && t.B <= 64 && (long long)t.B * t.kv_heads * p.blocks * p.splits > cus;
 }
 
+// Rows per workgroup, and key tiles per wavefront, of a call that fills the CUs without splitting (the reasons above and in
+// attention_plan.h).
+static int row_block(const di_attention &t, bool forward) {
+  const int DP = padded(t.head_dim);
+  const long long rows = (long long)(t.heads / t.kv_heads) * t.L;
+  const bool full = t.key_mask != nullptr || t.allowed != nullptr || t.dropout_p > 0.f;
+  if (rows <= 16) return 16;
+  return rows <= 64 || (!forward && DP >= 96 && full && t.dtype != DI_F32) ? 64 : 64 * row_tiles(DP);
+}
+static int widest_key_tiles(const di_attention &t) {
+  const int n = key_tiles(t.dtype, padded(t.head_dim));
+  return (t.allowed != nullptr || t.dropout_p > 0.f) && n > most_masked_key_tiles ? most_masked_key_tiles : n;
+}
+
 static int plan_rows(const di_attention &t, bool forward, Plan &p) {
   const int cus = device_cus();
   if (cus <= 0) return DI_ERR_LAUNCH;
-  const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L;
+  const int DP = padded(t.head_dim), rows = t.heads / t.kv_heads * t.L, block = row_block(t, forward);
   const long long problems = (long long)t.B * t.kv_heads;
-  if (rows <= 16) {
+  if (block == 16) {
     p.big = 0;
     cut(p, problems, rows, 16, t.S, t.dtype != DI_F32 ? 128 : 64, 4, 1, 24ll * cus);
     p.ragged = ragged(t, p, cus);
     return DI_OK;
   }
-  const bool wide = !forward && DP == 128, full = t.key_mask != nullptr || t.allowed != nullptr || t.dropout_p > 0.f;
+  const bool wide = !forward && DP == 128;
   const long long want = 2ll * cus * (t.key_lengths != nullptr ? 2 : 1);
   const int some = t.dtype == DI_F32 && DP >= 64 ? 16 : 1;
   p.big = 2;
   cut(p, problems, rows, 64 * row_tiles(DP), t.S, 64, 4, some, wide ? want / 2 : want);
-  if (rows <= 64 || (!forward && DP >= 96 && full && t.dtype != DI_F32) || problems * p.blocks * p.splits < cus) {
+  if (block == 64 || problems * p.blocks * p.splits < cus) {
     p.big = 1;
     cut(p, problems, rows, 64, t.S, 64, 4, some, DP <= 32 ? 4 * want : want);
   }
@@ -70,9 +84,7 @@ static int plan_keys(const di_attention &t, Plan &p) {
   const int tile = tile_rows(t.dtype, DP);
   const long long problems = (long long)t.B * t.kv_heads;
   const int S = t.S > 0 ? t.S : 1;                              // without keys, one block still writes gq's zeros
-  const bool full = t.allowed != nullptr || t.dropout_p > 0.f;
-  p.big = key_tiles(t.dtype, DP);
-  if (full && p.big > most_masked_key_tiles) p.big = most_masked_key_tiles;
+  p.big = widest_key_tiles(t);
   for (; p.big > least; p.big /= 2) {   // the largest key block that the keys fill, and that leaves work for all
     if (32 * p.big >= t.S) continue;
     cut(p, problems, S, 64 * p.big, rows, tile, 1, 1, 2ll * cus);
@@ -81,6 +93,21 @@ static int plan_keys(const di_attention &t, Plan &p) {
   if (p.big <= least) cut(p, problems, S, 64 * p.big, rows, tile, 1, 1, 2ll * cus);
   p.ragged = ragged(t, p, cus);
   return DI_OK;
+}
+
+// A launch has fewer than 2^32 work-items, 256 a workgroup.  Only calls of more workgroups than any plan splits for come near: the blocks
+// of the two plans as they are without splits, and the join of narrow heads' gq over the key blocks.
+static bool fits(const di_attention &t, bool forward) {
+  const int DP = padded(t.head_dim);
+  const long long problems = (long long)t.B * t.kv_heads, rows = (long long)(t.heads / t.kv_heads) * t.L, most = (1 << 24) - 1;
+  const int per = row_block(t, forward);
+  if ((forward || !one_launch(DP)) && problems * ((rows + per - 1) / per) > most) return false;
+  if (forward) return true;
+  int big = widest_key_tiles(t);
+  while (big > least_key_tiles(DP) && 32 * big >= t.S) big /= 2;
+  const long long blocks = t.S > 0 ? ((long long)t.S + 64 * big - 1) / (64 * big) : 1;
+  if (problems * blocks > most) return false;
+  return !one_launch(DP) || blocks == 1 || problems * join_shape(t.head_dim, (int)blocks, (int)rows).blocks <= most;
 }
 
 // floats of the backward's workspace: delta | the sums of gq | the sums of gk and gv.  Two launches: gq's are joined before the others
@@ -102,7 +129,7 @@ static bool aligned(const void *p, long long bs, long long rs, int size) {
   return ((uintptr_t)p & 15) == 0 && (bs * size) % 16 == 0 && (rs * size) % 16 == 0 && rs >= 0 && rs * size < (1ll << 24);
 }
 
-static int check(const di_attention *t) {
+static int check(const di_attention *t, bool forward) {
   DI_REQUIRE(t != nullptr, "attention: null pointer");
   DI_REQUIRE(t->dtype == DI_F32 || t->dtype == DI_F16 || t->dtype == DI_BF16, "attention: unsupported dtype %d", t->dtype);
   DI_REQUIRE(t->B >= 0 && t->L >= 0 && t->S >= 0, "attention: negative size");
@@ -112,9 +139,7 @@ static int check(const di_attention *t) {
   DI_REQUIRE(t->dropout_p >= 0.f && t->dropout_p < 1.f, "attention: dropout probability %f", (double)t->dropout_p);
   const long long rows = (long long)(t->heads / t->kv_heads) * t->L;
   DI_REQUIRE(rows <= 0x3fffffff && t->S <= 0x3fffffff, "attention: more than 2^30 rows or keys");
-  // every grid: problems x blocks x splits (few problems), and the joins' four rows and more per workgroup
-  const long long most = (long long)t->B * t->kv_heads * ((rows > t->S ? rows : t->S) / 4 + 2);
-  DI_REQUIRE(most <= 0x7fffffff / 2, "attention: too many rows for one launch");
+  DI_REQUIRE(fits(*t, forward), "attention: too many rows or keys for one launch (2^24 workgroups)");
   const int sz = t->dtype == DI_F32 ? 4 : 2;
   // rows of the output - and of the keys' gradients - are addressed as those of the inputs
   DI_REQUIRE((long long)t->heads * t->head_dim * sz < (1ll << 24), "attention: %d heads of %d (rows of 16 MB and more)", t->heads, t->head_dim);
@@ -161,7 +186,7 @@ extern "C" {
 
 long long di_attention_fwd_workspace_floats(const di_attention *t) {
   using namespace di::at;
-  if (check(t) != DI_OK) return -1;
+  if (check(t, true) != DI_OK) return -1;
   Plan p;
   if (plan_rows(*t, true, p) != DI_OK) return -1;
   return p.splits == 1 ? 0 : (long long)p.splits * t->B * t->heads * t->L * (t->head_dim + 2);
@@ -169,7 +194,7 @@ long long di_attention_fwd_workspace_floats(const di_attention *t) {
 
 long long di_attention_bwd_workspace_floats(const di_attention *t) {
   using namespace di::at;
-  if (check(t) != DI_OK) return -1;
+  if (check(t, false) != DI_OK) return -1;
   Plan p, k;
   if (plan_rows(*t, false, p) != DI_OK || plan_keys(*t, k) != DI_OK) return -1;
   const Room r = room_of(*t, p, k);
@@ -178,7 +203,7 @@ long long di_attention_bwd_workspace_floats(const di_attention *t) {
 
 int di_attention_fwd(const di_attention *t, void *out, float *lse, float *workspace, void *stream) {
   using namespace di::at;
-  if (int rc = check(t)) return rc;
+  if (int rc = check(t, true)) return rc;
   if (t->B == 0 || t->L == 0) return DI_OK;
   DI_REQUIRE(out != nullptr && ((uintptr_t)out & 15) == 0, "attention: the output must start on 16 bytes");
   Plan p;
@@ -199,7 +224,7 @@ int di_attention_bwd(const di_attention *t, const void *out, const float *lse, c
                      void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs, long long gv_rs, float *workspace,
                      void *stream) {
   using namespace di::at;
-  if (int rc = check(t)) return rc;
+  if (int rc = check(t, false)) return rc;
   if (t->B == 0 || (t->L == 0 && t->S == 0)) return DI_OK;
   const int sz = t->dtype == DI_F32 ? 4 : 2;
   DI_REQUIRE(t->L == 0 || (out && lse && grad_out && gq && ((uintptr_t)out & 15) == 0 && ((uintptr_t)gq & 15) == 0 && aligned(grad_out, go_bs, go_rs, sz)),

@@ -19,12 +19,9 @@ static int go(K kernel, LdsRaised &raised, int lds, long long grid, const Args &
 template <int TY, bool STATS>
 static int join(const Args &args, hipStream_t s) {
   Args a = args;
-  const int nd = (padded(a.D) == 96 ? 128 : padded(a.D)) / 4;    // lanes across the head dim: a power of two
-  int group = nd;
-  while (group < 64 && 4 * (group / nd) < a.splits) group *= 2;
-  const int per = 256 / group, blocks = (a.G * a.L + per - 1) / per;
-  a.by_unit = div_by(blocks);
-  hipLaunchKernelGGL((attention_join_kernel<TY, STATS>), dim3((unsigned)(a.B * a.Hk * blocks)), dim3(256), 0, s, a, nd, group);
+  const JoinShape j = join_shape(a.D, a.splits, a.G * a.L);
+  a.by_unit = div_by(j.blocks);
+  hipLaunchKernelGGL((attention_join_kernel<TY, STATS>), dim3((unsigned)(a.B * a.Hk * j.blocks)), dim3(256), 0, s, a, j.nd, j.group);
   return check_launch("attention_join");
 }
 

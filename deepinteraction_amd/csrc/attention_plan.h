@@ -28,6 +28,19 @@ constexpr int key_tiles(int TY, int DP) { return DP == 16 ? 4 : DP == 32 ? (TY =
 // mask 322 and 241)
 constexpr int most_masked_key_tiles = 2;
 constexpr int least_key_tiles(int DP) { return one_launch(DP) ? 2 : 1; }            // 16-bit products contract over 32 keys
+// The joins: lanes across the head dim (a power of two), lanes per row - up to 64, the others on further ranges - and workgroups per problem.
+struct JoinShape {
+  int nd, group, blocks;
+};
+inline JoinShape join_shape(int D, int ranges, int rows) {
+  JoinShape j;
+  j.nd = (padded(D) == 96 ? 128 : padded(D)) / 4;
+  j.group = j.nd;
+  while (j.group < 64 && 4 * (j.group / j.nd) < ranges) j.group *= 2;
+  const int per = 256 / j.group;
+  j.blocks = (rows + per - 1) / per;
+  return j;
+}
 constexpr int tile_rows(int TY, int DP) { return DP * (TY == DI_F32 ? 4 : 2) >= 512 || DP == 32 ? 32 : 64; }
 
 }  // namespace at

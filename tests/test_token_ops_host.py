@@ -125,3 +125,21 @@ def test_the_argument_block_s_layout():
     """Three pointers and six strides, five mask words and strides, seven ints, two floats, four bytes of padding, the seed."""
     A = _lib.Attention
     assert (A.q_bs.offset, A.key_lengths.offset, A.B.offset, A.scale.offset, A.seed.offset, ctypes.sizeof(A)) == (24, 72, 120, 148, 160, 168)
+
+
+LARGE = [(True, dict(B=3 << 20, L=1, S=1, heads=8, kv_heads=8)), (True, dict(B=1 << 22, L=600, S=9, heads=1, kv_heads=1, head_dim=128)),
+         (False, dict(B=1 << 20, L=1, S=4000, heads=1, kv_heads=1)), (False, dict(B=1 << 22, L=65, S=9, heads=2, kv_heads=2, head_dim=128, dropout_p=0.5)),
+         (False, dict(B=1 << 20, L=1000, S=600, heads=8, kv_heads=1))]     # the last: the join of gq over three key blocks
+
+
+@pytest.mark.parametrize('forward,sizes', LARGE, ids=str)
+def test_attention_of_more_workgroups_than_a_launch_has(forward, sizes):
+    """2^24 - 1 workgroups of 256 threads are the most that one launch takes."""
+    t = attention(q_bs=0, k_bs=0, v_bs=0, q_rs=1024, k_rs=1024, v_rs=1024, **sizes)
+    ref = ctypes.addressof(t)
+    if forward:
+        assert L.di_attention_fwd(ref, P, None, P, None) == -1 and 'one launch' in said()
+        assert L.di_attention_fwd_workspace_floats(ref) == -1 and 'one launch' in said()
+    else:
+        assert L.di_attention_bwd(ref, P, P, P, 0, 1024, P, P, 1 << 22, 1024, P, 1 << 22, 1024, P, None) == -1 and 'one launch' in said()
+        assert L.di_attention_bwd_workspace_floats(ref) == -1 and 'one launch' in said()
