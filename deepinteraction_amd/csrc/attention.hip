@@ -150,10 +150,29 @@ static int check(const di_attention *t, bool forward) {
   return DI_OK;
 }
 
-// rows of a gradient lie apart: each is written once
-static bool apart(const di_attention &t, long long bs, long long rs) {
-  const long long E = (long long)t.kv_heads * t.head_dim;
-  return (t.S == 1 || rs >= E) && (t.B == 1 || bs >= E || bs <= -E);
+// The rows of grad_k or grad_v in memory (in elements): `nin` rows `in` apart, `nout` groups of them `out` apart.
+struct Rows {
+  long long low, in, nin, out, nout, E;                         // low: the first byte's address
+  long long group() const { return (nin - 1) * in + E; }
+  long long span() const { return (nout - 1) * out + group(); }
+  // each row is written once (nested groups; other layouts without an overlap exist, and are refused with the rest)
+  bool apart() const { return (nin == 1 || in >= E) && (nout == 1 || out >= group()); }
+};
+static Rows rows_of(const di_attention &t, const void *p, long long bs, long long rs, int sz) {
+  const long long step = bs < 0 ? -bs : bs;
+  Rows r = {(long long)(uintptr_t)p + (bs < 0 ? (t.B - 1) * bs * sz : 0), rs, t.S, step, t.B, (long long)t.kv_heads * t.head_dim};
+  if (t.S > 1 && t.B > 1 && step < rs) r = {r.low, step, t.B, rs, t.S, r.E};
+  return r;
+}
+// ... and not by the other gradient: one behind the other, or one's rows, or groups, between the other's of the same strides
+static bool clear_of(const Rows &a, const Rows &b, int sz) {
+  const Rows &lo = a.low <= b.low ? a : b, &hi = a.low <= b.low ? b : a;
+  const long long by = hi.low - lo.low;
+  if (by >= lo.span() * sz) return true;
+  const bool same = (a.nin == 1 || a.in == b.in) && (a.nout == 1 || a.out == b.out) && a.nin == b.nin;
+  const bool rows = by >= a.E * sz && (a.nin == 1 || by + a.E * sz <= a.in * sz) && (a.nout == 1 || by + a.group() * sz <= a.out * sz);
+  const bool groups = by >= a.group() * sz && (a.nout == 1 || by + a.group() * sz <= a.out * sz);
+  return same && (rows || groups);
 }
 
 static Args args_of(const di_attention *t) {
@@ -231,8 +250,10 @@ int di_attention_bwd(const di_attention *t, const void *out, const float *lse, c
              "attention: out, grad_out and grad_q must start (and grad_out step) on 16 bytes");
   DI_REQUIRE(t->S == 0 || (gk && gv && aligned(gk, gk_bs, gk_rs, sz) && aligned(gv, gv_bs, gv_rs, sz)),
              "attention: grad_k and grad_v must start and step on 16 bytes");
-  DI_REQUIRE(t->S == 0 || (apart(*t, gk_bs, gk_rs) && apart(*t, gv_bs, gv_rs)), "attention: rows of grad_k or grad_v overlap");
+  const Rows rk = rows_of(*t, gk, gk_bs, gk_rs, sz), rv = rows_of(*t, gv, gv_bs, gv_rs, sz);
+  DI_REQUIRE(t->S == 0 || (rk.apart() && rv.apart()), "attention: rows of grad_k or grad_v overlap");
   DI_REQUIRE((workspace != nullptr || t->L == 0) && ((uintptr_t)workspace & 15) == 0, "attention: workspace");   // no rows: one range, no sums
+  DI_REQUIRE(t->S == 0 || clear_of(rk, rv, sz), "attention: grad_k and grad_v overlap");
   Plan p, k;
   if (int rc = plan_rows(*t, false, p)) return rc;
   if (int rc = plan_keys(*t, k)) return rc;

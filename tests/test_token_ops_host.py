@@ -143,3 +143,29 @@ def test_attention_of_more_workgroups_than_a_launch_has(forward, sizes):
     else:
         assert L.di_attention_bwd(ref, P, P, P, 0, 1024, P, P, 1 << 22, 1024, P, 1 << 22, 1024, P, None) == -1 and 'one launch' in said()
         assert L.di_attention_bwd_workspace_floats(ref) == -1 and 'one launch' in said()
+
+
+# rows of 32 elements (64 bytes), 2 samples of 9
+OVERLAPS = [dict(gk_bs=32, gv=P + 4096), dict(gk_bs=64, gk_rs=64, gv=P + 4096), dict(gk_bs=256, gv=P + 4096), dict(gk_bs=-256, gv=P + 8192), dict(gv_bs=256, gv=P + 4096),
+            dict(gv=P), dict(gv=P + 32), dict(gv=P + 64), dict(gv=P + 512), dict(gv=P + 576 + 64), dict(gk_rs=48, gk_bs=432, gv_rs=48, gv_bs=432, gv=P + 48),
+            dict(gk_rs=64, gk_bs=576, gv_rs=64, gv_bs=576, gv=P + 96), dict(gk_rs=64, gk_bs=576, gv_rs=32, gv_bs=576, gv=P + 64)]
+
+
+@pytest.mark.parametrize('change', OVERLAPS, ids=str)
+def test_key_gradients_that_overlap(change):
+    """Rows of two samples, or of the two gradients, in one place: the last writer would win."""
+    assert L.di_attention_bwd(ctypes.addressof(attention()), *{**GRAD, **change}.values(), None) == -1 and 'overlap' in said()
+
+
+APART = [dict(gv=P + 1152), dict(gk=P + 1152), dict(gk_bs=-288, gv=P + 1152), dict(gk_rs=64, gk_bs=576, gv_rs=64, gv_bs=576, gv=P + 64),       # behind it; halves
+         dict(gk_bs=32, gk_rs=64, gv_bs=32, gv_rs=64, gv=P + 4096), dict(gk_bs=64, gk_rs=128, gv_bs=64, gv_rs=128, gv=P + 64),                  # sequence first
+         dict(gk_bs=576, gv_bs=576, gv=P + 576)]                                                                                                  # (B, 2, S, E)
+
+
+@pytest.mark.parametrize('change', APART, ids=str)
+def test_key_gradients_side_by_side(change):
+    """What is refused, if anything, is not the layout (without a GPU: the launch)."""
+    assert L.di_attention_bwd(ctypes.addressof(attention(B=0)), *{**GRAD, **change}.values(), None) == 0
+    if torch.cuda.is_available():
+        return                                                       # the pointers must not be followed
+    assert L.di_attention_bwd(ctypes.addressof(attention()), *{**GRAD, **change}.values(), None) != -1 or 'overlap' not in said()
