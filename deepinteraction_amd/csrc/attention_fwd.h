@@ -9,7 +9,9 @@
 //
 // The maximum is corrected only when a score exceeds it by more than 8 (a factor of 256 in exp2's argument, harmless in float32 and
 // in the 16-bit probabilities): the test is one comparison per tile against the lane's own scores, the exchange between lanes and
-// the correction of the sums run when any lane asks for them - a few times per row, not once per tile.
+// the correction of the sums run when any lane asks for them - a few times per row, not once per tile.  `m` is what the exponents are
+// taken from: the maximum, for float16 less 7 - with the 8 above, probabilities of up to 2^15 (65 504 is the type's largest), their rounding
+// stays relative down to 2^-21 of the largest and reaches zero at 2^-32, where the float32 sum beside them would still count them at 2^-25.
 //
 // What bounds it, and what it measured:
 //   heads of 128 and 64 (2048 x 8192 x 16 heads of 128, bf16: 172 us = 800 TFLOP/s, a large matrix product reaches 1085 on this card):
@@ -38,6 +40,7 @@ struct FwdCfg {
   static constexpr int LDS = BIAS_AT + TILE * 4 > JOIN ? BIAS_AT + TILE * 4 : JOIN;
   static constexpr int ROWS_PER_BLOCK = 16 * MT * WQ;
   static constexpr int NP = (TILE * M::PPR + 255) / 256;        // pieces per thread, K and V each
+  static constexpr float P_LOG2 = TY == DI_F16 ? 7.f : 0.f;     // the scale of the probabilities in `o` and `l` alike
 };
 
 // The staged loads of a tile of keys: rows t0 .. of K and V, zeros where there is no key (so that no NaN of an excluded key or of
@@ -222,14 +225,14 @@ __global__ __launch_bounds__(256, (DP >= 96 && TY != DI_F32) || (DP == 32 && FUL
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx[t] = larger(s[t][u][r], mx[t]);
         mx[t] *= a.scale2;
-        over |= mx[t] > m[t] + 8.f;
+        over |= mx[t] > m[t] + (8.f + C::P_LOG2);
       }
       if (__any(over)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
           float x = fmaxf(mx[t], __shfl_xor(mx[t], 16));
           x = fmaxf(x, __shfl_xor(x, 32));
-          x = fmaxf(x, m[t]);
+          x = fmaxf(x - C::P_LOG2, m[t]);
           const float f = __builtin_amdgcn_exp2f(m[t] - x);
           m[t] = x;
           l[t] *= f;

@@ -468,3 +468,26 @@ def test_queries_past_32_bits():
         for b in range(0, B, 1 << 17):
             part = got[b:b + (1 << 17)]
             assert torch.equal(part, got[:1].expand_as(part)), (name, b)
+
+
+@pytest.mark.parametrize('far', [20.0, 25.3, 27.0])
+@pytest.mark.parametrize('L,S,D', [(1, 65537, 16), (40, 65537, 16), (3, 30001, 64), (70, 65537, 128)])
+def test_many_keys_far_below_the_largest(L, S, D, far):
+    """One key and tens of thousands of 2^-far of its weight, float16: they count in the sum of the softmax, and have to in o.  A far
+    probability is rounded once, to 11 bits or - below 2^-21 of the largest - to a step of 2^-31 of it: off by 2^-11 of itself or 2^-32."""
+    q = torch.zeros(1, L, D, device='cuda', dtype=F16)
+    q[..., 0] = 1
+    k = torch.zeros(1, S, D, device='cuda', dtype=F16)
+    k[:, :, 0] = -far * math.log(2)
+    k[:, S // 3] = 0
+    v = (1 + torch.rand(1, S, D, device='cuda')).to(F16)
+    o = ops.cross_attention(q, k, v, 1, scale=1.0).double()
+    s = k[0, :, 0].double()
+    p = torch.softmax(s, 0)
+    want = (p[:, None] * v[0].double()).sum(0)
+    # (the exponent's own error is that of a score of up to 27 ln 2; the sums' as everywhere above: (S / 16) u.  65 536 keys of 2^-25.3 are worth
+    # 1.6e-3 of o, three times the result's half step: left out, they would show)
+    e, rel = 2.0 ** -11, p / p.max()
+    off = torch.where(rel >= 2.0 ** -21, p * e, 2.0 ** -32 * p.max()) + p * (S / 16 + 300) * U
+    tol = (off[:, None] * v[0].double()).sum(0) + e * want
+    assert ((o - want).abs() <= tol).all(), float(((o - want).abs() / tol).max())
