@@ -471,17 +471,18 @@ def test_queries_past_32_bits():
 
 
 @pytest.mark.parametrize('far', [20.0, 25.3, 27.0])
-@pytest.mark.parametrize('L,S,D', [(1, 65537, 16), (40, 65537, 16), (3, 30001, 64), (70, 65537, 128)])
-def test_many_keys_far_below_the_largest(L, S, D, far):
-    """One key and tens of thousands of 2^-far of its weight, float16: they count in the sum of the softmax, and have to in o.  A far
+@pytest.mark.parametrize('B,L,S,G,D', [(1, 1, 65537, 1, 16), (1, 40, 65537, 1, 16), (6144, 1, 65537, 1, 16), (1, 300, 65537, 512, 16), (1, 300, 65537, 256, 64),
+                                       (1, 300, 65537, 256, 128)])
+def test_many_keys_far_below_the_largest(B, L, S, G, D, far):
+    """(Few queries: ranges of the keys with maxima of their own.  Many: one pass, the largest key first.)  One key and tens of thousands of 2^-far of its weight, float16: they count in the sum of the softmax, and have to in o.  A far
     probability is rounded once, to 11 bits or - below 2^-21 of the largest - to a step of 2^-31 of it: off by 2^-11 of itself or 2^-32."""
-    q = torch.zeros(1, L, D, device='cuda', dtype=F16)
-    q[..., 0] = 1
+    q = torch.zeros(B, L, G * D, device='cuda', dtype=F16)
+    q[..., ::D] = 1
     k = torch.zeros(1, S, D, device='cuda', dtype=F16)
     k[:, :, 0] = -far * math.log(2)
-    k[:, S // 3] = 0
+    k[:, 0] = 0
     v = (1 + torch.rand(1, S, D, device='cuda')).to(F16)
-    o = ops.cross_attention(q, k, v, 1, scale=1.0).double()
+    o = ops.cross_attention(q, k.expand(B, S, D), v.expand(B, S, D), G, scale=1.0).double().view(-1, D)
     s = k[0, :, 0].double()
     p = torch.softmax(s, 0)
     want = (p[:, None] * v[0].double()).sum(0)
