@@ -53,6 +53,8 @@ SIGNATURES = {
     'di_add_layernorm_fwd': [_c_p] * 5 + [ctypes.c_longlong, _c_i, _c_f, _c_i, _c_p],
     'di_attention_fwd': [_c_p] * 5,
     'di_attention_bwd': [_c_p] * 4 + [_c_ll, _c_ll, _c_p] + [_c_p, _c_ll, _c_ll] * 2 + [_c_p, _c_p],
+    'di_attention_fwd_seeded': [_c_p] * 6,
+    'di_attention_bwd_seeded': [_c_p] * 5 + [_c_ll, _c_ll, _c_p] + [_c_p, _c_ll, _c_ll] * 2 + [_c_p, _c_p],
     'di_layernorm_fwd': [_c_p, _c_ll, _c_i] * 2 + [_c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_p, _c_p, _c_ll, _c_i, _c_f, _c_p],
     'di_layernorm_bwd': [_c_p, _c_ll, _c_i, _c_p, _c_ll] + [_c_p, _c_ll, _c_i] * 2 + [_c_p, _c_i, _c_p, _c_p, _c_p, _c_i] + [_c_p] * 4 +
                         [_c_ll, _c_i, _c_p],

@@ -207,11 +207,11 @@ class CrossAttention(torch.autograd.Function):
 
     @staticmethod
     @_fwd
-    def forward(ctx, q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed):
+    def forward(ctx, q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, seed_word=None):
         Ek = k.shape[-1] // 2
         ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
-        out, lse = ops.cross_attention_train_fwd(q, ks, vs, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
-        ctx.save_for_backward(q, k, v, out, lse, key_lengths, key_mask, allowed)
+        out, lse = ops.cross_attention_train_fwd(q, ks, vs, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, seed_word)
+        ctx.save_for_backward(q, k, v, out, lse, key_lengths, key_mask, allowed, seed_word)
         ctx.args = (num_heads, scale, dropout_p, seed)
         return out
 
@@ -219,15 +219,35 @@ class CrossAttention(torch.autograd.Function):
     @once_differentiable
     @_bwd
     def backward(ctx, grad_out):
-        q, k, v, out, lse, key_lengths, key_mask, allowed = ctx.saved_tensors
+        q, k, v, out, lse, key_lengths, key_mask, allowed, seed_word = ctx.saved_tensors
         num_heads, scale, dropout_p, seed = ctx.args
         Ek = k.shape[-1] // 2
         packed = None if v is not None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
         ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
         gq, gk, gv = ops.cross_attention_train_bwd(q, ks, vs, out, grad_out, lse, num_heads, scale, key_lengths, key_mask, allowed,
                                                    dropout_p, seed,
-                                                   grads_kv=None if packed is None else (packed[..., :Ek], packed[..., Ek:]))
-        return gq, gk if packed is None else packed, gv if packed is None else None, None, None, None, None, None, None, None
+                                                   grads_kv=None if packed is None else (packed[..., :Ek], packed[..., Ek:]),
+                                                   seed_word=seed_word)
+        return (gq, gk if packed is None else packed, gv if packed is None else None) + (None,) * 8
+
+
+def _dropout_seed(like):
+    """(seed, device word or None) of one call's dropout mask.  From the CUDA generator of `like`'s device, whose state a saved and restored step
+    repeats: outside a capture its seed and offset, which moves on (mixed by splitmix64: Steele, Lea and Flood, 2014); inside one a word drawn
+    there, so that every replay draws its own.  Where a word is registered (`ops.set_i2p_seed_tensor`), that one with a seed of torch's CPU
+    generator."""
+    word = ops._I2P_SEED_REF[0]
+    if word is not None:
+        return int(torch.randint(0, 2 ** 62, (1,)).item()), word
+    if ops._on_device(like, torch.cuda.is_current_stream_capturing):
+        return 0, torch.randint(0, 2 ** 62, (1,), dtype=torch.int64, device=like.device)
+    gen = torch.cuda.default_generators[like.get_device()]
+    at = gen.get_offset()
+    gen.set_offset(at + 4)                               # philox: four numbers a step
+    z = (gen.initial_seed() + (at // 4 + 1) * 0x9E3779B97F4A7C15) & 0xFFFFFFFFFFFFFFFF
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & 0xFFFFFFFFFFFFFFFF
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & 0xFFFFFFFFFFFFFFFF
+    return z ^ (z >> 31), None
 
 
 def cross_attention_usable(q, k, num_heads):
@@ -239,11 +259,11 @@ def cross_attention_usable(q, k, num_heads):
 
 def cross_attention(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None, dropout_p=0.0):
     """`ops.cross_attention`, differentiable where a gradient is asked for; v None: k is [K | V] of one projection.  dropout_p: of the
-    attention weights, with a fresh seed from torch's CPU generator (inside a captured step: plus the word of
-    `ops.set_i2p_seed_tensor`)."""
+    attention weights, a fresh mask in every call and in every replay of a captured one (`_dropout_seed`)."""
+    ops._same_device(q)
     if dropout_p > 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v))):
-        seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if dropout_p > 0 else 0
-        return CrossAttention.apply(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+        seed, word = _dropout_seed(q) if dropout_p > 0 else (0, None)
+        return CrossAttention.apply(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, word)
     if v is None:
         k, v = k.chunk(2, -1)
     return ops.cross_attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed)

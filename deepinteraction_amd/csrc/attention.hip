@@ -175,7 +175,7 @@ static bool clear_of(const Rows &a, const Rows &b, int sz) {
   return same && (rows || groups);
 }
 
-static Args args_of(const di_attention *t) {
+static Args args_of(const di_attention *t, const unsigned long long *seed_word) {
   Args a = {};
   const int sz = t->dtype == DI_F32 ? 4 : 2;
   a.q = (const char *)t->q; a.k = (const char *)t->k; a.v = (const char *)t->v;
@@ -194,7 +194,7 @@ static Args args_of(const di_attention *t) {
   if (a.drop > 65535u) a.drop = 65535u;
   a.keep_scale = 65536.f / (float)(65536u - a.drop);
   a.seed = t->seed;
-  a.seed_ptr = i2p_seed_ptr();
+  a.seed_ptr = seed_word;
   return a;
 }
 
@@ -221,13 +221,17 @@ long long di_attention_bwd_workspace_floats(const di_attention *t) {
 }
 
 int di_attention_fwd(const di_attention *t, void *out, float *lse, float *workspace, void *stream) {
+  return di_attention_fwd_seeded(t, di::i2p_seed_ptr(), out, lse, workspace, stream);
+}
+
+int di_attention_fwd_seeded(const di_attention *t, const unsigned long long *seed_word, void *out, float *lse, float *workspace, void *stream) {
   using namespace di::at;
   if (int rc = check(t, true)) return rc;
   if (t->B == 0 || t->L == 0) return DI_OK;
   DI_REQUIRE(out != nullptr && ((uintptr_t)out & 15) == 0, "attention: the output must start on 16 bytes");
   Plan p;
   if (int rc = plan_rows(*t, true, p)) return rc;
-  Args a = args_of(t);
+  Args a = args_of(t, seed_word);
   a.o = (char *)out;
   a.lse = lse;
   if (p.splits > 1) {
@@ -242,6 +246,12 @@ int di_attention_fwd(const di_attention *t, void *out, float *lse, float *worksp
 int di_attention_bwd(const di_attention *t, const void *out, const float *lse, const void *grad_out, long long go_bs, long long go_rs,
                      void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs, long long gv_rs, float *workspace,
                      void *stream) {
+  return di_attention_bwd_seeded(t, di::i2p_seed_ptr(), out, lse, grad_out, go_bs, go_rs, gq, gk, gk_bs, gk_rs, gv, gv_bs, gv_rs, workspace, stream);
+}
+
+int di_attention_bwd_seeded(const di_attention *t, const unsigned long long *seed_word, const void *out, const float *lse, const void *grad_out,
+                            long long go_bs, long long go_rs, void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs,
+                            long long gv_rs, float *workspace, void *stream) {
   using namespace di::at;
   if (int rc = check(t, false)) return rc;
   if (t->B == 0 || (t->L == 0 && t->S == 0)) return DI_OK;
@@ -257,7 +267,7 @@ int di_attention_bwd(const di_attention *t, const void *out, const float *lse, c
   Plan p, k;
   if (int rc = plan_rows(*t, false, p)) return rc;
   if (int rc = plan_keys(*t, k)) return rc;
-  Args a = args_of(t);
+  Args a = args_of(t, seed_word);
   a.o = (char *)const_cast<void *>(out);
   a.lse = const_cast<float *>(lse);
   a.go = (const char *)grad_out;

@@ -1304,6 +1304,20 @@ def _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropou
     return t, keep
 
 
+def _seed_word(q, dropout_p, seed_word):
+    """The device word that a call with dropout adds to its seed: its own, the registered one, or None."""
+    if dropout_p == 0:
+        return None
+    own = seed_word is not None
+    word = seed_word if own else _I2P_SEED_REF[0]
+    if word is None:
+        return None
+    if word.dtype != torch.int64 or word.numel() != 1 or word.device != q.device:
+        raise ValueError(f'cross_attention: the {"" if own else "registered "}seed word is {word.dtype} {tuple(word.shape)} on {word.device}, one int64 on '
+                         f'{q.device} expected')
+    return word
+
+
 def _attention_workspace(name, ref, q):
     n = _on_device(q, lambda: getattr(_lib.lib(), name)(ref))
     if n < 0:
@@ -1311,13 +1325,18 @@ def _attention_workspace(name, ref, q):
     return q.new_empty(n, dtype=torch.float32) if n else None
 
 
-def _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, stats):
+def _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, stats, seed_word=None):
     t, keep = _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+    word = _seed_word(q, dropout_p, seed_word)
     out = q.new_empty(q.shape)
     lse = q.new_empty((t.B, t.heads, t.L), dtype=torch.float32) if stats else None
     ref = ctypes.addressof(t)
     ws = _attention_workspace('di_attention_fwd_workspace_floats', ref, q)
-    _launch('attention_fwd', t.B, q, ref, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr())
+    args = (out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr())
+    if word is None:
+        _launch('attention_fwd', t.B, q, ref, *args)
+    else:
+        _launch('attention_fwd_seeded', t.B, q, ref, word.data_ptr(), *args)
     return out, lse
 
 
@@ -1332,18 +1351,21 @@ def cross_attention(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=N
     return _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, 0.0, 0, False)[0]
 
 
-def cross_attention_train_fwd(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None, dropout_p=0.0, seed=0):
+def cross_attention_train_fwd(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None, dropout_p=0.0, seed=0,
+                              seed_word=None):
     """`cross_attention` with the per-query log2-sum-exp2 kept for the backward: (out, lse (B, heads, L)).  dropout_p: dropout of the
-    attention weights, decided per (query, head, key) by a counter-based hash of `seed` (plus the word of `set_i2p_seed_tensor`)
-    that the backward regenerates; p is rounded to a multiple of 2^-16."""
-    return _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, True)
+    attention weights, decided per (query, head, key) by a counter-based hash of `seed` plus `seed_word` (an int64 on the device, read
+    when the launch runs; None: the one of `set_i2p_seed_tensor`, if any) that the backward regenerates; p is rounded to a multiple
+    of 2^-16."""
+    return _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, True, seed_word)
 
 
 def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None,
-                              dropout_p=0.0, seed=0, grads_kv=None):
+                              dropout_p=0.0, seed=0, grads_kv=None, seed_word=None):
     """(grad_q, grad_k, grad_v) of `cross_attention_train_fwd`; the softmax is recomputed from `lse`, deterministic.  grads_kv: write
     grad_k and grad_v into these (B, S, key heads * D) tensors (halves of one packed gradient) instead of allocating them."""
     t, keep = _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed)
+    word = _seed_word(q, dropout_p, seed_word)
     _same_device(q, out, grad_out, lse, *(grads_kv or ()))
     if out.shape != q.shape or out.dtype != q.dtype or grad_out.shape != q.shape:
         raise ValueError(f'cross_attention: out {tuple(out.shape)}, grad_out {tuple(grad_out.shape)}, q {tuple(q.shape)}')
@@ -1362,8 +1384,12 @@ def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None
         k_strides, v_strides = _seq_view(gk)[1:], _seq_view(gv)[1:]
     ref = ctypes.addressof(t)
     ws = _attention_workspace('di_attention_bwd_workspace_floats', ref, q)
-    _launch('attention_bwd', t.B, q, ref, out.data_ptr(), lse.data_ptr(), go.data_ptr(), go_bs, go_rs, gq.data_ptr(),
-            gk.data_ptr(), *k_strides, gv.data_ptr(), *v_strides, 0 if ws is None else ws.data_ptr())
+    args = (out.data_ptr(), lse.data_ptr(), go.data_ptr(), go_bs, go_rs, gq.data_ptr(), gk.data_ptr(), *k_strides, gv.data_ptr(), *v_strides,
+            0 if ws is None else ws.data_ptr())
+    if word is None:
+        _launch('attention_bwd', t.B, q, ref, *args)
+    else:
+        _launch('attention_bwd_seeded', t.B, q, ref, word.data_ptr(), *args)
     return gq, gk, gv
 
 

@@ -685,7 +685,8 @@ int di_layernorm_bwd(const void *gy, long long gy_row_stride, int y_dtype, const
  *   into a product; those excluded by `allowed` enter as 0 * v and have to be finite.  A row without keys gives zeros, lse -inf and
  *   no gradient.
  *   dropout_p: attention dropout from a counter-based hash of (seed + the device word of di_i2p_set_seed_ptr, row, key), the same
- *   in forward and backward; p is rounded to a multiple of 2^-16.
+ *   in forward and backward; p is rounded to a multiple of 2^-16.  The _seeded forms take the device word (NULL: none) of the call
+ *   instead of the registered one: a forward and its backward that are captured, with a word drawn on the device inside the graph.
  * di_attention_fwd: out (B, L, heads * head_dim) dense; lse (B, heads, L) float32, log2-sum-exp2 of scale log2(e) q k (may be NULL).
  * di_attention_bwd: grad_q dense, grad_k / grad_v (B, S, kv_heads * head_dim) with strides, every row written.
  * workspace: the floats that the matching function returns (< 0: unsupported), private to the call until it has run. */
@@ -704,9 +705,13 @@ typedef struct {
 long long di_attention_fwd_workspace_floats(const di_attention *t);
 long long di_attention_bwd_workspace_floats(const di_attention *t);
 int di_attention_fwd(const di_attention *t, void *out, float *lse, float *workspace, void *stream);
+int di_attention_fwd_seeded(const di_attention *t, const unsigned long long *seed_word, void *out, float *lse, float *workspace, void *stream);
 int di_attention_bwd(const di_attention *t, const void *out, const float *lse, const void *grad_out, long long go_bs, long long go_rs,
                      void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs, long long gv_rs,
                      float *workspace, void *stream);
+int di_attention_bwd_seeded(const di_attention *t, const unsigned long long *seed_word, const void *out, const float *lse, const void *grad_out,
+                            long long go_bs, long long go_rs, void *gq, void *gk, long long gk_bs, long long gk_rs, void *gv, long long gv_bs,
+                            long long gv_rs, float *workspace, void *stream);
 
 #ifdef __cplusplus
 }

@@ -169,3 +169,13 @@ def test_key_gradients_side_by_side(change):
     if torch.cuda.is_available():
         return                                                       # the pointers must not be followed
     assert L.di_attention_bwd(ctypes.addressof(attention()), *{**GRAD, **change}.values(), None) != -1 or 'overlap' not in said()
+
+
+def test_seed_words():
+    q = torch.zeros(1, 2, 16)
+    assert ops._seed_word(q, 0.0, None) is None and ops._seed_word(q, 0.5, None) is None
+    word = torch.zeros(1, dtype=torch.int64)
+    assert ops._seed_word(q, 0.5, word) is word and ops._seed_word(q, 0.0, word) is None
+    for bad in (word.int(), torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int64, device='meta')):
+        with pytest.raises(ValueError):
+            ops._seed_word(q, 0.5, bad)

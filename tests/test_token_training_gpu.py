@@ -199,3 +199,77 @@ def test_captured_training_step_of_a_layer():
         for a, b in zip(got, step()):
             # library products may be chosen differently inside and outside a capture: a few roundings of the largest value
             assert (a is None) == (b is None) and (a is None or float((a - b).abs().max()) <= 2.0 ** -18 * max(float(b.abs().max()), 1e-6)), n
+
+
+def test_dropout_in_a_captured_step_is_fresh_in_every_replay(monkeypatch):
+    """Forward and backward of the attention in one graph: every replay has a mask of its own, the same in both directions - the one that the
+    word drawn by that replay gives - and a generator that is seeded again repeats it."""
+    q, kv, go = tokens((2, 37, 64), 'cuda', torch.float32, 0), tokens((2, 90, 128), 'cuda', torch.float32, 1), tokens((2, 37, 64), 'cuda', torch.float32, 2)
+    q, kv = q.requires_grad_(True), kv.requires_grad_(True)
+
+    def step():
+        o = autograd.cross_attention(q, kv, None, 4, dropout_p=0.4)
+        return (o.detach(),) + torch.autograd.grad(o, (q, kv), go)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    words, fwd = [], ops.cross_attention_train_fwd
+
+    def keep(*a, **k):
+        words.append(a[10])
+        return fwd(*a, **k)
+    monkeypatch.setattr(ops, 'cross_attention_train_fwd', keep)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    monkeypatch.undo()
+    assert len(words) == 1 and words[0] is not None
+    seen = []
+    with torch.no_grad():
+        k, v = kv.chunk(2, -1)
+        for n in range(4):
+            if n >= 2:
+                torch.cuda.manual_seed(11)
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in out]
+            o, lse = ops.cross_attention_train_fwd(q, k, v, 4, dropout_p=0.4, seed=0, seed_word=words[0])
+            gq, gk, gv = ops.cross_attention_train_bwd(q, k, v, o, go, lse, 4, dropout_p=0.4, seed=0, seed_word=words[0])
+            assert all(torch.equal(a, b) for a, b in zip(got, (o, gq, torch.cat((gk, gv), -1)))), n
+            seen.append((int(words[0]), got))
+    assert len({w for w, _ in seen}) == 3 and not torch.equal(seen[0][1][0], seen[1][1][0])
+    assert seen[2][0] == seen[3][0] and all(torch.equal(a, b) for a, b in zip(seen[2][1], seen[3][1]))
+
+
+def test_dropout_follows_the_cuda_generator():
+    """A saved and restored state of the device's generator repeats the mask; the CPU's generator is left alone."""
+    q, kv = tokens((2, 30, 128), 'cuda', torch.float32, 0), tokens((2, 90, 256), 'cuda', torch.float32, 1)
+    host, state = torch.get_rng_state(), torch.cuda.get_rng_state()
+    a = autograd.cross_attention(q, kv, None, 8, dropout_p=0.5)
+    b = autograd.cross_attention(q, kv, None, 8, dropout_p=0.5)
+    torch.cuda.set_rng_state(state)
+    assert torch.equal(a, autograd.cross_attention(q, kv, None, 8, dropout_p=0.5)) and not torch.equal(a, b)
+    assert torch.equal(b, autograd.cross_attention(q, kv, None, 8, dropout_p=0.5))
+    assert torch.equal(host, torch.get_rng_state())
+
+
+def test_dropout_s_backward_keeps_the_word_of_its_forward():
+    """A word that is registered for the forward alone, as around a capture, is the backward's as well."""
+    q, kv = tokens((1, 30, 64), 'cuda', torch.float32, 0).requires_grad_(True), tokens((1, 70, 128), 'cuda', torch.float32, 1)
+    word = torch.full((1,), 41, dtype=torch.int64, device='cuda')
+    grads = []
+    for cleared in (False, True):
+        torch.manual_seed(3)
+        ops.set_i2p_seed_tensor(word)
+        try:
+            o = autograd.cross_attention(q, kv, None, 4, dropout_p=0.5)
+            if cleared:
+                ops.set_i2p_seed_tensor(None)
+            grads.append(torch.autograd.grad(o, q, torch.ones_like(o))[0])
+        finally:
+            ops.set_i2p_seed_tensor(None)
+    assert torch.equal(*grads)
