@@ -25,8 +25,10 @@ graph, in place:
 No work is skipped on replay: depth scatter/completion, all gathers, attention and GEMM kernels
 are part of the graph.
 """
+import contextlib
 import queue
 import threading
+import weakref
 
 import torch
 
@@ -377,6 +379,31 @@ class GraphedHotPath:
                 mod.load_static_geometry(g, rec)
 
 
+def _lane(device, stream, jobs, done):
+    """The thread of one lane: runs the callables of `jobs` until a None."""
+    if device is not None:
+        torch.cuda.set_device(device)
+    on = torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
+    with torch.no_grad(), on:
+        while True:
+            fn = jobs.get()
+            if fn is None:
+                return
+            err = None
+            try:
+                fn()
+            except BaseException as e:             # handed to the caller of run()
+                err = e
+            fn = None                              # a waiting lane keeps no capture alive
+            done.put(err)
+            err = None
+
+
+def _end_lanes(jobs):
+    for q in jobs:
+        q.put(None)
+
+
 class LaneLaunchers:
     """One HOST THREAD per in-flight lane (a lane = a HIP stream on which captured forwards are replayed one behind the other).
 
@@ -395,29 +422,15 @@ class LaneLaunchers:
 
     def __init__(self, streams):
         self.streams = list(streams)                # (None entries: no stream switch - the host-logic tests run without a device)
-        self._device = torch.cuda.current_device() if torch.cuda.is_available() else None
+        device = torch.cuda.current_device() if torch.cuda.is_available() else None
         self._jobs = [queue.SimpleQueue() for _ in self.streams]
         self._done = queue.SimpleQueue()
-        self._threads = [threading.Thread(target=self._work, args=(l,), daemon=True, name=f'lane{l}')
-                         for l in range(len(self.streams))]
+        # (the threads hold their queues, not this object: dropping it ends them as `close` does)
+        self._threads = [threading.Thread(target=_lane, args=(device, s, jobs, self._done), daemon=True, name=f'lane{l}')
+                         for l, (s, jobs) in enumerate(zip(self.streams, self._jobs))]
+        self._end = weakref.finalize(self, _end_lanes, self._jobs)
         for t in self._threads:
             t.start()
-
-    def _work(self, l):
-        import contextlib
-        if self._device is not None:
-            torch.cuda.set_device(self._device)
-        on = torch.cuda.stream(self.streams[l]) if self.streams[l] is not None else contextlib.nullcontext()
-        with torch.no_grad(), on:
-            while True:
-                fn = self._jobs[l].get()
-                if fn is None:
-                    return
-                try:
-                    fn()
-                    self._done.put(None)
-                except BaseException as e:         # handed to the caller of run()
-                    self._done.put(e)
 
     def run(self, fns):
         assert len(fns) == len(self.streams)
@@ -431,8 +444,7 @@ class LaneLaunchers:
             raise err
 
     def close(self):
-        for q in self._jobs:
-            q.put(None)
+        self._end()
         for t in self._threads:
             t.join()
         self._threads = []

@@ -183,3 +183,37 @@ def test_msda_torch_formulation_matches_mmcv_core():
         want = tp.ms_deform_attn_core(v.view(bs, S, 8, 16), shapes, loc, w)
         assert (got - want).abs().max().item() <= 1e-5
     assert MultiScaleDeformableAttention(128, num_heads=8, num_levels=2, num_points=4).kernels_cover()
+
+
+def test_lanes_keep_no_job_and_end_with_their_pool():
+    """A waiting lane holds nothing of the callables that it ran (captures and their device memory), nor of what they raised; a pool that is
+    dropped without `close` ends its threads."""
+    import gc
+    import weakref
+    import pytest
+    from deepinteraction_amd.graphed import LaneLaunchers
+
+    class Job:
+        def __init__(self, fails=False):
+            self.fails = fails
+
+        def __call__(self):
+            if self.fails:
+                raise ValueError('failed')
+    pool = LaneLaunchers([None, None])
+    jobs = [Job(), Job()]
+    gone = [weakref.ref(j) for j in jobs]
+    pool.run(jobs)
+    jobs = [Job(), Job(fails=True)]
+    gone += [weakref.ref(j) for j in jobs]
+    with pytest.raises(ValueError):
+        pool.run(jobs)
+    del jobs
+    gc.collect()
+    assert [g() for g in gone] == [None] * 4
+    threads = pool._threads
+    del pool
+    gc.collect()
+    for t in threads:
+        t.join(10)
+    assert not any(t.is_alive() for t in threads)
