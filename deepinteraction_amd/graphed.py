@@ -26,11 +26,14 @@ No work is skipped on replay: depth scatter/completion, all gathers, attention a
 are part of the graph.
 """
 import contextlib
+import gc
 import queue
 import threading
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
+from torch.autograd.graph import get_gradient_edge
 
 from .geometry import SampleGeometry
 from .mmdet3d_plugin.models.utils.decoder_utils import QueryGeometry
@@ -377,6 +380,102 @@ class GraphedHotPath:
         for mod, recs in r.extra:
             for g, rec in zip(self.sample_geom, recs):
                 mod.load_static_geometry(g, rec)
+
+
+def accumulators_alive(params):
+    """The parameters whose gradient accumulator is held by an autograd graph that somebody keeps.  (An accumulator belongs to the graphs
+    that use it: one that nothing holds is made anew by the next look, without the mark that the last one left on it.)"""
+    alive = []
+    for p in params:
+        if not p.requires_grad:
+            continue
+        mark = object()
+        get_gradient_edge(p).node.metadata['alive'] = mark
+        if get_gradient_edge(p).node.metadata.pop('alive', None) is mark:
+            alive.append(p)
+    return alive
+
+
+def _training_pass(module, args, inputs):
+    """One forward and backward of `module`; nothing of its graph outlives the call."""
+    outs = [t for t in module(*args) if t.requires_grad]
+    torch.autograd.grad(outs, inputs, [torch.ones_like(t) for t in outs], allow_unused=True)
+
+
+class _Replayed(torch.autograd.Function):
+    """Forward and backward of a `GraphedTrainingModule`: one replay each."""
+
+    @staticmethod
+    def forward(ctx, owner, *inputs):
+        ctx.owner = owner
+        for static, t in zip(owner.args, inputs):
+            if static.data_ptr() != t.data_ptr():
+                static.copy_(t)
+        owner.forward_graph.replay()
+        outs = tuple(t.detach() for t in owner.outs)
+        ctx.mark_non_differentiable(*(t for t, live in zip(outs, owner.differentiable) if not live))
+        return outs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        owner = ctx.owner
+        live = [g for g, live in zip(grads, owner.differentiable) if live]
+        for static, g in zip(owner.grad_outs, live):
+            if static.data_ptr() != g.data_ptr():
+                static.copy_(g)
+        owner.backward_graph.replay()
+        return (None,) + tuple(None if g is None else g.detach() for g in owner.grads)
+
+
+class GraphedTrainingModule:
+    """A module that returns a tuple of tensors, its forward and its backward as two captured hipGraphs; called like the module, with
+    tensors of the shapes of `args` (the captured buffers themselves are not copied).  Outputs and gradients are the graphs' own
+    buffers: valid until the next call.
+
+    Captured while no autograd graph of the parameters is alive.  Such a graph holds their gradient accumulators, which keep the stream
+    that they were made on: the captured backward would hand its gradients over to that stream, fork onto a stream that is no part of the
+    capture, and the replay of such a graph has ended the process.  (`torch.cuda.make_graphed_callables` leaves the graph of its last warm-up
+    pass alive through its captures.)"""
+
+    def __init__(self, module, args, warmup=3):
+        self.module, self.args = module, tuple(args)
+        self.parameters = [p for p in module.parameters() if p.requires_grad]
+        inputs = [t for t in self.args if t.requires_grad] + self.parameters
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(warmup):
+                _training_pass(module, self.args, inputs)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        gc.collect()
+        held = len(accumulators_alive(inputs))
+        if held:
+            raise RuntimeError(f'an autograd graph of {held} of the {len(inputs)} parameters is alive (outputs or a loss of an earlier eager pass): '
+                               'drop it before the training step is captured')
+        pool = torch.cuda.graph_pool_handle()
+        self.forward_graph, self.backward_graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        # no garbage collection INSIDE the captures: what it frees may release device memory through calls that a capturing process may not make
+        was_enabled = gc.isenabled()
+        gc.disable()
+        try:
+            with torch.cuda.graph(self.forward_graph, pool=pool):
+                outs = tuple(module(*self.args))
+            self.differentiable = [t.requires_grad for t in outs]
+            live = [t for t in outs if t.requires_grad]
+            self.grad_outs = [torch.zeros_like(t) for t in live]
+            with torch.cuda.graph(self.backward_graph, pool=pool):
+                grads = iter(torch.autograd.grad(live, inputs, self.grad_outs, allow_unused=True))
+            self.grads = [next(grads) if t.requires_grad else None for t in self.args + tuple(self.parameters)]
+            self.outs = tuple(t.detach() for t in outs)              # the buffers, without the graph
+            del outs, live, grads
+        finally:
+            if was_enabled:
+                gc.enable()
+
+    def __call__(self, *args):
+        return _Replayed.apply(self, *args, *self.parameters)
 
 
 def _lane(device, stream, jobs, done):

@@ -204,7 +204,7 @@ class Trainer:
 
 
 class _HotPathModule(torch.nn.Module):
-    """encoder + decoder as ONE callable of the two static feature-map tensors (what `make_graphed_callables` captures):
+    """encoder + decoder as ONE callable of the two static feature-map tensors (what `graphed.GraphedTrainingModule` captures):
     points / pillars / geometry are the owner's static buffers, refreshed in place between replays."""
 
     def __init__(self, enc, dec, owner, amp=False):
@@ -229,8 +229,8 @@ class _HotPathModule(torch.nn.Module):
 
 
 class GraphedTrainer(Trainer):
-    """The training step with forward and backward of the hot path as TWO captured hipGraphs (`torch.cuda.
-    make_graphed_callables`) around the eager head loss, whose Hungarian assignment is a host round trip as in the
+    """The training step with forward and backward of the hot path as TWO captured hipGraphs
+    (`graphed.GraphedTrainingModule`) around the eager head loss, whose Hungarian assignment is a host round trip as in the
     reference.  The eager step issues ~3 000 launches from Python (52 ms of wall time for 41 ms of kernels, host-bound);
     replayed, the step is bound by its kernels.  Static input buffers, padded points / pillars and in-place geometry
     refresh are the inference graph's (`graphed.GraphedHotPath`)."""
@@ -242,7 +242,7 @@ class GraphedTrainer(Trainer):
         super().__init__(shape, num_proposals, device, world, batch=batch, pool=pool, rank=rank, seed=seed, amp=amp)
         if prepare_model is not None:
             prepare_model(self.enc, self.dec)
-        from .graphed import GraphedHotPath
+        from .graphed import GraphedHotPath, GraphedTrainingModule
         cap = max(range(len(self.pool)), key=lambda i: int(self.pool[i][0]['pts_metas']['pillars'].shape[0]))
         h = GraphedHotPath.__new__(GraphedHotPath)           # the static-buffer half of the inference graph, no capture
         h.enc, h.dec, h.glue, h.image_net, h._img_key = self.enc, self.dec, None, None, 'img_feats'
@@ -290,18 +290,10 @@ class GraphedTrainer(Trainer):
         self.seed_word = torch.zeros(1, dtype=torch.int64, device=h.img_feats.device)
         ops.set_i2p_seed_tensor(self.seed_word)
         self.module = _HotPathModule(self.enc, self.dec, h, amp=self.amp)
-        # no garbage collection INSIDE the captures: a collected autograd graph of a warm-up iteration (Python Function nodes are
-        # freed by the collector, not by reference counting) releases device memory through calls a capturing process may not make
-        import gc
-        gc.collect()
-        was_enabled = gc.isenabled()
-        gc.disable()
         try:
-            self.graphed = torch.cuda.make_graphed_callables(self.module, (h.img_feats, h.pts_feats), allow_unused_input=True)
+            self.graphed = GraphedTrainingModule(self.module, (h.img_feats, h.pts_feats))
         finally:
             ops.set_i2p_seed_tensor(None)
-            if was_enabled:
-                gc.enable()
 
     def step(self):
         i = self.i % len(self.pool)
