@@ -102,11 +102,11 @@ SIGNATURES = {
 # helpers that return a value instead of an error code
 VALUE_FUNCS = {'di_mha_decode_scratch_floats': [_c_i] * 4, 'di_i2p_key_table_bytes': [_c_i] * 4, 'di_i2p_dense_bytes': [_c_i] * 5, 'di_topk_workspace_bytes': [_c_i] * 3,
                'di_token_splitk_workspace_bytes': [_c_i] * 2, 'di_mha_decode_x_ranges': [_c_i] * 3,
-               'di_graph_node_count': [_c_p], 'di_local_attn_ring_timeouts': [_c_p], 'di_bn_workspace_floats': [_c_i],
+               'di_graph_node_count': [_c_p], 'di_graph_fill_by_kernels': [_c_p, _c_i], 'di_local_attn_ring_timeouts': [_c_p], 'di_bn_workspace_floats': [_c_i],
                'di_layernorm_bwd_workspace_floats': [_c_ll, _c_i],
                'di_attention_fwd_workspace_floats': [_c_p], 'di_attention_bwd_workspace_floats': [_c_p],
                'di_timed_consumed': [], 'di_wgrad_workspace_floats': [ctypes.c_longlong, _c_i, _c_i]}
-_LONGLONG = {'di_attention_fwd_workspace_floats', 'di_attention_bwd_workspace_floats', 'di_layernorm_bwd_workspace_floats', 'di_i2p_dense_bytes', 'di_wgrad_workspace_floats', 'di_topk_workspace_bytes', 'di_i2p_key_table_bytes', 'di_graph_node_count', 'di_token_splitk_workspace_bytes'}
+_LONGLONG = {'di_graph_fill_by_kernels', 'di_attention_fwd_workspace_floats', 'di_attention_bwd_workspace_floats', 'di_layernorm_bwd_workspace_floats', 'di_i2p_dense_bytes', 'di_wgrad_workspace_floats', 'di_topk_workspace_bytes', 'di_i2p_key_table_bytes', 'di_graph_node_count', 'di_token_splitk_workspace_bytes'}
 
 # ---- the step program of di_token_program (structs of include/deepinteraction_hip.h)
 TOK_LOAD, TOK_LOAD_PARTS, TOK_ATTN, TOK_COMBINE, TOK_LINEAR, TOK_ROWOP, TOK_STORE, TOK_HEADS = range(1, 9)

@@ -3,6 +3,8 @@
 
 #include <stdlib.h>
 
+#include <vector>
+
 #include "di_common.h"
 
 namespace di {
@@ -47,6 +49,72 @@ long long di_graph_node_count(void *graph) {
   }
   return (long long)n;
 }
+}
+
+namespace di {
+
+// rows of `width` bytes, `pitch` apart, filled with a value of 1, 2 or 4 bytes: by words where they start on words
+__global__ __launch_bounds__(256) void graph_fill_kernel(unsigned char *dst, size_t pitch, size_t width, size_t height, unsigned value, unsigned size) {
+  const bool words = (((uintptr_t)dst | pitch | width) & 3) == 0;
+  const unsigned all = size == 4 ? value : size == 2 ? (value & 0xffffu) * 0x10001u : (value & 0xffu) * 0x01010101u;
+  const size_t per = words ? width / 4 : width, n = per * height, step = (size_t)gridDim.x * 256;
+  for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < n; e += step) {
+    const size_t row = e / per, col = e - row * per;
+    if (words) *reinterpret_cast<unsigned *>(dst + row * pitch + 4 * col) = all;
+    else dst[row * pitch + col] = (unsigned char)(all >> (8 * (col % size)));
+  }
+}
+
+// one memset node of `graph` -> a kernel node in its place
+static hipError_t fill_by_kernel(hipGraph_t graph, hipGraphNode_t node) {
+  hipMemsetParams m = {};
+  hipError_t e = hipGraphMemsetNodeGetParams(node, &m);
+  if (e != hipSuccess) return e;
+  size_t before = 0, after = 0;
+  if ((e = hipGraphNodeGetDependencies(node, nullptr, &before)) != hipSuccess) return e;
+  if ((e = hipGraphNodeGetDependentNodes(node, nullptr, &after)) != hipSuccess) return e;
+  std::vector<hipGraphNode_t> from(before), to(after), self(after);
+  if (before > 0 && (e = hipGraphNodeGetDependencies(node, from.data(), &before)) != hipSuccess) return e;
+  if (after > 0 && (e = hipGraphNodeGetDependentNodes(node, to.data(), &after)) != hipSuccess) return e;
+  unsigned char *dst = (unsigned char *)m.dst;
+  size_t width = m.width * m.elementSize, height = m.height > 1 ? m.height : 1, pitch = height > 1 ? m.pitch : width;
+  unsigned value = m.value, size = m.elementSize;
+  const size_t work = width * height / 4 + 1, blocks = (work + 255) / 256;
+  void *args[] = {&dst, &pitch, &width, &height, &value, &size};
+  hipKernelNodeParams k = {};
+  k.func = (void *)graph_fill_kernel;
+  k.gridDim = dim3((unsigned)(blocks < 1024 ? blocks : 1024));
+  k.blockDim = dim3(256);
+  k.kernelParams = args;
+  hipGraphNode_t fill;
+  if ((e = hipGraphAddKernelNode(&fill, graph, from.data(), before, &k)) != hipSuccess) return e;
+  for (hipGraphNode_t &s : self) s = fill;
+  if (after > 0 && (e = hipGraphAddDependencies(graph, self.data(), to.data(), after)) != hipSuccess) return e;
+  return hipGraphDestroyNode(node);
+}
+
+}  // namespace di
+
+extern "C" long long di_graph_fill_by_kernels(void *graph, int replace) {
+  hipGraph_t g = (hipGraph_t)graph;
+  size_t n = 0;
+  hipError_t e = graph == nullptr ? hipErrorInvalidValue : hipGraphGetNodes(g, nullptr, &n);
+  std::vector<hipGraphNode_t> nodes(n);
+  if (e == hipSuccess && n > 0) e = hipGraphGetNodes(g, nodes.data(), &n);
+  long long found = 0;
+  for (size_t i = 0; i < n && e == hipSuccess; ++i) {
+    hipGraphNodeType type;
+    if ((e = hipGraphNodeGetType(nodes[i], &type)) != hipSuccess) break;
+    if (type != hipGraphNodeTypeMemset) continue;
+    ++found;
+    if (replace != 0) e = di::fill_by_kernel(g, nodes[i]);
+  }
+  if (e != hipSuccess) {
+    di::set_error("graph_fill_by_kernels: %s", hipGetErrorString(e));
+    (void)hipGetLastError();
+    return DI_ERR_LAUNCH;
+  }
+  return found;
 }
 
 namespace di {

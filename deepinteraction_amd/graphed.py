@@ -402,6 +402,18 @@ def _training_pass(module, args, inputs):
     torch.autograd.grad(outs, inputs, [torch.ones_like(t) for t in outs], allow_unused=True)
 
 
+def _without_memsets(graph):
+    """Instantiates a captured `torch.cuda.CUDAGraph(keep_graph=True)` with kernels in place of its memset nodes.  torch's sums over many rows
+    (the gradient of a bias) clear their counters with such nodes, and every replay after the first has returned wrong sums
+    (tests/test_graphed_training_gpu.py)."""
+    from . import _lib
+    n = int(_lib.lib().di_graph_fill_by_kernels(int(graph.raw_cuda_graph()), 1))
+    if n < 0:
+        raise _lib.HipLibraryError(f'di_graph_fill_by_kernels: {_lib.lib().di_last_error().decode()}')
+    graph.instantiate()
+    return graph
+
+
 class _Replayed(torch.autograd.Function):
     """Forward and backward of a `GraphedTrainingModule`: one replay each."""
 
@@ -436,7 +448,7 @@ class GraphedTrainingModule:
     Captured while no autograd graph of the parameters is alive.  Such a graph holds their gradient accumulators, which keep the stream
     that they were made on: the captured backward would hand its gradients over to that stream, fork onto a stream that is no part of the
     capture, and the replay of such a graph has ended the process.  (`torch.cuda.make_graphed_callables` leaves the graph of its last warm-up
-    pass alive through its captures.)"""
+    pass alive through its captures.)  Memset nodes: `_without_memsets`."""
 
     def __init__(self, module, args, warmup=3):
         self.module, self.args = module, tuple(args)
@@ -455,7 +467,7 @@ class GraphedTrainingModule:
             raise RuntimeError(f'an autograd graph of {held} of the {len(inputs)} parameters is alive (outputs or a loss of an earlier eager pass): '
                                'drop it before the training step is captured')
         pool = torch.cuda.graph_pool_handle()
-        self.forward_graph, self.backward_graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        self.forward_graph, self.backward_graph = torch.cuda.CUDAGraph(keep_graph=True), torch.cuda.CUDAGraph(keep_graph=True)
         # no garbage collection INSIDE the captures: what it frees may release device memory through calls that a capturing process may not make
         was_enabled = gc.isenabled()
         gc.disable()
@@ -473,6 +485,8 @@ class GraphedTrainingModule:
         finally:
             if was_enabled:
                 gc.enable()
+        _without_memsets(self.forward_graph)
+        _without_memsets(self.backward_graph)
 
     def __call__(self, *args):
         return _Replayed.apply(self, *args, *self.parameters)

@@ -58,6 +58,10 @@ const char *di_last_error(void);
 /* Measurement plumbing: number of nodes of a captured hipGraph_t (HOST handle), < 0 on error.  bench.py reports
  * it as `graph_nodes` of the captured forward. */
 long long di_graph_node_count(void *graph_host);
+/* The memset nodes of a captured hipGraph_t (HOST handle, not yet instantiated), each replaced by a kernel node that fills the same
+ * memory (replace != 0) or only counted; returns their number, < 0 on error.  Library reductions over many workgroups record such
+ * nodes to clear their counters, and graphs that hold them have given wrong sums on replays after the first. */
+long long di_graph_fill_by_kernels(void *graph_host, int replace);
 
 /* ---------------------------------------------------------------- local-window attention
  * Fused forward of LocalContextAttentionBlock.forward (encoder_utils.py:132-134):

@@ -5,6 +5,7 @@ import contextlib
 import pytest
 import torch
 
+from deepinteraction_amd import graphed
 from deepinteraction_amd.graphed import GraphedTrainingModule, accumulators_alive
 
 
@@ -26,7 +27,8 @@ class Stream:
 class Graph:
     """A graph whose replay does nothing: the buffers keep what the capture left in them."""
 
-    def __init__(self):
+    def __init__(self, keep_graph=False):
+        assert keep_graph
         self.replays = 0
 
     def replay(self):
@@ -38,6 +40,7 @@ def eager_cuda(monkeypatch):
     for name, value in dict(Stream=Stream, stream=nothing, current_stream=Stream, synchronize=lambda *a: None, CUDAGraph=Graph, graph=nothing,
                             graph_pool_handle=lambda: (0, 0)).items():
         monkeypatch.setattr(torch.cuda, name, value)
+    monkeypatch.setattr(graphed, '_without_memsets', lambda graph: graph)
 
 
 class Layer(torch.nn.Module):
