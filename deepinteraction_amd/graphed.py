@@ -179,8 +179,9 @@ class GraphedHotPath:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         # node count of the captured forward (measurement only): a throw-away capture that keeps the hipGraph_t, then
-        # the real one (a graph object created with keep_graph=True re-instantiates on replay with this torch build)
-        self._nodes = None
+        # the real one (a graph object created with keep_graph=True re-instantiates on replay with this torch build, unless it has been
+        # instantiated by hand: `_without_memsets`, for the captures that hold such nodes)
+        self._nodes, memsets = None, 1
         try:
             import os
             if os.environ.get('DI_GRAPH_NODES', '1') == '0':
@@ -191,13 +192,16 @@ class GraphedHotPath:
                 self._forward()
             n = int(_lib.lib().di_graph_node_count(int(probe.raw_cuda_graph())))
             self._nodes = n if n >= 0 else None
+            memsets = int(_lib.lib().di_graph_fill_by_kernels(int(probe.raw_cuda_graph()), 0))
             probe.reset()
             del probe
         except Exception:      # a torch build without raw graph access just reports None
             self._nodes = None
-        self.graph = torch.cuda.CUDAGraph()
+        self.graph = torch.cuda.CUDAGraph(keep_graph=memsets != 0)
         with torch.no_grad(), torch.cuda.graph(self.graph):
             self.out = self._forward()
+        if memsets != 0:
+            _without_memsets(self.graph)
 
     def check_health(self, stream=None):
         """Synchronises `stream` (default: the current one; InflightLanes passes the lane's) and raises when a captured
