@@ -16,10 +16,18 @@ from ....utils import param_key
 _NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
+def _only_a_layer_norm(norm):
+    """Whether calling the module is its LayerNorm and nothing else: no hooks (its own or global ones), no forward of a subclass or of
+    the instance."""
+    return (isinstance(norm, nn.LayerNorm) and type(norm).forward is nn.LayerNorm.forward and 'forward' not in vars(norm)
+            and not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks)
+            and not nn.modules.module._has_any_global_hook())
+
+
 def _norm_type(norm, x, branch):
     """The type of `norm(x + branch)` where the LayerNorm kernels take it, None elsewhere: autocast evaluates the norm in float32
     whatever its operands are; without it the operands' common type has to be the norm's own."""
-    if not (x.is_cuda and isinstance(norm, nn.LayerNorm) and norm.elementwise_affine and norm.bias is not None
+    if not (x.is_cuda and _only_a_layer_norm(norm) and norm.elementwise_affine and norm.bias is not None
             and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= ops.LAYERNORM_MAX_C
             and (branch is None or branch.shape == x.shape)):
         return None

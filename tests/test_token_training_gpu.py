@@ -273,3 +273,26 @@ def test_dropout_s_backward_keeps_the_word_of_its_forward():
         finally:
             ops.set_i2p_seed_tensor(None)
     assert torch.equal(*grads)
+
+
+def test_hooks_and_subclasses_of_the_norms_are_called():
+    """`post_norm` is the module's call for every norm that is more than its LayerNorm."""
+    x, branch = tokens((2, 9, 128), 'cuda', torch.float32, 0).requires_grad_(True), tokens((2, 9, 128), 'cuda', torch.float32, 1)
+    norm, seen = torch.nn.LayerNorm(128).cuda(), []
+    want = tb.post_norm(norm, x, branch)
+    for register in (norm.register_forward_hook, norm.register_forward_pre_hook, norm.register_full_backward_hook, norm.register_full_backward_pre_hook,
+                     torch.nn.modules.module.register_module_forward_hook):
+        handle = register(lambda *a: seen.append(register.__name__))
+        out = tb.post_norm(norm, x, branch)
+        out.sum().backward()
+        handle.remove()
+        assert seen and set(seen) == {register.__name__} and torch.allclose(out, want, atol=1e-5), register.__name__
+        seen.clear()
+
+    class Twice(torch.nn.LayerNorm):
+        def forward(self, x):
+            return 2 * super().forward(x)
+    assert torch.allclose(tb.post_norm(Twice(128).cuda(), x, branch), 2 * want, atol=1e-5)
+    patched = torch.nn.LayerNorm(128).cuda()
+    patched.forward = lambda x: x * 0
+    assert not tb.post_norm(patched, x, branch).any()
