@@ -6,6 +6,7 @@ predictions, exactly as in the reference (F.grid_sample's grid at encoder_utils.
 data; the RoI boxes come from deep-copied, decoded predictions, decoder_utils.py:672-679)."""
 import torch
 from torch.amp import custom_bwd, custom_fwd
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -250,9 +251,18 @@ def _dropout_seed(like):
     return z ^ (z >> 31), None
 
 
-def cross_attention_usable(q, k, num_heads):
+def transformed(*tensors):
+    """Whether torch.func's transforms or forward-mode differentiation act on a call: they know torch's own operations only."""
+    if torch._C._are_functorch_transforms_active():
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def cross_attention_usable(q, k, num_heads, v=None, dropout_p=0.0):
     """Whether `cross_attention` takes these projections: on the GPU, one of float32 / float16 / bfloat16, a head dim of 8 .. 128 in
-    steps of 8."""
+    steps of 8, weights that are not all dropped, outside of torch's transforms."""
+    if transformed(q, k, v) or not dropout_p < 1:
+        return False
     D = q.shape[-1] // num_heads
     return q.is_cuda and q.dtype == k.dtype and q.dtype in (torch.float32, torch.float16, torch.bfloat16) and D % 8 == 0 and 8 <= D <= 128
 

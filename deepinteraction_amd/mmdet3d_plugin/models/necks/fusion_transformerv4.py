@@ -150,7 +150,7 @@ class PackedMHA(nn.Module):
         if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (v is not None and v.requires_grad))):
             return ops.mha_small(q, *(k.chunk(2, -1) if v is None else (k, v)), self.num_heads)
         # training; attention dropout as in FlashAttention(attention_dropout=dropout)
-        if cross_attention_usable(q, k, self.num_heads):
+        if cross_attention_usable(q, k, self.num_heads, v, self.dropout if self.training else 0.0):
             return cross_attention(q, k, v, self.num_heads, dropout_p=self.dropout if self.training else 0.0)
         # scores materialised per (sequence, head) through library GEMMs and their autograd
         if v is None:

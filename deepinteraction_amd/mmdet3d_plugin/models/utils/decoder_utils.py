@@ -154,7 +154,7 @@ def mha_tokens(q_in, k_in, v_in, w, b, out_proj, H, dropout_p=0.0, key_allowed=N
         q = F.linear(q_in, w[:E], b[:E])
         k = F.linear(k_in, w[E:2 * E], b[E:2 * E])
         v = F.linear(v_in, w[2 * E:], b[2 * E:])
-    if cross_attention_usable(q, k, H):
+    if cross_attention_usable(q, k, H, v, dropout_p):
         return out_proj(cross_attention(q, k, v, H, allowed=key_allowed, dropout_p=dropout_p))
     q = q.view(B, L, H, D).transpose(1, 2) * (float(D) ** -0.5)
     k = k.view(B, S, H, D).transpose(1, 2)
@@ -225,7 +225,7 @@ class TransformerDecoderLayer(nn.Module):
             kv = F.linear(kin, ca.in_proj_weight[E:], ca.in_proj_bias[E:])     # (B,Pk,2C) = [K | V]
         if x.is_cuda and not (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad)):
             o = ops.mha_decode(q, kv, ca.num_heads, float(ca.head_dim) ** -0.5)
-        elif cross_attention_usable(q, kv, ca.num_heads):
+        elif cross_attention_usable(q, kv, ca.num_heads, None, ca.dropout if self.training else 0.0):
             # training: one pass over the keys per direction, the (B,H,Q,32400) scores (:471-485) never reach memory
             o = cross_attention(q, kv, None, ca.num_heads, dropout_p=ca.dropout if self.training else 0.0)
         else:

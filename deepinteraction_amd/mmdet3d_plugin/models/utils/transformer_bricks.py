@@ -9,7 +9,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .... import ops
-from ....autograd import AddLayerNorm, MSDeformAttn
+from ....autograd import AddLayerNorm, MSDeformAttn, transformed
 from ....utils import param_key
 
 
@@ -29,7 +29,7 @@ def _norm_type(norm, x, branch):
     whatever its operands are; without it the operands' common type has to be the norm's own."""
     if not (x.is_cuda and _only_a_layer_norm(norm) and norm.elementwise_affine and norm.bias is not None
             and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= ops.LAYERNORM_MAX_C
-            and (branch is None or branch.shape == x.shape)):
+            and (branch is None or branch.shape == x.shape) and not transformed(x, branch, norm.weight, norm.bias)):
         return None
     halves = {t for t in (x.dtype, x.dtype if branch is None else branch.dtype, norm.weight.dtype) if t != torch.float32}
     if len(halves) > 1 or not halves <= set(_NORM_TYPES) or norm.weight.dtype != norm.bias.dtype:

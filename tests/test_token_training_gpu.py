@@ -296,3 +296,37 @@ def test_hooks_and_subclasses_of_the_norms_are_called():
     patched = torch.nn.LayerNorm(128).cuda()
     patched.forward = lambda x: x * 0
     assert not tb.post_norm(patched, x, branch).any()
+
+
+def test_transforms_and_forward_mode_pass_the_modules():
+    """torch.func's transforms and forward-mode differentiation of the attention and norm steps, as torch's own operations have them: against
+    the float64 modules on the CPU (float32 chains of a dozen operations: 2^-16 of the largest value, or of 1.  The functional's gradient is
+    a difference: with y = h, d sum y^2 = 2 rstd (h - h mean h^2) = 2 rstd h eps / (var + eps), about 1e-5, of terms 2 rstd h of 1 and more)."""
+    torch.manual_seed(3)
+    m = du.MultiheadAttention(128, 8).train()
+    norm = torch.nn.LayerNorm(128)
+    x, dx = tokens((3, 20, 128), 'cpu', torch.float64, 0), tokens((3, 20, 128), 'cpu', torch.float64, 1)
+
+    def run(dev, dtype):
+        a, n = copy.deepcopy(m).to(dev, dtype), copy.deepcopy(norm).to(dev, dtype)
+        f = lambda t: tb.post_norm(n, t, du.mha_tokens(t, t, t, a.in_proj_weight, a.in_proj_bias, a.out_proj, 8))
+        t, dt = x.to(dev, dtype), dx.to(dev, dtype)
+        out = list(torch.func.jvp(f, (t,), (dt,)))
+        out.append(torch.func.grad(lambda t: f(t).square().sum())(t))
+        out.append(torch.func.vmap(lambda t: f(t[None])[0])(t))
+        with torch.autograd.forward_ad.dual_level():
+            out.append(torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(t, dt))).tangent)
+        return [o.detach().double().cpu() for o in out]
+    for got, want in zip(run('cuda', torch.float32), run('cpu', torch.float64)):
+        assert float((got - want).abs().max()) <= 2.0 ** -16 * max(float(want.abs().max()), 1.0)
+
+
+def test_everything_dropped():
+    """A dropout of 1, which torch's functions allow: out_proj's bias, and no gradient."""
+    torch.manual_seed(4)
+    m = du.MultiheadAttention(64, 4).cuda()
+    x = tokens((2, 9, 64), 'cuda', torch.float32, 0).requires_grad_(True)
+    y = du.mha_tokens(x, x, x, m.in_proj_weight, m.in_proj_bias, m.out_proj, 4, 1.0)
+    assert torch.allclose(y, m.out_proj.bias.expand_as(y), atol=1e-6)
+    y.sum().backward()
+    assert not x.grad.any()
