@@ -7,7 +7,6 @@ data; the RoI boxes come from deep-copied, decoded predictions, decoder_utils.py
 import torch
 from torch.amp import custom_bwd, custom_fwd
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -170,6 +169,15 @@ class I2PAttention(torch.autograd.Function):
         return g_img.to(img.dtype), g_q.to(qfold.dtype), None, None, None, None, None, None, None, None, None
 
 
+def _formula_grads(formula, inputs, needs, grad_out):
+    """Gradients of formula(*inputs) that can be differentiated again (a backward with create_graph): through torch's operations on views
+    of the inputs, so that each gradient is its own input's share even where one input was computed from another."""
+    with torch.enable_grad(), torch.autocast('cuda', enabled=False):
+        views = [t.view_as(t) if need else t for t, need in zip(inputs, needs)]
+        grads = iter(torch.autograd.grad(formula(*views), [t for t, need in zip(views, needs) if need], grad_out, create_graph=True, allow_unused=True))
+    return [next(grads) if need else None for need in needs]
+
+
 class AddLayerNorm(torch.autograd.Function):
     """y = LayerNorm(x + res) (csrc/layernorm.hip, layernorm_bwd.hip; res may be None), or (y, x + res) with `with_sum`: the post-norm
     and pre-norm steps of a training forward.  x and res are kept, not their sum; with_sum keeps the sum instead."""
@@ -179,14 +187,36 @@ class AddLayerNorm(torch.autograd.Function):
     def forward(ctx, x, res, weight, bias, eps, out_dtype, with_sum):
         y, total, mean, rstd = ops.layernorm_train_fwd(x, weight, bias, res, eps, with_sum, out_dtype)
         ctx.save_for_backward(x if total is None else total, res if total is None else None, weight, mean, rstd)
-        ctx.types = (x.dtype, None if res is None else res.dtype)
+        ctx.types, ctx.eps = (x.dtype, None if res is None else res.dtype), eps
         ctx.set_materialize_grads(False)
         return (y, total) if with_sum else y
 
     @staticmethod
-    @once_differentiable
+    def _formula_backward(ctx, gy, gsum):
+        """`backward` for create_graph: through the formula (float32, as the kernels)."""
+        x, res, weight, _, _ = ctx.saved_tensors
+        xt, rt = ctx.types
+        need = ctx.needs_input_grad
+        both = rt is not None and res is None                      # x is the sum: its gradient is the residual's as well
+        wants = [need[0] or (both and need[1]), res is not None and need[1], need[2]]
+        gx = gres = gw = gb = None
+        if gy is not None:
+            def formula(x, res, weight):
+                s = x.float() if res is None else x.float() + res.float()
+                return torch.nn.functional.layer_norm(s, s.shape[-1:], weight.float(), None, ctx.eps)
+            gx, gres, gw = _formula_grads(formula, (x, res, weight), wants, gy.float())
+            gb = gy.float().reshape(-1, gy.shape[-1]).sum(0).to(weight.dtype) if need[3] else None
+        if gsum is not None:
+            gx = gsum if gx is None else gx + gsum
+        if both and need[1] and gx is not None:
+            gres = gx.to(rt)
+        return gx.to(xt) if need[0] and gx is not None else None, gres, gw, gb, None, None, None
+
+    @staticmethod
     @_bwd
     def backward(ctx, gy, gsum=None):
+        if torch.is_grad_enabled():
+            return AddLayerNorm._formula_backward(ctx, gy, gsum)
         x, res, weight, mean, rstd = ctx.saved_tensors
         xt, rt = ctx.types
         need = ctx.needs_input_grad
@@ -217,11 +247,15 @@ class CrossAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     @_bwd
     def backward(ctx, grad_out):
         q, k, v, out, lse, key_lengths, key_mask, allowed, seed_word = ctx.saved_tensors
         num_heads, scale, dropout_p, seed = ctx.args
+        if torch.is_grad_enabled():                                # create_graph: through the formula
+            def formula(q, k, v):
+                return attention_formula(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, seed_word)
+            need = [t is not None and n for t, n in zip((q, k, v), ctx.needs_input_grad)]
+            return tuple(_formula_grads(formula, (q, k, v), need, grad_out)) + (None,) * 8
         Ek = k.shape[-1] // 2
         packed = None if v is not None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
         ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
@@ -230,6 +264,55 @@ class CrossAttention(torch.autograd.Function):
                                                    grads_kv=None if packed is None else (packed[..., :Ek], packed[..., Ek:]),
                                                    seed_word=seed_word)
         return (gq, gk if packed is None else packed, gv if packed is None else None) + (None,) * 8
+
+
+def _dropout_factors(B, H, L, S, p, seed, seed_word, device):
+    """(B, H, L, S) float32: 0 or the reciprocal of the kept share - the decisions of csrc/attention.h's hash, in torch's operations."""
+    M = 0xFFFFFFFF
+
+    def mix(x):
+        x = ((x ^ (x >> 16)) * 0x7FEB352D) & M
+        x = ((x ^ (x >> 15)) * 0x846CA68B) & M
+        return x ^ (x >> 16)
+    seed = seed & 0xFFFFFFFFFFFFFFFF
+    seed = torch.full((1,), seed - (1 << 64) if seed >> 63 else seed, dtype=torch.int64, device=device)
+    if seed_word is not None:
+        seed = seed + seed_word
+    row = torch.arange(B * H * L, device=device)
+    h = mix(mix(((seed & M) + (row & M) * 0x9E3779B9) & M) ^ ((seed >> 32) & M) ^ (((row >> 32) * 0x85EBCA6B) & M))[:, None]
+    x = mix(h ^ (torch.arange((S + 3) // 4, device=device) * 0xC2B2AE35 & M))
+    y = mix((x + 0x68BC21EB) & M)
+    numbers = torch.stack((x & 0xFFFF, x >> 16, y & 0xFFFF, y >> 16), -1).view(B, H, L, -1)[..., :S]
+    drop = min(int(p * 65536 + 0.5), 65535)
+    return (numbers >= drop).float() * (65536 / (65536 - drop))
+
+
+def attention_formula(q, k, v, num_heads, scale=None, key_lengths=None, key_mask=None, allowed=None, dropout_p=0.0, seed=0, seed_word=None):
+    """What `ops.cross_attention_train_fwd` computes, in torch's operations (float32, scores materialised) and differentiable as often as
+    those are; v None: k is [K | V]."""
+    if v is None:
+        k, v = k.chunk(2, -1)
+    (B, L, E), S = q.shape, k.shape[1]
+    D = E // num_heads
+    Hk = k.shape[-1] // D
+    G = num_heads // Hk
+    keep = torch.ones((B, 1, S), dtype=torch.bool, device=q.device)
+    if key_lengths is not None:
+        keep = keep & (torch.arange(S, device=q.device) < key_lengths[:, None])[:, None]
+    if key_mask is not None:
+        keep = keep & (key_mask != 0)[:, None]
+    zero = q.new_zeros((), dtype=torch.float32)
+    kh, vh = (torch.where(keep.view(B, 1, S, 1), t.float().view(B, S, Hk, D).transpose(1, 2), zero) for t in (k, v))       # whatever lies there
+    if allowed is not None:
+        keep = keep & (allowed != 0)
+    some = keep.any(-1).view(B, 1, 1, -1, 1)                           # rows with a key at all: the others are zeros, whatever they hold
+    qh = torch.where(some, q.float().view(B, L, Hk, G, D).permute(0, 2, 3, 1, 4), zero).reshape(B, Hk, G * L, D)
+    s = torch.matmul(qh, kh.transpose(-1, -2).contiguous()).view(B, Hk, G, L, S) * (D ** -0.5 if scale is None else scale)
+    a = torch.softmax(s.masked_fill(~(keep[:, None, None] | ~some), float('-inf')), -1)
+    if dropout_p > 0:
+        a = a * _dropout_factors(B, num_heads, L, S, dropout_p, seed, seed_word, q.device).view(B, Hk, G, L, S)
+    o = torch.matmul(a.view(B, Hk, G * L, S), vh).view(B, Hk, G, L, D)
+    return torch.where(some, o, zero).permute(0, 3, 1, 2, 4).reshape(B, L, E).to(q.dtype)
 
 
 def _dropout_seed(like):

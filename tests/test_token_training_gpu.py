@@ -330,3 +330,71 @@ def test_everything_dropped():
     assert torch.allclose(y, m.out_proj.bias.expand_as(y), atol=1e-6)
     y.sum().backward()
     assert not x.grad.any()
+
+
+def second_order(f, inputs, seed):
+    """[outputs, gradients, gradients of a functional of the gradients] of f(*inputs), every input a leaf."""
+    leaves = [t.detach().clone().requires_grad_(True) for t in inputs]
+    outs = f(*leaves)
+    dt, dev = leaves[0].dtype, leaves[0].device
+    gos = [tokens(o.shape, dev, dt, seed + i).requires_grad_(True) for i, o in enumerate(outs)]
+    grads = torch.autograd.grad(outs, leaves, gos, create_graph=True)
+    total = sum((g * tokens(g.shape, dev, dt, seed + 10 + i)).sum() for i, g in enumerate(grads))
+    again = torch.autograd.grad(total, leaves + gos, allow_unused=True)
+    return [t.detach().double().cpu() for t in list(outs) + list(grads)] + [None if t is None else t.double().cpu() for t in again]
+
+
+def test_gradients_of_gradients():
+    """create_graph through both Functions, against float64: float32 sums of up to a hundred terms, twice - 2^-14 of the largest value."""
+    B, L, S, H, Hk, D = 2, 9, 30, 4, 2, 16
+    lengths = torch.tensor([30, 11])
+    allowed = torch.rand(B, L, S, generator=torch.Generator().manual_seed(0)) < 0.7
+    allowed[:, 3] = False
+    keep = allowed & (torch.arange(S) < lengths[:, None])[:, None]
+
+    def plain(q, k, v):
+        qh, kh, vh = q.view(B, L, H, D).transpose(1, 2), k.view(B, S, Hk, D).transpose(1, 2), v.view(B, S, Hk, D).transpose(1, 2)
+        s = torch.matmul(qh, kh.repeat_interleave(H // Hk, 1).transpose(-1, -2)) * 0.3
+        s = torch.where(keep.any(-1)[:, None, :, None], s.masked_fill(~keep[:, None], float('-inf')), torch.zeros_like(s))
+        a = torch.softmax(s, -1) * keep[:, None]
+        return (torch.matmul(a, vh.repeat_interleave(H // Hk, 1)).transpose(1, 2).reshape(B, L, -1),)
+
+    def own(q, k, v):
+        return (autograd.cross_attention(q, k, v, H, 0.3, lengths.cuda().int(), None, allowed.cuda()),)
+    cases = [(plain, own, [(B, L, H * D), (B, S, Hk * D), (B, S, Hk * D)]),
+             (lambda q, kv: plain(q, *kv.chunk(2, -1)), lambda q, kv: (autograd.cross_attention(q, kv, None, H, 0.3, lengths.cuda().int(), None, allowed.cuda()),),
+              [(B, L, H * D), (B, S, 2 * Hk * D)])]
+    ln = torch.nn.functional.layer_norm
+    cases += [(lambda x, r, w, b: (ln(x + r, (24,), w, b, 1e-3),), lambda x, r, w, b: (autograd.AddLayerNorm.apply(x, r, w, b, 1e-3, None, False),),
+               [(5, 7, 24), (5, 7, 24), (24,), (24,)]),
+              (lambda x, w, b: (ln(x, (24,), w, b, 1e-3),), lambda x, w, b: (autograd.AddLayerNorm.apply(x, None, w, b, 1e-3, None, False),),
+               [(5, 7, 24), (24,), (24,)]),
+              (lambda x, r, w, b: (ln(x + r, (24,), w, b, 1e-3), x + r), lambda x, r, w, b: autograd.AddLayerNorm.apply(x, r, w, b, 1e-3, None, True),
+               [(5, 7, 24), (5, 7, 24), (24,), (24,)]),
+              # an input that another one is computed from
+              (lambda x, w, b: (ln(x + x * x, (24,), w, b, 1e-3),), lambda x, w, b: (autograd.AddLayerNorm.apply(x, x * x, w, b, 1e-3, None, False),),
+               [(5, 7, 24), (24,), (24,)])]
+    for n, (f64, f, shapes) in enumerate(cases):
+        inputs = [tokens(s, 'cpu', torch.float64, i) for i, s in enumerate(shapes)]
+        want, got = second_order(f64, inputs, 20), second_order(f, [t.float().cuda() for t in inputs], 20)
+        for i, (a, b) in enumerate(zip(got, want)):
+            if a is None or b is None:
+                assert all(t is None or not t.any() for t in (a, b)), (n, i)
+            else:
+                assert float((a - b).abs().max()) <= 2.0 ** -14 * max(float(b.abs().max()), 1.0), (n, i, float((a - b).abs().max()), float(b.abs().max()))
+
+
+def test_the_formula_s_dropout_is_the_kernel_s():
+    """The gradients of a backward with create_graph, which torch's operations compute, against the kernel's: the same decisions, heads shared
+    and odd numbers of keys among them (float32 both: 2^-16 of the largest)."""
+    for L, S, H, Hk, D, seed in ((5, 70, 4, 2, 32, 7), (90, 151, 8, 8, 16, 2 ** 63 + 5)):
+        q, kv = tokens((2, L, H * D), 'cuda', torch.float32, 0).requires_grad_(True), tokens((2, S, 2 * Hk * D), 'cuda', torch.float32, 1).requires_grad_(True)
+        go, word = tokens((2, L, H * D), 'cuda', torch.float32, 2), torch.full((1,), 3, dtype=torch.int64, device='cuda')
+        for w in (None, word):
+            o = autograd.CrossAttention.apply(q, kv, None, H, None, None, None, None, 0.3, seed, w)
+            f = autograd.attention_formula(q, kv, None, H, dropout_p=0.3, seed=seed, seed_word=w)
+            a = torch.autograd.grad(o, (q, kv), go, retain_graph=True)
+            b = torch.autograd.grad(o, (q, kv), go, create_graph=True)
+            for x, y in zip((o,) + a, (f,) + b):
+                assert float((x - y).abs().max()) <= 2.0 ** -16 * float(y.abs().max())
+            assert b[0].requires_grad and not a[0].requires_grad
