@@ -141,8 +141,7 @@ def _post_norm(norm, x, branch=None):
 def mha_tokens(q_in, k_in, v_in, w, b, out_proj, H, dropout_p=0.0, key_allowed=None):
     """Batch-first multi-head attention on small token sets with library GEMMs.
     q_in (B,L,E), k_in/v_in (B,S,E); key_allowed: optional bool (B,L,S) - query l attends only to the
-    keys s with key_allowed[b,l,s] (a row without any allowed key yields out_proj's bias on the GPU, NaN in
-    the torch formulation; callers drop it).
+    keys s with key_allowed[b,l,s] (a row without any allowed key yields out_proj's bias and no gradient).
     Returns (B,L,E)."""
     B, L, E = q_in.shape
     S = k_in.shape[1]
@@ -161,8 +160,12 @@ def mha_tokens(q_in, k_in, v_in, w, b, out_proj, H, dropout_p=0.0, key_allowed=N
     v = v.view(B, S, H, D).transpose(1, 2)
     sc = torch.matmul(q, k.transpose(-1, -2)).float()                      # (B,H,L,S)
     if key_allowed is not None:
-        sc = sc.masked_fill(~key_allowed.view(B, 1, L, S), float('-inf'))
+        key_allowed = key_allowed.view(B, 1, L, S)
+        some = key_allowed.any(-1, keepdim=True)                           # the other rows attend to every key, and then to none
+        sc = sc.masked_fill(~(key_allowed | ~some), float('-inf'))
     a = torch.softmax(sc, -1).to(v.dtype)
+    if key_allowed is not None:
+        a = a * some.to(a.dtype)
     if dropout_p > 0:
         a = F.dropout(a, dropout_p)
     o = torch.matmul(a, v).transpose(1, 2).reshape(B, L, E)

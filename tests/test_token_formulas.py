@@ -54,3 +54,27 @@ def test_formula_gradients_are_each_input_s_share():
     gx, none, gy = autograd._formula_grads(lambda x, c, y: x * c * y, (x, torch.tensor(3.0), y), (True, False, True), torch.ones(4).double())
     assert none is None and torch.equal(gx, 3 * y) and torch.equal(gy, 3 * x)
     assert torch.allclose(torch.autograd.grad(gx.sum(), x)[0], 6 * x)
+
+
+def test_tokens_without_an_allowed_key():
+    """`mha_tokens` in its torch formulation gives such a row the projection's bias and reaches no gradient through it, as on the GPU; the others
+    are as with the rows left out."""
+    from deepinteraction_amd.mmdet3d_plugin.models.utils import decoder_utils as du
+    torch.manual_seed(0)
+    m, H = du.MultiheadAttention(32, 4), 4
+    torch.nn.init.normal_(m.in_proj_bias), torch.nn.init.normal_(m.out_proj.bias)
+    allowed = torch.rand(2, 7, 7, generator=torch.Generator().manual_seed(1)) < 0.5
+    allowed[..., 0] = True
+    allowed[0, 2], allowed[1, 6] = False, False
+    some = allowed.any(-1)
+    grads = []
+    for mask in (allowed, allowed | ~some[..., None]):               # the second: those rows attend, and are dropped afterwards
+        x = randn(2, 7, 32, seed=3).requires_grad_(True)
+        y = du.mha_tokens(x, x, x, m.in_proj_weight, m.in_proj_bias, m.out_proj, H, 0.0, mask)
+        if mask is allowed:
+            assert torch.equal(y[~some], m.out_proj.bias.expand(2, 32))
+        kept = torch.where(some[..., None], y, torch.zeros_like(y))
+        m.zero_grad()
+        (kept * randn(2, 7, 32, seed=4)).sum().backward()
+        grads.append([kept.detach(), x.grad] + [p.grad.clone() for p in m.parameters()])
+    assert all(torch.allclose(a, b, rtol=0, atol=2.0 ** -20 * max(1.0, float(b.abs().max()))) for a, b in zip(*grads))
