@@ -339,18 +339,20 @@ class FrozenSwinFPN(_FrozenImageNet):
 
     # ------------------------------------------------------------------ forward
     def _ln(self, x, name):
-        if x.is_cuda and x.dtype != torch.float64:
-            from .... import ops
-            return ops.layernorm(x, self._p(name + '.weight'), self._p(name + '.bias'))
-        return F.layer_norm(x, x.shape[-1:], self._p(name + '.weight'), self._p(name + '.bias'), 1e-5)
+        from .... import ops
+        w, b = self._p(name + '.weight'), self._p(name + '.bias')
+        dt = ops.layernorm_type(x, None, w.dtype)
+        return F.layer_norm(x, x.shape[-1:], w, b, 1e-5) if dt is None else ops.layernorm(x, w, b, out_dtype=dt)
 
     def _add_ln(self, x, branch, name):
         """(x + branch, its norm) in one pass."""
-        if x.is_cuda and x.dtype != torch.float64:
-            from .... import ops
-            return ops.layernorm(x, self._p(name + '.weight'), self._p(name + '.bias'), branch, with_sum=True)[::-1]
-        x = x + branch
-        return x, self._ln(x, name)
+        from .... import ops
+        w, b = self._p(name + '.weight'), self._p(name + '.bias')
+        dt = ops.layernorm_type(x, branch, w.dtype)
+        if dt is None or torch.promote_types(x.dtype, branch.dtype) != x.dtype:
+            x = x + branch
+            return x, self._ln(x, name)
+        return ops.layernorm(x, w, b, branch, with_sum=True, out_dtype=dt)[::-1]
 
     def _region_mask(self, Hp, Wp, device):
         """(nW, 49, 49): 0 inside a region of the cyclically shifted map, -100 across regions (swin.py:195-217)."""

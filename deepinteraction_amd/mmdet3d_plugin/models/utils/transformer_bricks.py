@@ -13,9 +13,6 @@ from ....autograd import AddLayerNorm, MSDeformAttn, transformed
 from ....utils import param_key
 
 
-_NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
-
-
 def _only_a_layer_norm(norm):
     """Whether calling the module is its LayerNorm and nothing else: no hooks (its own or global ones), no forward of a subclass or of
     the instance."""
@@ -25,19 +22,11 @@ def _only_a_layer_norm(norm):
 
 
 def _norm_type(norm, x, branch):
-    """The type of `norm(x + branch)` where the LayerNorm kernels take it, None elsewhere: autocast evaluates the norm in float32
-    whatever its operands are; without it the operands' common type has to be the norm's own."""
-    if not (x.is_cuda and _only_a_layer_norm(norm) and norm.elementwise_affine and norm.bias is not None
-            and norm.normalized_shape == (x.shape[-1],) and x.shape[-1] <= ops.LAYERNORM_MAX_C
-            and (branch is None or branch.shape == x.shape) and not transformed(x, branch, norm.weight, norm.bias)):
+    """The type of `norm(x + branch)` where the LayerNorm kernels take it, None elsewhere."""
+    if not (_only_a_layer_norm(norm) and norm.elementwise_affine and norm.bias is not None and norm.weight.dtype == norm.bias.dtype
+            and norm.normalized_shape == (x.shape[-1],)) or transformed(x, branch, norm.weight, norm.bias):
         return None
-    halves = {t for t in (x.dtype, x.dtype if branch is None else branch.dtype, norm.weight.dtype) if t != torch.float32}
-    if len(halves) > 1 or not halves <= set(_NORM_TYPES) or norm.weight.dtype != norm.bias.dtype:
-        return None
-    if torch.is_autocast_enabled('cuda'):
-        return torch.float32
-    dt = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)
-    return dt if dt == norm.weight.dtype else None
+    return ops.layernorm_type(x, branch, norm.weight.dtype)
 
 
 def post_norm(norm, x, branch=None):

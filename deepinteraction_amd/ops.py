@@ -1149,6 +1149,20 @@ def _row_view(t, C):
 LAYERNORM_MAX_C = 16384
 
 
+def layernorm_type(x, branch, param_dtype):
+    """The type of torch's LayerNorm of x (+ branch) with parameters of `param_dtype`, where the kernels take the call - None elsewhere:
+    autocast evaluates the norm in float32 whatever its operands are; without it the operands' common type has to be the parameters'."""
+    if not (x.is_cuda and 1 <= x.shape[-1] <= LAYERNORM_MAX_C and (branch is None or branch.shape == x.shape)):
+        return None
+    dt = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)
+    halves = {t for t in (x.dtype, dt if branch is None else branch.dtype, param_dtype) if t != torch.float32}
+    if len(halves) > 1 or not halves <= set(_DT3):
+        return None
+    if torch.is_autocast_enabled('cuda'):
+        return torch.float32
+    return dt if dt == param_dtype else None
+
+
 def _layernorm_fwd(x, weight, bias, res, eps, with_sum, out_dtype, stats):
     _same_device(x, weight, bias, res)
     C = x.shape[-1] if x.dim() else 0

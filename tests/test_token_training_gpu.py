@@ -398,3 +398,30 @@ def test_the_formula_s_dropout_is_the_kernel_s():
             for x, y in zip((o,) + a, (f,) + b):
                 assert float((x - y).abs().max()) <= 2.0 ** -16 * float(y.abs().max())
             assert b[0].requires_grad and not a[0].requires_grad
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize('amp', [None, torch.float16, torch.bfloat16], ids=str)
+def test_the_image_branch_s_norms_keep_their_types(monkeypatch, dtype, amp):
+    """The Swin image branch with its norms in the kernels and as torch evaluates them, plain and under autocast (whose norms are float32): the
+    same types, and values as far apart as a dozen blocks' roundings leave them - a norm in the other type, or a sum carried in 16 bits,
+    doubles the count of those: 32 half steps of the largest value."""
+    from deepinteraction_amd.mmdet3d_plugin.models.detectors import image_glue
+    net = image_glue.FrozenSwinFPN(dtype=dtype)
+    net.load_mmdet_state(*net.synthetic_state(seed=1))
+    net = net.cuda()
+    img = tokens((2, 3, 64, 96), 'cuda', torch.float32, 0)
+
+    def run():
+        with torch.autocast('cuda', dtype=amp or torch.float16, enabled=amp is not None):
+            return net.stage_maps(img)
+    calls, real = [], ops.layernorm
+    monkeypatch.setattr(ops, 'layernorm', lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    got = run()
+    assert len(calls) >= 20 or {dtype, amp} == {torch.float16, torch.bfloat16}
+    monkeypatch.setattr(ops, 'layernorm_type', lambda *a: None)
+    want = run()
+    half = max(torch.finfo(t).eps for t in (dtype, amp or dtype)) / 2
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+        assert float((a.float() - b.float()).abs().max()) <= max(32 * half, 2.0 ** -14) * float(b.float().abs().max())
