@@ -3,6 +3,7 @@
 
 #include <stdlib.h>
 
+#include <exception>
 #include <vector>
 
 #include "di_common.h"
@@ -95,7 +96,7 @@ static hipError_t fill_by_kernel(hipGraph_t graph, hipGraphNode_t node) {
 
 }  // namespace di
 
-extern "C" long long di_graph_fill_by_kernels(void *graph, int replace) {
+extern "C" long long di_graph_fill_by_kernels(void *graph, int replace) try {
   hipGraph_t g = (hipGraph_t)graph;
   size_t n = 0;
   hipError_t e = graph == nullptr ? hipErrorInvalidValue : hipGraphGetNodes(g, nullptr, &n);
@@ -115,6 +116,9 @@ extern "C" long long di_graph_fill_by_kernels(void *graph, int replace) {
     return DI_ERR_LAUNCH;
   }
   return found;
+} catch (const std::exception &e) {                             // the lists of nodes: no memory
+  di::set_error("graph_fill_by_kernels: %s", e.what());
+  return DI_ERR_LAUNCH;
 }
 
 namespace di {

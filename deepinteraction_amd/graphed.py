@@ -493,6 +493,8 @@ class GraphedTrainingModule:
         _without_memsets(self.backward_graph)
 
     def __call__(self, *args):
+        if [t.shape for t in args] != [t.shape for t in self.args]:
+            raise ValueError(f'inputs of {[tuple(t.shape) for t in args]}, captured with {[tuple(t.shape) for t in self.args]}')
         return _Replayed.apply(self, *args, *self.parameters)
 
 

@@ -123,3 +123,10 @@ def test_a_replay_s_outputs_and_gradients(eager_cuda):
     with torch.no_grad():
         assert not g(torch.zeros(5, 3))[0].requires_grad
     assert not g.args[0].any()                                        # another input is copied into the captured one
+
+
+def test_inputs_of_other_shapes_are_refused(eager_cuda):
+    g = GraphedTrainingModule(Layer(), (torch.randn(5, 3),))
+    for bad in ((), (torch.randn(1, 3),), (torch.randn(5, 3), torch.randn(5, 3))):
+        with pytest.raises(ValueError):
+            g(*bad)
