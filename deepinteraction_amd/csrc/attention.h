@@ -203,7 +203,8 @@ __device__ __forceinline__ unsigned drop_pair(unsigned row, unsigned k4, bool se
   return second ? mix(x + 0x68bc21ebu) : x;
 }
 
-// n / d for 0 <= n < 2^31 by one multiplication (d fixed for the launch): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// n / d for 0 <= n < 2^31 by one multiplication (d fixed for the launch; T. Granlund and P. Montgomery, "Division by invariant integers
+// using multiplication", 1994): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
 // n / d = (mulhi(n, m) + n) >> s
 struct Div {
   unsigned d, m, s;

@@ -14,14 +14,18 @@
 // scores are formed once, and rows of few dims make the key blocks' sums small (rows x D floats per 128 - 256 keys); wide heads would
 // write more sums than the second pass over the keys costs.
 //
-// What bounds them, and what they measured:
-//   heads of 128 (2048 x 8192 x 16, bf16): gq 252 us = 818 TFLOP/s, the matrix cores; gk and gv 350 - 380 us = 720 - 790: a SIMD's two
-//     wavefronts hold 16 keys each, so every fragment of Q and go from LDS feeds one product (the fragments take half of LDS's cycles),
-//     and a quarter of the cycles waits for them and at the tiles' barriers
-//   heads of 64, four to a key head (4 x 511 x 4100, 2733, 1366, 0, bf16): gq 46 us, gk and gv 78: 264 workgroups for 256 CUs, one
-//     wavefront a SIMD - its own chain of product, exponential, product is the time of a tile
-//   heads of 16, one launch (200 x 32 400 x 8, float32: 100 us; half precision 2 samples: 66 us; 1200 x 60 x 112: 77 us): the vector unit
-//     (ten instructions and an exponential a pair), in float32 the matrix cores beside it
+// What bounds them, and what they measured (shares of the SIMDs' cycles from the counters of the final build):
+//   heads of 128 (2048 x 8192 x 16, bf16): gq 256 - 269 us = 770 - 805 TFLOP/s, gk and gv 356 - 375 us = 730 - 770: matrix cores 38 %, vector
+//     unit 32; gq has one wavefront a SIMD, gk and gv two that hold 16 keys each, so every fragment of Q and go from LDS feeds one product
+//     (LDS works in 53 % of the cycles) and the wavefronts wait 42 % of theirs for a unit to take their next instruction
+//   heads of 64, four to a key head (4 x 511 x 4100, 2733, 1366, 0, bf16): gq 47 us, gk and gv 79: 264 workgroups for 256 CUs, one
+//     wavefront a SIMD (1.15) - its own chain of product, exponential, product is the time of a tile
+//   heads of 16, one launch: 200 x 32 400 x 8, float32: 102 us, matrix cores 64 %, vector unit 24; half precision, 2 samples: 67 us, vector
+//     unit 62 %, and 1200 x 60 x 112: 78 us, 56 % (ten instructions and an exponential a pair)
+// Attention dropout, p = 0.1 (forward and backward): the hashes of a pair, formed in both directions - float32 200 x 32 400: 52 + 101 -> 62 +
+// 130 us; half precision, 2 samples: 41 + 71 -> 70 + 138; 1200 x 60 x 112: 31 + 68 -> 49 + 111.
+// Spilled registers: masked gk and gv of 16-bit heads of 64 (19, 48 bytes of scratch, at the bound of two wavefronts a SIMD; 1024 x 4096 x 8:
+// the whole backward 97 us with a (query, key) mask, 68 without) and float32 masked gq of 128 dims (4 of its accumulation registers).
 // Not taken: the products over a chunk's rows left for the next chunk, to hide behind its exponentials - the registers that this takes
 // cost the second wavefront of the SIMD (4 x 511 x .. of 64: 79 -> 110 us; heads of 128: 410 -> 433).
 #pragma once

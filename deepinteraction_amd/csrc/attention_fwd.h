@@ -13,14 +13,18 @@
 // taken from: the maximum, for float16 less 7 - with the 8 above, probabilities of up to 2^15 (65 504 is the type's largest), their rounding
 // stays relative down to 2^-21 of the largest and reaches zero at 2^-32, where the float32 sum beside them would still count them at 2^-25.
 //
-// What bounds it, and what it measured:
-//   heads of 128 and 64 (2048 x 8192 x 16 heads of 128, bf16: 172 us = 800 TFLOP/s, a large matrix product reaches 1085 on this card):
-//     the matrix cores, then the exponentials of the same wavefronts - both units have their own work, two wavefronts a SIMD share them
-//   heads of 16 (200 x 32 400 x 8, float32: 49 us = 68 TFLOP/s of 149, half precision 2 samples 37 us): a pair of row and key costs 32
-//     multiply-adds and an exponential, so the vector unit (5 instructions and the exponential a score) and, in float32, the matrix cores
-//     in turn.  Writing float32 operands as three bf16 parts would take the products to the 16-bit rate and put the splitting of every
-//     probability, six instructions, on the vector unit: no gain
+// What bounds it, and what it measured (shares of the SIMDs' cycles from the counters of the final build):
+//   heads of 128 and 64 (2048 x 8192 x 16 heads of 128, bf16: 180 us = 765 TFLOP/s, a large matrix product reaches 1085 on this card): the
+//     matrix cores work in 40 % of the cycles, the vector unit in 44, LDS in 40; two wavefronts a SIMD, each of which alternates products and
+//     exponentials, overlap them in part and wait 43 % of their time for a unit to take their next instruction
+//   heads of 16: a pair of row and key costs 32 multiply-adds, an exponential and five vector instructions.  Float32 (200 x 32 400 x 8, 49 us
+//     = 68 TFLOP/s of 149): matrix cores 53 %, vector unit 29, overlapped in part.  Half precision, 2 samples (37 us): vector unit 61 %,
+//     matrix cores 13.  Writing float32 operands as three bf16 parts would take the products of a tile from 256 to 96 cycles and the
+//     vector instructions from 160 to 256 (six more a probability): 416 -> 352 where nothing overlaps, a loss where everything does; not built
 //   single queries (16 samples of up to 32 768 keys x 8 key heads of 128, 1.07 GB): the memory, 190 us = 5.6 TB/s
+// Spilled registers: with masks and dropout the 16-bit kernels of 32 dims keep 2 - 6 and those of 128 dims 8 of their lanes' values in scratch
+// (12 - 36 bytes, at the bound of two wavefronts a SIMD); every other variant none.  1024 x 4096, 8 heads, bf16, with a (query, key) mask against
+// without: 32 dims 36.1 and 27.5 us, 64 (no spills) 37.9 and 30.2, 128 47.6 and 38.0 - the mask's own instructions in all three.
 #pragma once
 #include <type_traits>
 
