@@ -241,7 +241,9 @@ class CrossAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, seed_word=None):
         Ek = k.shape[-1] // 2
         ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
-        out, lse = ops.cross_attention_train_fwd(q, ks, vs, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, seed_word)
+        seed_word = ops._seed_word(q, dropout_p, seed_word)        # the backward's as well, whatever is registered by then
+        out, lse = ops.cross_attention_train_fwd(q, ks, vs, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed,
+                                                 False if seed_word is None else seed_word)
         ctx.save_for_backward(q, k, v, out, lse, key_lengths, key_mask, allowed, seed_word)
         ctx.args = (num_heads, scale, dropout_p, seed)
         return out
@@ -262,7 +264,7 @@ class CrossAttention(torch.autograd.Function):
         gq, gk, gv = ops.cross_attention_train_bwd(q, ks, vs, out, grad_out, lse, num_heads, scale, key_lengths, key_mask, allowed,
                                                    dropout_p, seed,
                                                    grads_kv=None if packed is None else (packed[..., :Ek], packed[..., Ek:]),
-                                                   seed_word=seed_word)
+                                                   seed_word=False if seed_word is None else seed_word)
         return (gq, gk if packed is None else packed, gv if packed is None else None) + (None,) * 8
 
 

@@ -1319,8 +1319,8 @@ def _attention(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropou
 
 
 def _seed_word(q, dropout_p, seed_word):
-    """The device word that a call with dropout adds to its seed: its own, the registered one, or None."""
-    if dropout_p == 0:
+    """The device word that a call with dropout adds to its seed: its own, the registered one, or None (also where its own is False)."""
+    if dropout_p == 0 or seed_word is False:
         return None
     own = seed_word is not None
     word = seed_word if own else _I2P_SEED_REF[0]
@@ -1347,10 +1347,7 @@ def _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dr
     ref = ctypes.addressof(t)
     ws = _attention_workspace('di_attention_fwd_workspace_floats', ref, q)
     args = (out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr())
-    if word is None:
-        _launch('attention_fwd', t.B, q, ref, *args)
-    else:
-        _launch('attention_fwd_seeded', t.B, q, ref, word.data_ptr(), *args)
+    _launch('attention_fwd_seeded', t.B, q, ref, 0 if word is None else word.data_ptr(), *args)
     return out, lse
 
 
@@ -1369,7 +1366,7 @@ def cross_attention_train_fwd(q, k, v, num_heads, scale=None, key_lengths=None, 
                               seed_word=None):
     """`cross_attention` with the per-query log2-sum-exp2 kept for the backward: (out, lse (B, heads, L)).  dropout_p: dropout of the
     attention weights, decided per (query, head, key) by a counter-based hash of `seed` plus `seed_word` (an int64 on the device, read
-    when the launch runs; None: the one of `set_i2p_seed_tensor`, if any) that the backward regenerates; p is rounded to a multiple
+    when the launch runs; None: the one of `set_i2p_seed_tensor`, if any; False: none) that the backward regenerates; p is rounded to a multiple
     of 2^-16."""
     return _attention_fwd(q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, True, seed_word)
 
@@ -1400,10 +1397,7 @@ def cross_attention_train_bwd(q, k, v, out, grad_out, lse, num_heads, scale=None
     ws = _attention_workspace('di_attention_bwd_workspace_floats', ref, q)
     args = (out.data_ptr(), lse.data_ptr(), go.data_ptr(), go_bs, go_rs, gq.data_ptr(), gk.data_ptr(), *k_strides, gv.data_ptr(), *v_strides,
             0 if ws is None else ws.data_ptr())
-    if word is None:
-        _launch('attention_bwd', t.B, q, ref, *args)
-    else:
-        _launch('attention_bwd_seeded', t.B, q, ref, word.data_ptr(), *args)
+    _launch('attention_bwd_seeded', t.B, q, ref, 0 if word is None else word.data_ptr(), *args)
     return gq, gk, gv
 
 

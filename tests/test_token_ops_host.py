@@ -179,3 +179,4 @@ def test_seed_words():
     for bad in (word.int(), torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int64, device='meta')):
         with pytest.raises(ValueError):
             ops._seed_word(q, 0.5, bad)
+    assert ops._seed_word(q, 0.5, False) is None

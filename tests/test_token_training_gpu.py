@@ -425,3 +425,18 @@ def test_the_image_branch_s_norms_keep_their_types(monkeypatch, dtype, amp):
     for a, b in zip(got, want):
         assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
         assert float((a.float() - b.float()).abs().max()) <= max(32 * half, 2.0 ** -14) * float(b.float().abs().max())
+
+
+def test_a_word_registered_later_does_not_reach_the_backward():
+    q, kv = tokens((1, 30, 64), 'cuda', torch.float32, 0).requires_grad_(True), tokens((1, 70, 128), 'cuda', torch.float32, 1)
+    word = torch.full((1,), 41, dtype=torch.int64, device='cuda')
+    grads = []
+    for registered in (None, word):
+        torch.manual_seed(3)
+        o = autograd.cross_attention(q, kv, None, 4, dropout_p=0.5)
+        ops.set_i2p_seed_tensor(registered)
+        try:
+            grads.append(torch.autograd.grad(o, q, torch.ones_like(o))[0])
+        finally:
+            ops.set_i2p_seed_tensor(None)
+    assert torch.equal(*grads)
