@@ -180,10 +180,10 @@ def _formula_grads(formula, inputs, needs, grad_out):
 
 class AddLayerNorm(torch.autograd.Function):
     """y = LayerNorm(x + res) (csrc/layernorm.hip, layernorm_bwd.hip; res may be None), or (y, x + res) with `with_sum`: the post-norm
-    and pre-norm steps of a training forward.  x and res are kept, not their sum; with_sum keeps the sum instead."""
+    and pre-norm steps of a training forward.  x and res are kept, not their sum; with_sum keeps the sum instead.  (Neither this Function nor
+    CrossAttention calls anything that autocast changes: without custom_fwd / custom_bwd a forward and backward take 10 us of the host less.)"""
 
     @staticmethod
-    @_fwd
     def forward(ctx, x, res, weight, bias, eps, out_dtype, with_sum):
         y, total, mean, rstd = ops.layernorm_train_fwd(x, weight, bias, res, eps, with_sum, out_dtype)
         ctx.save_for_backward(x if total is None else total, res if total is None else None, weight, mean, rstd)
@@ -213,7 +213,6 @@ class AddLayerNorm(torch.autograd.Function):
         return gx.to(xt) if need[0] and gx is not None else None, gres, gw, gb, None, None, None
 
     @staticmethod
-    @_bwd
     def backward(ctx, gy, gsum=None):
         if torch.is_grad_enabled():
             return AddLayerNorm._formula_backward(ctx, gy, gsum)
@@ -237,7 +236,6 @@ class CrossAttention(torch.autograd.Function):
     packed gradient.  Gradients: q, k, v; lengths and masks have none."""
 
     @staticmethod
-    @_fwd
     def forward(ctx, q, k, v, num_heads, scale, key_lengths, key_mask, allowed, dropout_p, seed, seed_word=None):
         Ek = k.shape[-1] // 2
         ks, vs = (k[..., :Ek], k[..., Ek:]) if v is None else (k, v)
@@ -249,7 +247,6 @@ class CrossAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @_bwd
     def backward(ctx, grad_out):
         q, k, v, out, lse, key_lengths, key_mask, allowed, seed_word = ctx.saved_tensors
         num_heads, scale, dropout_p, seed = ctx.args

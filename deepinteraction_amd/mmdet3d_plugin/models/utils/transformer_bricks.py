@@ -23,10 +23,12 @@ def _only_a_layer_norm(norm):
 
 def _norm_type(norm, x, branch):
     """The type of `norm(x + branch)` where the LayerNorm kernels take it, None elsewhere."""
-    if not (_only_a_layer_norm(norm) and norm.elementwise_affine and norm.bias is not None and norm.weight.dtype == norm.bias.dtype
-            and norm.normalized_shape == (x.shape[-1],)) or transformed(x, branch, norm.weight, norm.bias):
+    if not (x.is_cuda and _only_a_layer_norm(norm)):
         return None
-    return ops.layernorm_type(x, branch, norm.weight.dtype)
+    w, b = norm.weight, norm.bias
+    if w is None or b is None or w.dtype != b.dtype or norm.normalized_shape != (x.shape[-1],) or transformed(x, branch, w, b):
+        return None
+    return ops.layernorm_type(x, branch, w.dtype)
 
 
 def post_norm(norm, x, branch=None):

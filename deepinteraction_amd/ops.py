@@ -8,6 +8,7 @@ physically (n,H,W,C) - the layout the kernels are written for.
 No CPU implementation lives here; CPU tensors are rejected.
 """
 import ctypes
+import functools
 
 import collections
 import math
@@ -1154,12 +1155,14 @@ def layernorm_type(x, branch, param_dtype):
     autocast evaluates the norm in float32 whatever its operands are; without it the operands' common type has to be the parameters'."""
     if not (x.is_cuda and 1 <= x.shape[-1] <= LAYERNORM_MAX_C and (branch is None or branch.shape == x.shape)):
         return None
-    dt = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)
-    halves = {t for t in (x.dtype, dt if branch is None else branch.dtype, param_dtype) if t != torch.float32}
-    if len(halves) > 1 or not halves <= set(_DT3):
-        return None
+    xt, bt = x.dtype, x.dtype if branch is None else branch.dtype
+    if not (xt == bt == param_dtype and xt in _DT3):              # otherwise float32 and one 16-bit type
+        halves = {t for t in (xt, bt, param_dtype) if t != torch.float32}
+        if len(halves) > 1 or not halves <= _DT3.keys():
+            return None
     if torch.is_autocast_enabled('cuda'):
         return torch.float32
+    dt = xt if xt == bt else torch.float32
     return dt if dt == param_dtype else None
 
 
@@ -1205,6 +1208,12 @@ def layernorm_train_fwd(x, weight, bias, res=None, eps=1e-5, with_sum=False, out
     return _layernorm_fwd(x, weight, bias, res, eps, with_sum, out_dtype, True)
 
 
+@functools.lru_cache(maxsize=4096)
+def _layernorm_bwd_floats(device, rows, C):
+    with torch.cuda.device(device):
+        return max(4, _lib.lib().di_layernorm_bwd_workspace_floats(rows, C))
+
+
 def layernorm_train_bwd(grad_y, x, weight, mean, rstd, res=None, grad_sum=None, grad_dtype=None):
     """Gradients of `layernorm_train_fwd`: (grad_x, grad_res, grad_weight, grad_bias).  x and res are what the forward read; where
     it returned the sum, x = that sum and res = None (grad_x is then the gradient of both).  grad_sum: gradient of the returned
@@ -1238,7 +1247,7 @@ def layernorm_train_bwd(grad_y, x, weight, mean, rstd, res=None, grad_sum=None, 
     rv, rs = (None, 0) if res is None else _row_view(res, C)
     w = weight.contiguous()
     ptr = lambda t: 0 if t is None else t.data_ptr()
-    ws = x.new_empty(max(4, _on_device(x, lambda: _lib.lib().di_layernorm_bwd_workspace_floats(rows, C))), dtype=torch.float32)
+    ws = x.new_empty(_layernorm_bwd_floats(x.get_device(), rows, C), dtype=torch.float32)
     _launch('layernorm_bwd', rows, x, gv.data_ptr(), gs, codes[0], ptr(sv), ss, xv.data_ptr(), xs, codes[1], ptr(rv), rs, codes[2],
             w.data_ptr(), codes[3], mean.data_ptr(), rstd.data_ptr(), gx.data_ptr(), codes[4], 0 if gres is gx else ptr(gres),
             gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), rows, C)
